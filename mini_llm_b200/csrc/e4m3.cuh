@@ -1,0 +1,83 @@
+// The cache in 8 bits: e4m3 codes (sign, 4 bits of exponent, 3 of fraction, up to 448; no infinity) and a 32-bit scale, a power
+// of two, for each block of 16 positions and key/value head; an entry is code * scale.
+//   pages   [pages, kv_heads, page, size] bytes, page and size multiples of 16
+//   scales  [pages, kv_heads, page / 16] fp32
+// A head's positions of a page lie side by side, so that a block is one contiguous piece of 16 * size bytes.
+#pragma once
+
+#include "common.cuh"
+
+constexpr int E4M3_BLOCK = 16;                 // positions that share a scale
+constexpr float E4M3_TOP = 448.0f;             // the largest code
+constexpr int E4M3_LEAST_EXPONENT = -64;       // of a scale
+
+// Two numbers to two codes, nearest, ties to even; beyond 448 to 448, what is no number to the code that is none.
+__device__ __forceinline__ uint32_t e4m3_pair(float low, float high) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
+    return r;
+}
+
+// Two codes to two 16-bit floats (every code is one exactly).
+__device__ __forceinline__ uint32_t e4m3_to_half2(uint16_t pair) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(pair));
+    return r;
+}
+__device__ __forceinline__ void e4m3_to_half2(uint32_t four, uint32_t& low, uint32_t& high) {
+    low = e4m3_to_half2((uint16_t)(four & 0xffffu));
+    high = e4m3_to_half2((uint16_t)(four >> 16));
+}
+
+__device__ __forceinline__ float2 half2_to_floats(uint32_t h) {
+    float2 r;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(h));
+    return r;
+}
+
+// Two numbers to two 16-bit floats, nearest.
+__device__ __forceinline__ uint32_t half2_of(float low, float high) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    return r;
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }     // -126 <= e <= 127
+__device__ __forceinline__ int exponent_of(float power) { return ((__float_as_int(power) >> 23) & 255) - 127; }
+
+// 2^x by the hardware (about 2 ulp).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// cap * tanh(x / cap) = cap * (1 - 2 / (1 + e^(2x / cap))): two of the hardware's approximations with an error of some 2^-22 of the
+// cap, where its approximate tanh has 2^-11: of a cap of 50 that would be 2.4 % of a weight.
+__device__ __forceinline__ float capped(float x, float cap, float two_log2e_over_cap) {
+    const float e = exp2_fast(x * two_log2e_over_cap);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return cap - 2.0f * cap * r;
+}
+
+// What attention over the cache gets.  An entry is a request's tokens of this step: rows item_offset .. + item_count of q, at
+// positions item_start, item_start + 1, ...; entries without tokens are allowed.
+struct E4m3Attention {
+    void* out;                     // [rows, heads * vdim]
+    long ld_out;
+    const void* q;                 // [rows, heads * dim]
+    long ld_q;
+    const uint8_t *k_pages, *v_pages;
+    const float *k_scales, *v_scales;
+    const int* block_table;        // [entries, max_blocks]
+    int max_blocks, n_pages, page;
+    const int *item_offset, *item_count, *item_start;
+    int n_items;
+    int n_heads, n_kv_heads, dim, vdim;
+    float scale, cap;              // cap 0: none
+    int window;                    // 0: all keys
+    float* partial;                // results of parts, and how many of a result's parts have arrived (zero between launches)
+    int* counters;
+    int* status;                   // where a bounded wait that ran out leaves its code
+};

@@ -46,6 +46,7 @@ LIBRARIES = {
     "streams": "stream_kernels.cu",
     "unit": "recurrent_unit_kernels.cu",
     "token": "token_kernels.cu",
+    "e4m3": "e4m3_cache.cu",
 }
 
 _lock = threading.Lock()

@@ -1887,3 +1887,210 @@ def add_normed_norm(hidden, y, gain, eps, normed, next_gain, next_eps):
     _add_normed_norm(hidden.data_ptr(), y.data_ptr(), gain.data_ptr(), float(eps), normed.data_ptr(), next_gain.data_ptr(), float(next_eps),
                      width, n, dtype_code(normed.dtype), _stream())
     return hidden
+
+
+# ---- a cache in 8 bits ---------------------------------------------------------------------------
+#
+# Keys and values as e4m3 codes (torch.float8_e4m3fn) in pages [pages, kv_heads, page, size], with a 32-bit scale, a power of
+# two, for each block of 16 positions and key/value head in scales [pages, kv_heads, page / 16]: an entry is code * scale.
+
+E4M3_BLOCK = 16
+E4M3_STEP_SIZES = 128          # entries of a key or value up to which the kernel for single tokens takes them
+
+
+class _E4m3Attention(ctypes.Structure):
+    _fields_ = [("out", P), ("ld_out", L), ("q", P), ("ld_q", L), ("k_pages", P), ("v_pages", P), ("k_scales", P), ("v_scales", P),
+                ("block_table", P), ("max_blocks", I), ("n_pages", I), ("page", I), ("item_offset", P), ("item_count", P),
+                ("item_start", P), ("n_items", I), ("n_heads", I), ("n_kv_heads", I), ("dim", I), ("vdim", I), ("scale", F), ("cap", F),
+                ("window", I), ("partial", P), ("counters", P), ("status", P)]
+
+
+_e4m3_store = Function("e4m3", "mllm_e4m3_store", [P, L, P, L, I, I, I, I, I, I, I, P, ctypes.c_double, P, P, P, I, I, I, P, P, P, P, I, I, I, P])
+_e4m3_plain = Function("e4m3", "mllm_e4m3_attention_plain", [ctypes.POINTER(_E4m3Attention), I, I, P])
+_e4m3_step = Function("e4m3", "mllm_e4m3_attention_step", [ctypes.POINTER(_E4m3Attention), I, P])
+
+_sm_counts = {}
+
+
+def _sm_count(device) -> int:
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if index not in _sm_counts:
+        _sm_counts[index] = torch.cuda.get_device_properties(index).multi_processor_count
+    return _sm_counts[index]
+
+
+def e4m3_sizes_take(dim, vdim, page_size) -> bool:
+    """Whether a cache in 8 bits takes the sizes: keys and values of 16 to 256 entries and pages of positions, all multiples of 16."""
+    return all(n % 16 == 0 and n > 0 for n in (dim, vdim, page_size)) and dim <= 256 and vdim <= 256
+
+
+def _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table):
+    """The pages' sizes: (pages, kv_heads, page, dim, vdim)."""
+    for name, pages, scales in (("k", k_pages, k_scales), ("v", v_pages, v_scales)):
+        _check(pages, f"{who}.{name}_pages", torch.float8_e4m3fn, 4)
+        _check(scales, f"{who}.{name}_scales", torch.float32, 3)
+        if not pages.is_contiguous() or not scales.is_contiguous() or pages.data_ptr() % 16 != 0:
+            raise KernelError(f"{who}: pages and scales must be contiguous, pages on a 16-byte boundary")
+    n_pages, kv_heads, page, dim = k_pages.shape
+    vdim = v_pages.shape[3]
+    if tuple(v_pages.shape[:3]) != (n_pages, kv_heads, page):
+        raise KernelError(f"{who}: keys {tuple(k_pages.shape)} and values {tuple(v_pages.shape)} are not of the same pages")
+    if not e4m3_sizes_take(dim, vdim, page):
+        raise KernelError(f"{who} does not take heads of {dim} and {vdim} entries in pages of {page} (multiples of 16, heads up to 256)")
+    if tuple(k_scales.shape) != (n_pages, kv_heads, page // E4M3_BLOCK) or k_scales.shape != v_scales.shape:
+        raise KernelError(f"{who}: scales must be [pages, kv_heads, page / {E4M3_BLOCK}]")
+    _check(block_table, f"{who}.block_table", torch.int32, 2)
+    if not block_table.is_contiguous():
+        raise KernelError(f"{who}: the block table must be contiguous")
+    return n_pages, kv_heads, page, dim, vdim
+
+
+def _check_same_device(who, first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise KernelError(f"{who}: tensors lie on {first.device} and {t.device}")
+
+
+def _rows_of_sixteen_bytes(t, who):
+    size = t.element_size()
+    if t.data_ptr() % 16 != 0 or (t.shape[0] > 1 and t.stride(0) * size % 16 != 0):
+        raise KernelError(f"{who}: rows must begin on 16-byte boundaries")
+
+
+def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, positions, token_item,
+               block_table, k_pages, v_pages, k_scales, v_scales, writes=True):
+    """Append a step's keys and values to a cache in 8 bits, with the rotation of queries and keys on the way.
+
+    Rows of ``qkv`` (fp32 or bf16 [T, columns]) hold [q | k | v], k from column ``k_off``, v from ``v_off``.  The first ``rot_dims``
+    entries of every query and key head turn in interleaved pairs by position * ``inv_freq`` [rot_dims / 2] (float64; None without
+    turned entries), cosine and sine times ``amplitude``.  The turned queries go to ``q_out`` [T, heads * dim] (None: they are
+    not wanted); ``qkv`` stays as it is.  ``writes=False``: queries only.
+
+    Row t goes to position ``positions[t]`` of the request in row ``token_item[t]`` of the block table.  A request's rows stand side by
+    side at positions that grow by one; a row at a negative position, or whose page the table does not name (an index
+    outside the pages, a column outside the table), is stored nowhere.  The scale of a block of 16 positions is the least power of two
+    s >= 2^-64 with n <= (448 s)^2 for all its rows so far, n being x^2 + y^2 of a pair that turns (times ``amplitude``^2; a turn
+    keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
+    row that begins a block begins it anew, whatever was there.  A key or value head with an n that is not finite is stored as
+    NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes."""
+    _check(qkv, "e4m3_store.qkv", None, 2)
+    n = qkv.shape[0]
+    if min(heads, kv_heads) <= 0 or dim % 16 != 0 or vdim % 16 != 0 or not 0 < dim <= 256 or not 0 < vdim <= 256:
+        raise KernelError(f"e4m3_store does not take heads of {dim} and {vdim} entries (multiples of 16 up to 256)")
+    if rot_dims < 0 or rot_dims % 2 != 0 or rot_dims > dim:
+        raise KernelError(f"e4m3_store: {rot_dims} turned entries do not fit a head of {dim}")
+    if min(k_off, v_off) < 0 or max(heads * dim, k_off + kv_heads * dim, v_off + kv_heads * vdim) > qkv.shape[1] or k_off % 8 or v_off % 8:
+        raise KernelError("e4m3_store: the columns do not hold queries, keys and values, or are not multiples of 8")
+    dtype = dtype_code(qkv.dtype)
+    _rows_of_sixteen_bytes(qkv, "e4m3_store.qkv")
+    if rot_dims:
+        _check(inv_freq, "e4m3_store.inv_freq", torch.float64, 1)
+        if inv_freq.shape[0] < rot_dims // 2:
+            raise KernelError("e4m3_store: fewer frequencies than turned pairs")
+    _check(positions, "e4m3_store.positions", torch.int32, 1)
+    _check(token_item, "e4m3_store.token_item", torch.int32, 1)
+    if positions.shape[0] < n or token_item.shape[0] < n:
+        raise KernelError("e4m3_store: fewer positions or entries than rows")
+    _check_same_device("e4m3_store", qkv, q_out, inv_freq if rot_dims else None, positions, token_item)
+    if q_out is not None:
+        _check(q_out, "e4m3_store.q_out", qkv.dtype, 2)
+        if q_out.shape[0] != n or q_out.shape[1] != heads * dim:
+            raise KernelError("e4m3_store: q_out does not have heads * dim columns")
+        _rows_of_sixteen_bytes(q_out, "e4m3_store.q_out")
+    n_pages = page = max_blocks = 0
+    if writes:
+        n_pages, held_heads, page, held_dim, held_vdim = _check_e4m3_pages("e4m3_store", k_pages, v_pages, k_scales, v_scales, block_table)
+        if (held_heads, held_dim, held_vdim) != (kv_heads, dim, vdim):
+            raise KernelError("e4m3_store: the pages hold heads of another number or size")
+        max_blocks = block_table.shape[1]
+        _check_same_device("e4m3_store", qkv, k_pages, v_pages, k_scales, v_scales, block_table)
+    with torch.cuda.device(qkv.device):
+        _e4m3_store(_ptr(q_out), q_out.stride(0) if q_out is not None else 0, qkv.data_ptr(), qkv.stride(0), k_off, v_off, heads, kv_heads,
+                    dim, vdim, rot_dims, inv_freq.data_ptr() if rot_dims else None, float(amplitude), positions.data_ptr(),
+                    token_item.data_ptr(), block_table.data_ptr() if writes else None, max_blocks, n_pages, page,
+                    k_pages.data_ptr() if writes else None, v_pages.data_ptr() if writes else None,
+                    k_scales.data_ptr() if writes else None, v_scales.data_ptr() if writes else None, n, dtype,
+                    _sm_count(qkv.device), _stream())
+    return q_out
+
+
+def _padded_64(n) -> int:
+    return -(-n // 64) * 64
+
+
+class E4m3Workspace:
+    """What ``e4m3_attention`` needs beside its operands for values of up to ``vdim`` entries: 32-bit results of parts, counters of arrived
+    parts (zero between launches) and a status word (0; a kernel that gives up a bounded wait leaves a code there, and its
+    result is invalid).  Calls that may run at the same time need one each."""
+
+    def __init__(self, device, vdim: int):
+        self.vdim = int(vdim)
+        n_sms = _sm_count(torch.device(device))
+        self.partial = torch.empty(2 * n_sms * 256 * (_padded_64(self.vdim) + 2), dtype=torch.float32, device=device)
+        self.counters = torch.zeros(4 * n_sms, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def reset(self) -> None:
+        """After a kernel gave up: counters and status start over."""
+        self.counters.zero_()
+        self.status.zero_()
+
+
+def e4m3_workspace(device, vdim: int) -> E4m3Workspace:
+    return E4m3Workspace(device, vdim)
+
+
+def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start, heads, kv_heads, scale,
+                   cap=0.0, window=0, longest=None, singles=True, workspace=None, plain=False):
+    """Causal attention over a cache in 8 bits.  Entry i of the step: rows ``item_offset[i]`` .. + ``item_count[i]`` of ``q`` (fp32 or bf16
+    [T, heads * dim]) and ``out`` [T, heads * vdim], at positions ``item_start[i]``, ... of the request in row i of the block table, whose
+    keys and values are stored up to there; entries have rows of their own, and rows of no entry stay as they are.  score =
+    q . k * ``scale``, with ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if
+    given; softmax and the weighted sum in 32 bits; query head h reads key/value head h // (heads / kv_heads).  A row that sees no key (a
+    negative position) is zero; pages that the table does not name are not seen.
+
+    ``longest``: the most tokens of an entry, where the caller knows (1: a step of single tokens); ``singles``: whether some entry may
+    bring one token.  ``workspace`` (``e4m3_workspace``) is needed but with ``plain``: the kernel of every size and type, which 32-bit
+    queries, and heads of more than 128 entries, take anyway."""
+    who = "e4m3_attention"
+    n_pages, held_heads, page, dim, vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table)
+    _check(q, f"{who}.q", None, 2)
+    _check(out, f"{who}.out", q.dtype, 2)
+    dtype = dtype_code(q.dtype)
+    if kv_heads != held_heads or heads <= 0 or heads % kv_heads != 0:
+        raise KernelError(f"{who}: {heads} heads over {kv_heads} key/value heads, pages hold {held_heads}")
+    if q.shape[1] != heads * dim or out.shape[0] != q.shape[0] or out.shape[1] != heads * vdim:
+        raise KernelError(f"{who}: q / out do not have heads * size columns")
+    _rows_of_sixteen_bytes(q, f"{who}.q")
+    _rows_of_sixteen_bytes(out, f"{who}.out")
+    n_items = block_table.shape[0]
+    for name, t in (("item_offset", item_offset), ("item_count", item_count), ("item_start", item_start)):
+        _check(t, f"{who}.{name}", torch.int32, 1)
+        n_items = min(n_items, t.shape[0])
+    if any(t.shape[0] > n_items for t in (item_offset, item_count, item_start)):
+        raise KernelError(f"{who}: offsets, counts and starts of the entries, and rows of the block table, differ in number")
+    if window < 0 or cap < 0:
+        raise KernelError(f"{who}: a window and a cap are positive, or 0 for none")
+    _check_same_device(who, q, out, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start)
+    fast = not plain and q.dtype == torch.bfloat16 and max(dim, vdim) <= E4M3_STEP_SIZES
+    if fast and workspace is None:
+        raise KernelError(f"{who}: a workspace is needed (e4m3_workspace)")
+    if fast:
+        _check_same_device(who, q, workspace.partial)
+        if _padded_64(vdim) > _padded_64(workspace.vdim):
+            raise KernelError(f"{who}: the workspace is for values of {workspace.vdim} entries, not {vdim}")
+    params = _E4m3Attention()
+    params.out, params.ld_out, params.q, params.ld_q = out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0)
+    params.k_pages, params.v_pages, params.k_scales, params.v_scales = (t.data_ptr() for t in (k_pages, v_pages, k_scales, v_scales))
+    params.block_table, params.max_blocks, params.n_pages, params.page = block_table.data_ptr(), block_table.shape[1], n_pages, page
+    params.item_offset, params.item_count, params.item_start = (t.data_ptr() for t in (item_offset, item_count, item_start))
+    params.n_items, params.n_heads, params.n_kv_heads, params.dim, params.vdim = n_items, heads, kv_heads, dim, vdim
+    params.scale, params.cap, params.window = float(scale), float(cap or 0.0), int(window or 0)
+    if fast:
+        params.partial, params.counters, params.status = (t.data_ptr() for t in (workspace.partial, workspace.counters, workspace.status))
+    with torch.cuda.device(q.device):
+        if not fast or longest != 1:
+            _e4m3_plain(ctypes.byref(params), q.shape[0], dtype, _stream())
+            return out
+        _e4m3_step(ctypes.byref(params), _sm_count(q.device), _stream())
+    return out
