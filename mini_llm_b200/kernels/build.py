@@ -47,6 +47,7 @@ LIBRARIES = {
     "unit": "recurrent_unit_kernels.cu",
     "token": "token_kernels.cu",
     "e4m3": "e4m3_cache.cu",
+    "e4m3_tiles": "e4m3_attention_tcgen05.cu",
 }
 
 _lock = threading.Lock()

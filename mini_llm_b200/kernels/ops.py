@@ -1909,6 +1909,8 @@ _e4m3_store = Function("e4m3", "mllm_e4m3_store", [P, L, P, L, I, I, I, I, I, I,
 _e4m3_plain = Function("e4m3", "mllm_e4m3_attention_plain", [ctypes.POINTER(_E4m3Attention), I, I, P])
 _e4m3_step = Function("e4m3", "mllm_e4m3_attention_step", [ctypes.POINTER(_E4m3Attention), I, P])
 
+_e4m3_tiles = Function("e4m3_tiles", "mllm_e4m3_tiles_attention", [ctypes.POINTER(_E4m3Attention), I, I, P, P])
+
 _sm_counts = {}
 
 
@@ -2027,7 +2029,7 @@ class E4m3Workspace:
         self.vdim = int(vdim)
         n_sms = _sm_count(torch.device(device))
         self.partial = torch.empty(2 * n_sms * 256 * (_padded_64(self.vdim) + 2), dtype=torch.float32, device=device)
-        self.counters = torch.zeros(4 * n_sms, dtype=torch.int32, device=device)
+        self.counters = torch.zeros(4 * n_sms + 2, dtype=torch.int32, device=device)     # (the last two: the tiles' work counter)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
 
     def reset(self) -> None:
@@ -2069,8 +2071,8 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
         n_items = min(n_items, t.shape[0])
     if any(t.shape[0] > n_items for t in (item_offset, item_count, item_start)):
         raise KernelError(f"{who}: offsets, counts and starts of the entries, and rows of the block table, differ in number")
-    if window < 0 or cap < 0:
-        raise KernelError(f"{who}: a window and a cap are positive, or 0 for none")
+    if not (window >= 0 and cap >= 0 and scale >= 0):
+        raise KernelError(f"{who}: a window and a cap are positive, or 0 for none, and no scale is negative")
     _check_same_device(who, q, out, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start)
     fast = not plain and q.dtype == torch.bfloat16 and max(dim, vdim) <= E4M3_STEP_SIZES
     if fast and workspace is None:
@@ -2089,8 +2091,12 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
     if fast:
         params.partial, params.counters, params.status = (t.data_ptr() for t in (workspace.partial, workspace.counters, workspace.status))
     with torch.cuda.device(q.device):
-        if not fast or longest != 1:
+        if not fast:
             _e4m3_plain(ctypes.byref(params), q.shape[0], dtype, _stream())
             return out
-        _e4m3_step(ctypes.byref(params), _sm_count(q.device), _stream())
+        n_sms, stream = _sm_count(q.device), _stream()
+        if longest != 1:
+            _e4m3_tiles(ctypes.byref(params), q.shape[0], n_sms, params.counters + 4 * (workspace.counters.shape[0] - 2), stream)
+        if longest == 1 or singles:
+            _e4m3_step(ctypes.byref(params), n_sms, stream)
     return out

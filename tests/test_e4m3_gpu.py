@@ -331,3 +331,25 @@ def test_plain_attention(heads, kv_heads, dim, vdim, page, dtype):
     for cap, window in ((0.0, 0), (10.0, 33)):
         got = attend(pool, table, entries, q, heads, vdim, scale, dtype, cap=cap, window=window, plain=True)
         check_attention(got, q, pool, table, entries, heads, scale, dtype, cap, window)
+
+
+PORTIONS = [
+    [(2, 0)], [(100, 0)], [(128, 0)], [(129, 3)], [(300, 57)], [(256, 1000), (5, 127)], [(1, 40), (17, 128), (0, 9), (1, 0), (260, 0), (2, 511)],
+    [(600, 0), (1, 255), (257, 255)], [(33, 2000)],
+]
+
+
+@pytest.mark.parametrize("cap, window", [(0.0, 0), (20.0, 0), (0.0, 100), (5.0, 1), (0.0, 300)])
+@pytest.mark.parametrize("shapes", PORTIONS)
+@pytest.mark.parametrize("heads, kv_heads, dim, vdim, page", [(2, 2, 64, 64, 64), (4, 1, 128, 128, 16), (2, 1, 96, 48, 48), (3, 3, 16, 112, 128), (2, 1, 32, 16, 16)])
+def test_attention_of_portions(heads, kv_heads, dim, vdim, page, shapes, cap, window):
+    from mini_llm_b200.kernels import ops
+    rng = np.random.default_rng(heads + dim + len(shapes))
+    pool, table = filled_pool(rng, [max(1, count + start) for count, start in shapes], kv_heads, page, dim, vdim)
+    entries = laid_out(shapes)
+    q = rows_of(rng, entries[-1][0] + entries[-1][1] + 3, heads * dim, torch.bfloat16)
+    scale = 0.5 * dim ** -0.5
+    workspace = ops.e4m3_workspace("cuda", vdim)
+    got = attend(pool, table, entries, q, heads, vdim, scale, cap=cap, window=window, workspace=workspace)
+    check_attention(got, q, pool, table, entries, heads, scale, torch.bfloat16, cap, window)
+    assert int(workspace.status) == 0 and int(workspace.counters.abs().sum()) == 0
