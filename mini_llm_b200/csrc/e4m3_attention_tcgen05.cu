@@ -1,11 +1,11 @@
 // Attention of prompt portions over the 8-bit cache (e4m3.cuh) on the fifth-generation tensor cores.
 //
-// A CTA takes 256 consecutive tokens of an entry (a "unit": two tiles of 128 rows) and one head, and walks the keys up to the
-// unit's last position in blocks of 128, or a part of them:
+// A unit is 256 consecutive tokens of an entry (two tiles of 128 rows) and one head; a CTA walks the keys up to the unit's last
+// position in blocks of 128:
 //   converter warps  read a block's codes, page by page, and leave them as 16-bit floats in shared memory, swizzled like a TMA tile
 //                    (every code is one exactly; the scales stay outside); both tiles use them;
 //   MMA warp         S = Q K^T with tcgen05.mma into tensor memory, then O += P V, P from tensor memory;
-//   softmax warps    a thread a row: reads S, applies scale, cap and mask, and writes P over S as 16-bit floats.
+//   softmax warps    two threads a row, each with 64 of a block's columns: read S, apply scale, cap and mask, write P as 16-bit floats.
 // While one tile's softmax runs the other's products do.  Scales cost nothing an entry: a block of 16 keys has one factor for its scores, and
 // its values' scale 2^t goes into the exponent, p = 2^(s + t - m + 7), with the sum of the weights getting p / 2^t; p keeps the 11 bits of a
 // 16-bit float however far apart the scales lie.  Queries are scaled by a power of two to lie below 2^15.  O stays in tensor
@@ -14,8 +14,8 @@
 // What bounds it is the exponential (16 a clock and SM): 2,048 clocks a unit and block, against 1,024 of the products of heads of 64.
 //
 // The work is laid out on the device, from the entries alone (no list is made on the host, and a replayed graph takes any
-// entries): units in the order of the entries, the last of an entry first, times heads; where they are fewer than the SMs their keys
-// are shared among parts, whose 32-bit results the one that arrives last adds up in order.  Every wait is bounded.
+// entries): the units, each as long as its blocks and one more, stand in a row, and every CTA takes an equal stretch of it.  A unit that
+// lies in several stretches leaves 32-bit results of its parts, which the CTA that arrives last adds up in order.  Every wait is bounded.
 #include "common.cuh"
 #include "e4m3.cuh"
 #include "tcgen05.cuh"
@@ -26,19 +26,37 @@ namespace {
 
 constexpr int TILE = 128, UNIT = 2 * TILE;
 constexpr int GROUP_BYTES = TILE * 128;            // 128 rows of 64 16-bit floats
-constexpr int SOFTMAX_WARPS = 8, CONVERTER_WARPS = 2, MMA_WARP = SOFTMAX_WARPS + CONVERTER_WARPS;
-constexpr int THREADS = (MMA_WARP + 2) * 32;     // 384: 168 registers each
+constexpr int SOFTMAX_WARPS = 16, CONVERTER_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + CONVERTER_WARPS;
+constexpr int THREADS = (MMA_WARP + 2) * 32;       // 704: 88 registers each
 constexpr int MAX_STAGES = 4;
-constexpr int MIN_PART_BLOCKS = 4;                 // blocks of 128 keys that a part has at least
+constexpr int MIN_STRETCH = 5;                     // of a CTA, where no unit is longer: its blocks and one more
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// What one thread of the MMA warp does while all of its lanes run: a warp that does not branch apart keeps descriptors where the
+// instruction wants them (issued by a lane that is alone in a branch, each product took 70 to 120 clocks of moves).
+__device__ __forceinline__ uint32_t elected_lane() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is;
+}
+__device__ __forceinline__ void umma_by(uint32_t elected, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(elected)
         : "memory");
+}
+__device__ __forceinline__ void umma_from_tmem_by(uint32_t elected, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(elected)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint32_t elected, uint64_t* bar) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(elected)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_store_bits_16(uint32_t taddr, const uint32_t* r) {
@@ -79,110 +97,119 @@ __device__ __forceinline__ uint32_t f16_instr_desc(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// The units of the step, as every thread can work them out from the entries.
+// A piece of work: a unit, or the part of it that lies in this CTA's stretch.
 struct Unit {
     int entry, row0, rows, pos0;                   // rows of the step, and the first one's position
-    int block_lo, blocks;                          // the blocks of 128 keys that this part walks
-    int part, parts, cell, index;                  // where parts of it go, and the unit's number
+    int block_lo, blocks;                          // the blocks of 128 keys
+    int part, parts, first_cta;                    // of the unit, and the CTA with its first part
+    int head;
 };
 
+// All units in a row, by one whole warp.
 struct Schedule {
     const E4m3Attention& p;
-    int units, share;                              // all units; blocks of a part, or 0: none comes in parts
+    long total, stretch, lo, hi;                   // the row's length, a CTA's share, this CTA's
+    long begin;                                    // of the unit that is next
+    int entry, tile, head, length, start, count;
 
-    __device__ int last_block(int start, int count, int tile) const { return (start + min(count, (tile + 1) * UNIT) - 1) / TILE; }
-    __device__ int first_block(int start, int tile) const {
-        const int first = p.window > 0 ? start + tile * UNIT - p.window + 1 : 0;
+    __device__ int first_block(int s, int t) const {
+        const int first = p.window > 0 ? s + t * UNIT - p.window + 1 : 0;
         return first > 0 ? first / TILE : 0;
     }
-    __device__ int blocks_of(int start, int count, int tile) const { return max(0, last_block(start, count, tile) - first_block(start, tile) + 1); }
-    __device__ int units_of(int entry) const {
-        const int count = p.item_count[entry];
-        return count > 1 ? (count + UNIT - 1) / UNIT : 0;
+    __device__ int blocks_of(int s, int c, int t) const {
+        const int last = s + min(c, (t + 1) * UNIT) - 1;
+        return last < 0 ? 0 : last / TILE - first_block(s, t) + 1;
     }
-    __device__ int parts_of(int entry) const {     // of all its units
-        const int n = units_of(entry);
-        if (share == 0) return n;
-        const int start = p.item_start[entry], count = p.item_count[entry];
-        int sum = 0;
-        for (int t = 0; t < n; t++) sum += max(1, (blocks_of(start, count, t) + share - 1) / share);
-        return sum;
-    }
+    __device__ int length_of(int s, int c, int t) const { return blocks_of(s, c, t) + 1; }
+    __device__ static int tiles_of(int c) { return (c + UNIT - 1) / UNIT; }
 
-    // By one whole warp, as is what is asked of it.
-    __device__ explicit Schedule(const E4m3Attention& params, int n_sms) : p(params), units(0), share(0) {
-        const int lane = threadIdx.x & 31;
-        for (int e = lane; e < p.n_items; e += 32) units += units_of(e);
-        units = __reduce_add_sync(0xffffffffu, units);
-        if (units == 0 || units * p.n_heads >= n_sms) return;
-        int blocks = 0;
-        for (int e = lane; e < p.n_items; e += 32) {
-            const int start = p.item_start[e], count = p.item_count[e];
-            for (int t = units_of(e) - 1; t >= 0; t--) blocks += blocks_of(start, count, t);
-        }
-        blocks = __reduce_add_sync(0xffffffffu, blocks);
-        share = max(MIN_PART_BLOCKS, (blocks * p.n_heads + n_sms - 1) / n_sms);
-    }
-    // Unit or part number `at` (over all entries); false behind the last.
-    __device__ bool find(int at, Unit& u) const {
-        const int lane = threadIdx.x & 31;
-        int units_before = 0, before = 0;
+    __device__ Schedule(const E4m3Attention& params, int lane) : p(params), total(0), entry(-1) {
+        int sum = 0, most = 0;
         for (int base = 0; base < p.n_items; base += 32) {
             const int e = base + lane;
-            int n = 0, parts = 0;
-            if (e < p.n_items) n = units_of(e), parts = parts_of(e);
-            int upto = parts, units_upto = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, units_upto, o);
-                if (lane >= o) upto += x, units_upto += y;
-            }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > at);
-            if (past != 0) {
-                const int src = __ffs(past) - 1;
-                u.entry = base + src;
-                int left = at - before - __shfl_sync(0xffffffffu, upto - parts, src);
-                int index = units_before + __shfl_sync(0xffffffffu, units_upto - n, src);
-                const int start = p.item_start[u.entry], count = p.item_count[u.entry];
-                int tile = units_of(u.entry) - 1;
-                u.part = 0, u.parts = 1;
-                if (share == 0) {
-                    tile -= left, index += left;
-                } else {
-                    for (;; tile--, index++) {
-                        u.parts = max(1, (blocks_of(start, count, tile) + share - 1) / share);
-                        if (left < u.parts) break;
-                        left -= u.parts;
-                    }
-                    u.part = left;
+            const int c_of = e < p.n_items ? p.item_count[e] : 0, s_of = e < p.n_items ? p.item_start[e] : 0;
+            for (uint32_t bits = __ballot_sync(0xffffffffu, c_of > 1); bits != 0; bits &= bits - 1) {
+                const int c = __shfl_sync(0xffffffffu, c_of, __ffs(bits) - 1), s = __shfl_sync(0xffffffffu, s_of, __ffs(bits) - 1);
+                for (int t = lane; t < tiles_of(c); t += 32) {
+                    const int n = length_of(s, c, t);
+                    sum += n, most = max(most, n);
                 }
-                const int blocks = blocks_of(start, count, tile);
-                const int each = (blocks + u.parts - 1) / u.parts;
-                u.row0 = p.item_offset[u.entry] + tile * UNIT, u.rows = min(UNIT, count - tile * UNIT), u.pos0 = start + tile * UNIT;
-                u.block_lo = first_block(start, tile) + u.part * each;
-                u.blocks = max(0, min(each, blocks - u.part * each));
-                u.cell = at, u.index = index;
-                return true;
             }
-            before += __shfl_sync(0xffffffffu, upto, 31);
-            units_before += __shfl_sync(0xffffffffu, units_upto, 31);
         }
-        return false;
+        total = (long)__reduce_add_sync(0xffffffffu, sum) * p.n_heads;
+        most = __reduce_max_sync(0xffffffffu, most);
+        stretch = max((total + gridDim.x - 1) / gridDim.x, (long)min(most, MIN_STRETCH));
+        lo = blockIdx.x * stretch, hi = min(total, lo + stretch);
+        if (lo >= hi) return;
+        // the unit in which the stretch begins
+        begin = 0;
+        for (int base = 0; base < p.n_items; base += 32) {
+            const int e = base + lane;
+            const int c_of = e < p.n_items ? p.item_count[e] : 0, s_of = e < p.n_items ? p.item_start[e] : 0;
+            for (uint32_t bits = __ballot_sync(0xffffffffu, c_of > 1); bits != 0; bits &= bits - 1) {
+                const int src = __ffs(bits) - 1;
+                const int c = __shfl_sync(0xffffffffu, c_of, src), s = __shfl_sync(0xffffffffu, s_of, src), n = tiles_of(c);
+                for (int first = 0; first < n; first += 32) {
+                    const int t = n - 1 - first - lane;
+                    const int mine = t >= 0 ? length_of(s, c, t) : 0;
+                    int upto = mine;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += x;
+                    }
+                    const uint32_t past = __ballot_sync(0xffffffffu, begin + (long)upto * p.n_heads > lo);
+                    if (past != 0) {
+                        const int at = __ffs(past) - 1;
+                        length = __shfl_sync(0xffffffffu, mine, at);
+                        begin += (long)__shfl_sync(0xffffffffu, upto - mine, at) * p.n_heads;
+                        head = (int)((lo - begin) / length);
+                        begin += (long)head * length;
+                        entry = base + src, tile = n - 1 - first - at, start = s, count = c;
+                        return;
+                    }
+                    begin += (long)__shfl_sync(0xffffffffu, upto, 31) * p.n_heads;
+                }
+            }
+        }
+    }
+    __device__ bool next(Unit& u) {
+        if (lo >= hi || begin >= hi) return false;
+        const long end = begin + length;
+        const int from = (int)(max(lo, begin) - begin), to = (int)(min(hi, end) - begin);      // place 0 is the unit's set-up
+        u.entry = entry, u.head = head;
+        u.row0 = p.item_offset[entry] + tile * UNIT, u.rows = min(UNIT, count - tile * UNIT), u.pos0 = start + tile * UNIT;
+        u.block_lo = first_block(start, tile) + max(0, from - 1);
+        u.blocks = max(0, to - 1) - max(0, from - 1);
+        u.first_cta = (int)(begin / stretch);
+        u.parts = (int)((end - 1) / stretch) - u.first_cta + 1;
+        u.part = (int)blockIdx.x - u.first_cta;
+        begin = end;
+        if (++head == p.n_heads && begin < hi) {
+            head = 0;
+            if (--tile < 0) {
+                do entry++; while (p.item_count[entry] <= 1);          // (the row goes on, so there is one)
+                start = p.item_start[entry], count = p.item_count[entry];
+                tile = tiles_of(count) - 1;
+            }
+            length = length_of(start, count, tile);
+        }
+        return true;
     }
 };
 
 struct Shared {
-    uint64_t unit_full[2], unit_empty[2], q_full, q_empty;
+    uint64_t unit_full[2], unit_empty[2], q_full[2], q_empty[2];
     uint64_t k_full[MAX_STAGES], k_empty[MAX_STAGES], v_full[MAX_STAGES], v_empty[MAX_STAGES];
-    uint64_t s_ready[2], p_ready[2], o_ready[2], o_free[2];
+    uint64_t s_ready[2], s_read[2], p_ready[2], o_added[2], o_free[2];
     uint32_t tmem;
     int failed, ticket[2];
     Unit unit[2];                                  // entry < 0: there are no more
-    int head[2];
     float q_factor[2][UNIT];
-    // of the blocks of 16 keys: the keys' scale, the values' scale's exponent, and one by the values' scale
+    float of_half[2][2][TILE];                     // what the two threads of a row tell one another
+    // of the blocks of 16 keys: the keys' scale, the values' scale's exponent, and one by what a value's 16-bit floats lack
     float k_scale[MAX_STAGES][TILE / E4M3_BLOCK], v_exponent[MAX_STAGES][TILE / E4M3_BLOCK], v_inverse[MAX_STAGES][TILE / E4M3_BLOCK];
-    uint4 absent[MAX_STAGES], none[MAX_STAGES];    // keys that are not there; values that are no numbers (a bit a key)
+    uint32_t absent[MAX_STAGES][4], none[MAX_STAGES][4];      // keys that are not there, and that or whose values are no numbers (a bit a key)
 };
 
 // (a role that gave up leaves its barriers as they are, so that the others' waits run out, or find out here)
@@ -220,12 +247,11 @@ struct Blocks {
     }
 };
 
-// A warp's next unit (the k-th it asks for); false when there are none, or a wait ran out.
-__device__ __forceinline__ bool next_unit(Shared& sh, int k, Unit& u, int& head) {
-    const bool ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.unit_full[k & 1], (k >> 1) & 1));
+// A warp's next unit (the k-th it asks for); false when there are none, or (`ok`) a wait ran out.
+__device__ __forceinline__ bool next_unit(Shared& sh, int k, Unit& u, bool& ok) {
+    ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.unit_full[k & 1], (k >> 1) & 1));
     if (!ok) return false;
     u = sh.unit[k & 1];
-    head = sh.head[k & 1];
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.unit_empty[k & 1]);
     return u.entry >= 0;
@@ -244,20 +270,47 @@ __device__ __forceinline__ void add_pair(float& x, float& y, float a, float b) {
         : "f"(a), "f"(b));
 }
 
-template <bool CAP>
-__global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3Attention p, int stages, int n_sms, int* work) {
+// The 256 threads of a tile meet; whether any of them says yes.  (Where a wait ran out for some of them only, they leave together all the same,
+// from a meeting in which one said so: one that left alone would keep the others waiting here for good.)
+__device__ __forceinline__ bool any_of_tile(int tile, bool yes) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any)
+                 : "r"(1 + tile), "r"(yes ? 1u : 0u)
+                 : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void tile_meets(int tile) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(1 + tile) : "memory"); }
+
+__device__ __forceinline__ void store_sixteen(bf16* to, const float (&o)[16], float factor) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(o[2 * i] * factor, o[2 * i + 1] * factor);
+        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// GROUPS: groups of 64 columns that a key and a value take in shared memory.
+// Tensor memory: S of the tiles from columns 0 and 128 on.  With one group O lies from 256 and 320 on, and P, which two 16-bit floats a column
+// make half as wide, from 384 and 448 on, so that S of the next block need not wait for the product with P; with two, O from 256 and
+// 384 on, and P over S, each half of a row's columns over the first half of its own.
+template <bool CAP, int GROUPS>
+__global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3Attention p, int stages) {
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ __align__(16) Shared sh;
     dependents_may_start();
+    constexpr bool P_APART = GROUPS == 1;
+    constexpr int O_AT = 2 * TILE, O_STEP = 64 * GROUPS, P_AT = P_APART ? 384 : 0, P_STEP = P_APART ? 64 : TILE, P_HALF = P_APART ? 32 : 64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int k_groups = (p.dim + 63) / 64, v_groups = (p.vdim + 63) / 64;
     unsigned char* tiles = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
-    unsigned char* q_tile = tiles;                                             // [2][k_groups]
-    unsigned char* k_stage = q_tile + 2 * k_groups * GROUP_BYTES;              // [stages][k_groups]
-    unsigned char* v_stage = k_stage + stages * k_groups * GROUP_BYTES;        // [stages][v_groups]
+    constexpr int Q_PLACES = GROUPS == 1 ? 2 : 1;                              // (there is room for the next unit's)
+    unsigned char* q_tile = tiles;                                             // [Q_PLACES][2][GROUPS]
+    unsigned char* k_stage = q_tile + Q_PLACES * 2 * GROUPS * GROUP_BYTES;                // [stages][GROUPS]
+    unsigned char* v_stage = k_stage + stages * GROUPS * GROUP_BYTES;          // [stages][GROUPS]
     if (threadIdx.x == 0) {
-        mbar_init(&sh.q_full, CONVERTER_WARPS);
-        mbar_init(&sh.q_empty, 1);
         for (int s = 0; s < MAX_STAGES; s++) {
             mbar_init(&sh.k_full[s], CONVERTER_WARPS);
             mbar_init(&sh.v_full[s], CONVERTER_WARPS);
@@ -265,12 +318,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             mbar_init(&sh.v_empty[s], 1);
         }
         for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.q_full[i], CONVERTER_WARPS);
+            mbar_init(&sh.q_empty[i], 1);
             mbar_init(&sh.unit_full[i], 1);
             mbar_init(&sh.unit_empty[i], SOFTMAX_WARPS + CONVERTER_WARPS + 1);
             mbar_init(&sh.s_ready[i], 1);
-            mbar_init(&sh.p_ready[i], 4);
-            mbar_init(&sh.o_ready[i], 1);
-            mbar_init(&sh.o_free[i], 4);
+            mbar_init(&sh.s_read[i], SOFTMAX_WARPS / 2);
+            mbar_init(&sh.p_ready[i], SOFTMAX_WARPS / 2);
+            mbar_init(&sh.o_added[i], 1);
+            mbar_init(&sh.o_free[i], SOFTMAX_WARPS / 2);
         }
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -283,92 +339,93 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
     wait_for_earlier_kernels();
 
     Ring ring;                                      // of the next block
+    Unit u;
     if (warp < SOFTMAX_WARPS) {
-        // ---- softmax: a thread a row ----
-        const int tile = warp >> 2, r = threadIdx.x - tile * TILE, row = tile * TILE + r;
-        const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lane_addr + TILE * tile, o_at = tmem + lane_addr + 256 + TILE * tile;
+        // ---- softmax: two threads a row ----
+        const int tile = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, row = tile * TILE + r;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t s_at = lanes + TILE * tile + 64 * half, o_at = lanes + O_AT + O_STEP * tile, p_at = lanes + P_AT + P_STEP * tile + P_HALF * half;
         const float cap_factor = CAP ? 2.0f * LOG2E / p.cap : 0.0f, cap_log2 = p.cap * LOG2E;
-        uint32_t s_seen = 0, o_seen = 0;
-        Unit u;
-        int head;
-        for (int k = 0; next_unit(sh, k, u, head); k++) {
+        uint32_t seen_blocks = 0;                    // of this tile, over all units
+        bool ok = true;
+        for (int k = 0;; k++) {
+            const bool more = next_unit(sh, k, u, ok);
+            if (any_of_tile(tile, !ok)) ok = false;
+            if (!ok || !more) break;
             const Blocks blocks(u);
             const int n = tile == 0 ? blocks.n[0] : blocks.n[1];
             const bool has_row = row < u.rows;
             const int pos = u.pos0 + (has_row ? row : u.rows - 1);
             const int first = p.window > 0 ? pos - p.window + 1 : 0;
-            const int tile_first_pos = u.pos0 + tile * TILE;
             float m = -INFINITY, l = 0.0f, q_factor = 0.0f;
-            bool ok = true, sees_none = false;
-            for (int j = 0; j < n; j++) {
-                const int s = ring.stage, key0 = (u.block_lo + j) * TILE;
+            bool sees_none = false;
+            for (int j = 0; j < n; j++, seen_blocks++) {
+                const int s = ring.stage, key0 = (u.block_lo + j) * TILE + 64 * half;
                 // (the values' barrier too: what stands beside the tiles comes with it)
-                ok = wait_or_fail(sh, &sh.v_full[s], ring.parity) && wait_or_fail(sh, &sh.s_ready[tile], (s_seen + j) & 1);
-                ring = ring.next(stages);
+                ok = wait_or_fail(sh, &sh.v_full[s], ring.parity) && wait_or_fail(sh, &sh.s_ready[tile], seen_blocks & 1);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                ring = ring.next(stages);
                 tcgen05_after_sync();
                 if (j == 0) q_factor = sh.q_factor[k & 1][row];
-                const uint4 absent = sh.absent[s], none = sh.none[s];
-                const bool needs_mask = key0 + TILE - 1 > tile_first_pos || p.window > 0 ||
-                                        (absent.x | absent.y | absent.z | absent.w | none.x | none.y | none.z | none.w) != 0;
+                const uint2 absent = *reinterpret_cast<const uint2*>(&sh.absent[s][2 * half]), none = *reinterpret_cast<const uint2*>(&sh.none[s][2 * half]);
+                const bool needs_mask = key0 + 63 > u.pos0 + tile * TILE || p.window > 0 || (absent.x | absent.y | none.x | none.y) != 0;
                 // which of the columns c .. c + 31 this row sees
                 auto seen = [&](int c) -> uint32_t {
                     const int most = pos - key0 - c, least = first - key0 - c;
                     uint32_t bits = most >= 31 ? 0xffffffffu : (most < 0 ? 0u : (2u << most) - 1u);
                     if (least > 0) bits &= least > 31 ? 0u : 0xffffffffu << least;
-                    return bits & ~(c == 0 ? absent.x : c == 32 ? absent.y : c == 64 ? absent.z : absent.w);
+                    return bits & ~(c == 0 ? absent.x : absent.y);
                 };
                 auto mask = [&](uint32_t (&v)[32], uint32_t bits) {
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[i] = (bits >> i) & 1 ? v[i] : 0xff800000u;
                 };
-                // The row is read twice, 32 columns at a time, the next ones on their way (all 128 in registers spill, and a loop body of
-                // 128 columns does not stay with the instructions near the warps: 3,500 clocks a block against ...).
+                // The row is read twice, 32 columns at a time (a loop body of all of them does not stay with the instructions near the warps).
                 // First its largest, in powers of two, with the values' scale (no factor is negative, and the cap keeps the order: the largest
                 // score is the largest product's).
                 float top = -INFINITY;
-                uint32_t v[2][32];
-                tmem_ask_32(s_at, v[0]);
-                auto largest = [&](uint32_t (&x)[32], int c) {
+                uint32_t v[32];
+#pragma unroll 1
+                for (int c = 0; ok && c < 64; c += 32) {
+                    tmem_ask_32(s_at + c, v);
+                    tmem_wait_32(v);
                     if (needs_mask) {
                         const uint32_t bits = seen(c);
-                        if (((c == 0 ? none.x : c == 32 ? none.y : c == 64 ? none.z : none.w) & bits) != 0) sees_none = true;
-                        mask(x, bits);
+                        if (((c == 0 ? none.x : none.y) & bits) != 0) sees_none = true;
+                        mask(v, bits);
                     }
 #pragma unroll
-                    for (int half = 0; half < 2; half++) {
+                    for (int g = 0; g < 2; g++) {
                         float most[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const uint32_t* y = x + 16 * half + 8 * e;
+                            const uint32_t* y = v + 16 * g + 8 * e;
                             most[e] = max_of_three(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
                             most[e] = max_of_three(most[e], __uint_as_float(y[3]), __uint_as_float(y[4]));
                             most[e] = max_of_three(most[e], __uint_as_float(y[5]), __uint_as_float(y[6]));
                             most[e] = fmaxf(most[e], __uint_as_float(y[7]));
                         }
+                        const int group = 4 * half + c / 16 + g;
                         const float of_all = fmaxf(most[0], most[1]);
-                        const float y = of_all * (q_factor * sh.k_scale[s][c / 16 + half]), t = sh.v_exponent[s][c / 16 + half];
-                        const float z = (CAP ? capped(y, cap_log2, cap_factor) : y) + t;
+                        const float y = of_all * (q_factor * sh.k_scale[s][group]);
+                        const float z = (CAP ? capped(y, cap_log2, cap_factor) : y) + sh.v_exponent[s][group];
                         top = fmaxf(top, of_all == -INFINITY ? of_all : z);
                     }
-                };
-#pragma unroll 1
-                for (int c = 0; c < TILE; c += 64) {
-                    tmem_wait_32(v[0]);
-                    tmem_ask_32(s_at + c + 32, v[1]);
-                    largest(v[0], c);
-                    tmem_wait_32(v[1]);
-                    tmem_ask_32(s_at + ((c + 64) & (TILE - 1)), v[0]);      // (the last time: where the second reading begins)
-                    largest(v[1], c + 32);
                 }
-                if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                    const float most = fmaxf(m, top), down = m == -INFINITY ? 0.0f : exp2_fast(m - most);
+                // the product before has been added to O, and has read its P
+                if (j > 0) ok = ok && wait_or_fail(sh, &sh.o_added[tile], (seen_blocks - 1) & 1);
+                if (any_of_tile(tile, top > m + 8.0f || !ok)) {
+                    sh.of_half[tile][half][r] = top;
+                    if (any_of_tile(tile, !ok)) {
+                        ok = false;
+                        break;
+                    }
+                    const float most = fmaxf(m, fmaxf(top, sh.of_half[tile][half ^ 1][r])), down = m == -INFINITY ? 0.0f : exp2_fast(m - most);
                     m = most;
                     l *= down;
-                    if (j > 0) {                     // (the products into O up to here are done: S of this block came behind them)
-                        for (int c = 0; c < p.vdim; c += 16) {
+                    if (j > 0) {
+                        tcgen05_after_sync();
+                        for (int c = 16 * half; c < p.vdim; c += 32) {       // (the two threads take turns with 16 columns)
                             float o[16];
                             tmem_load_16(o_at + c, o);
                             uint32_t w[16];
@@ -379,17 +436,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                     }
                 }
                 const float base = (m == -INFINITY ? 0.0f : m) - 7.0f;
-                auto weights = [&](uint32_t (&v32)[32], int c) {
-                    if (needs_mask) mask(v32, seen(c));
+#pragma unroll 1
+                for (int c = 0; c < 64; c += 32) {
+                    tmem_ask_32(s_at + c, v);
+                    tmem_wait_32(v);
+                    if (P_APART && c == 32) {
+                        // S may be written again
+                        tcgen05_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.s_read[tile]);
+                    }
+                    if (needs_mask) mask(v, seen(c));
                     uint32_t packed[16];
 #pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        const int g = c / 16 + half;
-                        const float from = sh.v_exponent[s][g] - base, factor = q_factor * sh.k_scale[s][g];
+                    for (int g = 0; g < 2; g++) {
+                        const int group = 4 * half + c / 16 + g;
+                        const float from = sh.v_exponent[s][group] - base, factor = q_factor * sh.k_scale[s][group];
                         float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            float x = __uint_as_float(v32[16 * half + i]), y = __uint_as_float(v32[16 * half + i + 1]);
+                            float x = __uint_as_float(v[16 * g + i]), y = __uint_as_float(v[16 * g + i + 1]);
                             if (CAP) {
                                 // (what is hidden stays hidden: its score is minus infinity, not minus the cap)
                                 const float a = capped(x * factor, cap_log2, cap_factor) + from, b = capped(y * factor, cap_log2, cap_factor) + from;
@@ -399,379 +465,351 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                             }
                             x = exp2_fast(x), y = exp2_fast(y);
                             add_pair(sum[(i >> 1) & 1][0], sum[(i >> 1) & 1][1], x, y);
-                            packed[8 * half + i / 2] = half2_of(x, y);
+                            packed[8 * g + i / 2] = half2_of(x, y);
                         }
                         add_pair(sum[0][0], sum[0][1], sum[1][0], sum[1][1]);
-                        l = fmaf(sum[0][0] + sum[0][1], sh.v_inverse[s][g], l);
+                        l = fmaf(sum[0][0] + sum[0][1], sh.v_inverse[s][group], l);
                     }
-                    tmem_store_bits_16(s_at + c / 2, packed);      // P of columns c .. c + 31, over S, which has been read
-                };
-#pragma unroll 1
-                for (int c = 0; c < TILE; c += 64) {
-                    tmem_wait_32(v[0]);
-                    tmem_ask_32(s_at + c + 32, v[1]);
-                    weights(v[0], c);
-                    tmem_wait_32(v[1]);
-                    if (c + 64 < TILE) tmem_ask_32(s_at + c + 64, v[0]);
-                    weights(v[1], c + 32);
+                    tmem_store_bits_16(p_at + c / 2, packed);
                 }
                 tmem_stores_landed();
                 tcgen05_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_ready[tile]);
             }
-            if (ok && n > 0) {
-                ok = wait_or_fail(sh, &sh.o_ready[tile], o_seen & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                tcgen05_after_sync();
-            }
-            if (!ok) {
-                if (lane == 0) give_up(sh, p, 34);
+            if (!ok) break;                          // (all 256 threads)
+            if (n > 0) ok = wait_or_fail(sh, &sh.o_added[tile], (seen_blocks - 1) & 1);
+            for (int j = n; j < blocks.most; j++) ring = ring.next(stages);
+            if (sees_none) l = __int_as_float(0x7fffffff);
+            sh.of_half[tile][half][r] = l;
+            if (any_of_tile(tile, !ok)) {
+                ok = false;
                 break;
             }
-            if (sees_none) l = __int_as_float(0x7fffffff);
-            bf16* out = static_cast<bf16*>(p.out) + (u.row0 + (has_row ? row : 0)) * p.ld_out + (long)head * p.vdim;
-            const int width = (p.vdim + 63) / 64 * 64;
-            float* cell = p.partial + ((long)u.cell * p.n_heads + head) * UNIT * (width + 2) + row;
-            if (u.parts == 1) {
-                const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-                for (int c = 0; c < p.vdim; c += 16) {
-                    float o[16];
-                    if (n > 0) tmem_load_16(o_at + c, o);
-                    uint32_t w[8];
+            tcgen05_after_sync();
+            l += sh.of_half[tile][half ^ 1][r];
+            bf16* out = static_cast<bf16*>(p.out) + (u.row0 + (has_row ? row : 0)) * p.ld_out + (long)u.head * p.vdim;
+            // Parts leave their sums column by column, so that the rows of a warp lie side by side.  A part that begins a unit is its CTA's last and has
+            // the second of the CTA's two places; any other is its first.
+            const int width = p.vdim <= 64 ? 64 : 128, rows_of_cell = width + 2;
+            auto cell = [&](int part) { return p.partial + (long)(2 * (u.first_cta + part) + (part == 0 ? 1 : 0)) * UNIT * rows_of_cell + row; };
+            float* mine = cell(u.part);
+            const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+            for (int c = 16 * half; c < p.vdim; c += 32) {
+                float o[16];
+                if (n > 0) {
+                    tmem_load_16(o_at + c, o);
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const __nv_bfloat162 two = n > 0 ? __floats2bfloat162_rn(o[2 * i] * inverse, o[2 * i + 1] * inverse)
-                                                         : __floats2bfloat162_rn(0.0f, 0.0f);
-                        w[i] = *reinterpret_cast<const uint32_t*>(&two);
-                    }
-                    if (has_row) {
-                        *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
+                    for (int i = 0; i < 16; i++) o[i] = 0.0f;
                 }
-            } else {
-                // this part's sums, column by column, so that the rows of a warp lie side by side
-                for (int c = 0; c < p.vdim; c += 16) {
-                    float o[16];
-                    if (n > 0) tmem_load_16(o_at + c, o);
+                if (u.parts == 1) {
+                    if (has_row) store_sixteen(out + c, o, inverse);
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) __stcg(cell + (long)(c + i) * UNIT, n > 0 ? o[i] : 0.0f);
+                    for (int i = 0; i < 16; i++) __stcg(mine + (c + i) * UNIT, o[i]);
                 }
-                __stcg(cell + (long)width * UNIT, m);
-                __stcg(cell + (long)(width + 1) * UNIT, l);
             }
             // O may be written again
             tcgen05_before_sync();
             __syncwarp();
             if (lane == 0 && n > 0) mbar_arrive(&sh.o_free[tile]);
             if (u.parts > 1) {
+                if (half == 0) __stcg(mine + width * UNIT, m), __stcg(mine + (width + 1) * UNIT, l);
                 __threadfence();
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
-                int* counter = p.counters + 2 * (u.index * p.n_heads + head) + tile;
-                if (r == 0) sh.ticket[tile] = atomicAdd(counter, 1);
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
+                tile_meets(tile);
+                int* counter = p.counters + 2 * u.first_cta + tile;
+                if (half == 0 && r == 0) sh.ticket[tile] = atomicAdd(counter, 1);
+                tile_meets(tile);
                 if (sh.ticket[tile] == u.parts - 1) {
                     __threadfence();
-                    if (r == 0) *counter = 0;
+                    if (half == 0 && r == 0) *counter = 0;
                     if (has_row) {
-                        const long step = (long)p.n_heads * UNIT * (width + 2);
-                        const float* all = cell - u.part * step;
                         float top = -INFINITY, total = 0.0f;
-                        for (int q = 0; q < u.parts; q++) top = fmaxf(top, __ldcg(all + q * step + (long)width * UNIT));
+                        for (int q = 0; q < u.parts; q++) top = fmaxf(top, __ldcg(cell(q) + width * UNIT));
                         const float anchor = top == -INFINITY ? 0.0f : top;
                         for (int q = 0; q < u.parts; q++)
-                            total += exp2_fast(__ldcg(all + q * step + (long)width * UNIT) - anchor) * __ldcg(all + q * step + (long)(width + 1) * UNIT);
-                        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-                        for (int c = 0; c < p.vdim; c += 16) {
+                            total += exp2_fast(__ldcg(cell(q) + width * UNIT) - anchor) * __ldcg(cell(q) + (width + 1) * UNIT);
+                        for (int c = 16 * half; c < p.vdim; c += 32) {
                             float o[16];
 #pragma unroll
                             for (int i = 0; i < 16; i++) o[i] = 0.0f;
                             for (int q = 0; q < u.parts; q++) {
-                                const float weight = exp2_fast(__ldcg(all + q * step + (long)width * UNIT) - anchor);
+                                const float* theirs = cell(q);
+                                const float weight = exp2_fast(__ldcg(theirs + width * UNIT) - anchor);
 #pragma unroll
-                                for (int i = 0; i < 16; i++) o[i] += weight * __ldcg(all + q * step + (long)(c + i) * UNIT);
+                                for (int i = 0; i < 16; i++) o[i] += weight * __ldcg(theirs + (c + i) * UNIT);
                             }
-                            uint32_t w[8];
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                const __nv_bfloat162 two = __floats2bfloat162_rn(o[2 * i] * inverse, o[2 * i + 1] * inverse);
-                                w[i] = *reinterpret_cast<const uint32_t*>(&two);
-                            }
-                            *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                            *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                            store_sixteen(out + c, o, total == 0.0f ? 0.0f : 1.0f / total);
                         }
                     }
                 }
             }
-            for (int j = n; j < blocks.most; j++) ring = ring.next(stages);
-            s_seen += n;
-            o_seen += n > 0 ? 1 : 0;
         }
+        if (!ok && lane == 0) give_up(sh, p, 34);
     } else if (warp < MMA_WARP) {
-        // ---- converters: a thread a key of each half of a block (and four queries) ----
-        constexpr int CONVERTERS = CONVERTER_WARPS * 32, HALVES = TILE / CONVERTERS;
+        // ---- converters: a thread a key (and two queries) ----
         const int t = threadIdx.x - SOFTMAX_WARPS * 32;
-        const int k_pieces = p.dim / 16, v_pieces = p.vdim / 16;
-        Unit u;
-        int head;
-        for (int k = 0; next_unit(sh, k, u, head); k++) {
-            const int kv_head = head / (p.n_heads / p.n_kv_heads);
-            const int n_blocks = Blocks(u).most, last = u.pos0 + u.rows - 1;
+        bool ok = true;
+        for (int k = 0; next_unit(sh, k, u, ok); k++) {
+            const int kv_head = u.head / (p.n_heads / p.n_kv_heads);
+            const int n_blocks = Blocks(u).most;
             const int* table = p.block_table + (long)u.entry * p.max_blocks;
-            uint4 k_row[8], v_row[8];
-            float k_scale = 1.0f, v_scale = 1.0f;
-            bool there = false;
-            // This thread's key in steps of half a block: its position, its page's place in the table and its own in the page.
+            // This thread's key, block after block: its position, its page's place in the table and its own in the page.
             int key = u.block_lo * TILE + t, page_index = key / p.page, slot = key - page_index * p.page;
-            const int key_end = min(last + 1, (u.block_lo + n_blocks) * TILE);
-            auto look_up = [&](int& at_slot) -> int {        // the key's page, or -1 where it is not there; then on to the next step's
-                at_slot = slot;
-                int id = -1;
-                if (key < key_end && page_index < p.max_blocks) id = table[page_index];
-                key += CONVERTERS, slot += CONVERTERS;
-                while (slot >= p.page) slot -= p.page, page_index++;
+            const int key_end = min(u.pos0 + u.rows, (u.block_lo + n_blocks) * TILE);
+            auto look_up = [&]() -> int {                    // the key's page, or -1 where it is not there
+                const int id = key < key_end && page_index < p.max_blocks ? table[page_index] : -1;
                 return id < p.n_pages ? id : -1;
             };
-            auto at_of = [&](int id, int at_slot) -> long { return id >= 0 ? ((long)id * p.n_kv_heads + kv_head) * p.page + at_slot : 0; };
-            auto load_k = [&](int id, long at) {
-                there = id >= 0;
-                k_scale = v_scale = 1.0f;
-                if ((t & 15) == 0 && there) k_scale = p.k_scales[at >> 4], v_scale = p.v_scales[at >> 4];
-                const uint4* from = reinterpret_cast<const uint4*>(p.k_pages + at * p.dim);
+            auto row_of = [&](int id) -> long { return id >= 0 ? ((long)id * p.n_kv_heads + kv_head) * p.page + slot : -1; };
+            auto go_on = [&]() {
+                key += TILE, slot += TILE;
+                while (slot >= p.page) slot -= p.page, page_index++;
+            };
+            // 64 columns of a key or a value
+            auto fetch = [&](uint4 (&to)[4], const uint8_t* pages, int size, int group, long at) {
+                const uint4* from = reinterpret_cast<const uint4*>(pages + max(at, 0L) * size + 64 * group);
 #pragma unroll
-                for (int i = 0; i < 8; i++) k_row[i] = (there && i < k_pieces) ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+                for (int i = 0; i < 4; i++) to[i] = at >= 0 && 64 * group + 16 * i < size ? from[i] : make_uint4(0u, 0u, 0u, 0u);
             };
-            auto load_v = [&](int id, long at) {
-                const uint4* from = reinterpret_cast<const uint4*>(p.v_pages + at * p.vdim);
+            // 16 codes are two 16-byte chunks of a row in a swizzled tile; returns whether a code is no number (it has become one here: the
+            // softmax puts it back in where it is seen)
+            auto put = [&](unsigned char* group, const uint4 (&v)[4]) -> uint32_t {
+                uint32_t none = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) v_row[i] = (id >= 0 && i < v_pieces) ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+                for (int i = 0; i < 4; i++) {
+                    uint4 a, b;
+                    none |= codes_none(v[i].x) | codes_none(v[i].y) | codes_none(v[i].z) | codes_none(v[i].w);
+                    e4m3_to_half2_by_bits(v[i].x, a.x, a.y);
+                    e4m3_to_half2_by_bits(v[i].y, a.z, a.w);
+                    e4m3_to_half2_by_bits(v[i].z, b.x, b.y);
+                    e4m3_to_half2_by_bits(v[i].w, b.z, b.w);
+                    *reinterpret_cast<uint4*>(group + t * 128 + (((2 * i) ^ (t & 7)) * 16)) = a;
+                    *reinterpret_cast<uint4*>(group + t * 128 + (((2 * i + 1) ^ (t & 7)) * 16)) = b;
+                }
+                return none;
             };
-            // 16 codes to two 16-byte chunks of a row in a swizzled tile
-            auto put = [&](unsigned char* stage, int row, int piece, const uint4& v) {
-                uint4 a, b;
-                e4m3_to_half2(v.x, a.x, a.y);
-                e4m3_to_half2(v.y, a.z, a.w);
-                e4m3_to_half2(v.z, b.x, b.y);
-                e4m3_to_half2(v.w, b.z, b.w);
-                unsigned char* at = stage + (piece >> 2) * GROUP_BYTES + row * 128;
-                const int c = (piece & 3) * 2;
-                *reinterpret_cast<uint4*>(at + ((c ^ (row & 7)) * 16)) = a;
-                *reinterpret_cast<uint4*>(at + (((c + 1) ^ (row & 7)) * 16)) = b;
-            };
-            int slot_now, slot_after;
-            const int id = look_up(slot_now);
-            int id_after = look_up(slot_after);
-            load_k(id, at_of(id, slot_now));
-            load_v(id, at_of(id, slot_now));
-            // the queries, once the unit before has read its own for the last time
-            if (!__all_sync(0xffffffffu, wait_or_fail(sh, &sh.q_empty, (k & 1) ^ 1))) {
-                if (lane == 0) give_up(sh, p, 30);
-                break;
-            }
-            for (int row = t; row < UNIT; row += CONVERTERS) {
-                const int tile = row / TILE, tile_row = row - tile * TILE;
-                const bool has_row = row < u.rows;
-                const uint4* from = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + (u.row0 + (has_row ? row : 0)) * p.ld_q + (long)head * p.dim);
-                float top = 0.0f;
-                if (has_row)
-#pragma unroll 4
-                    for (int i = 0; i < p.dim / 8; i++) {
-                        const uint4 v = from[i];
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            const int id_first = look_up();
+            // The queries, eight or sixteen lanes a row, once the unit that had this place before has read its own for the last time.
+            unsigned char* q_here = q_tile + (k % Q_PLACES) * 2 * GROUPS * GROUP_BYTES;
+            ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.q_empty[k % Q_PLACES], ((k / Q_PLACES) & 1) ^ 1));
+            if (!ok) break;
+            {
+                constexpr int LANES = 8 * GROUPS, ROWS = 32 / LANES, AT_ONCE = 8, OF_WARP = UNIT / CONVERTER_WARPS;
+                const int chunk = lane % LANES, first_row = (warp - SOFTMAX_WARPS) * OF_WARP + lane / LANES;
+                const bf16* from = static_cast<const bf16*>(p.q) + (long)u.row0 * p.ld_q + (long)u.head * p.dim + 8 * chunk;
+#pragma unroll 1
+                for (int base = 0; base < OF_WARP; base += AT_ONCE * ROWS) {
+                    uint4 v[AT_ONCE];
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; i++) {
+                        const int row = first_row + base + i * ROWS;
+                        v[i] = row < u.rows && 8 * chunk < p.dim ? *reinterpret_cast<const uint4*>(from + row * p.ld_q) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; i++) {
+                        const int row = first_row + base + i * ROWS;
+                        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                        float top = 0.0f;
 #pragma unroll
                         for (int c = 0; c < 4; c++) top = max_of_three(top, fabsf(__uint_as_float(w[c] << 16)), fabsf(__uint_as_float(w[c] & 0xffff0000u)));
-                    }
-                // (zeros, and what is not finite, stay as they are)
-                const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
-                const float factor = power_of_two(e);
-                sh.q_factor[k & 1][row] = p.scale * power_of_two(-e) * (CAP ? 1.0f : LOG2E);
-#pragma unroll 4
-                for (int i = 0; i < p.dim / 8; i++) {
-                    const uint4 v = has_row ? from[i] : make_uint4(0u, 0u, 0u, 0u);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                    uint32_t h[4];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) h[c] = half2_of(__uint_as_float(w[c] << 16) * factor, __uint_as_float(w[c] & 0xffff0000u) * factor);
-                    *reinterpret_cast<uint4*>(q_tile + (tile * k_groups + i / 8) * GROUP_BYTES + tile_row * 128 + (((i & 7) ^ (tile_row & 7)) * 16)) =
-                        make_uint4(h[0], h[1], h[2], h[3]);
+                        for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        // (zeros, and what is not finite, stay as they are)
+                        const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
+                        const float factor = power_of_two(e);
+                        if (chunk == 0) sh.q_factor[k & 1][row] = p.scale * E4M3_BITS_SCALE * power_of_two(-e) * (CAP ? 1.0f : LOG2E);
+                        uint32_t h[4];
+#pragma unroll
+                        for (int c = 0; c < 4; c++) h[c] = half2_of(__uint_as_float(w[c] << 16) * factor, __uint_as_float(w[c] & 0xffff0000u) * factor);
+                        *reinterpret_cast<uint4*>(q_here + ((row / TILE) * GROUPS + chunk / 8) * GROUP_BYTES + (row % TILE) * 128 + (((chunk ^ row) & 7) * 16)) =
+                            make_uint4(h[0], h[1], h[2], h[3]);
+                    }
                 }
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.q_full);
-            bool ok = true;
-            for (int step = 0; step < HALVES * n_blocks; step++) {
-                const int half = step % HALVES, row = half * CONVERTERS + t, s = ring.stage;
+            if (lane == 0) mbar_arrive(&sh.q_full[k % Q_PLACES]);
+            long at = row_of(id_first);
+            go_on();
+            float k_scale = 1.0f, v_scale = 1.0f;
+            auto scales = [&]() {
+                k_scale = v_scale = 1.0f;
+                if ((t & 15) == 0 && at >= 0) k_scale = p.k_scales[at >> 4], v_scale = p.v_scales[at >> 4];
+            };
+            uint4 buffer[2][4];                              // on their way: the next 128 columns, keys' before values'
+            fetch(buffer[0], p.k_pages, p.dim, 0, at);
+            if (GROUPS == 2) fetch(buffer[1], p.k_pages, p.dim, 1, at);
+            else fetch(buffer[1], p.v_pages, p.vdim, 0, at);
+            scales();
+            for (int j = 0; j < n_blocks; j++) {
+                const int s = ring.stage;
                 const uint32_t parity = ring.parity ^ 1;
-                if (half == 0) ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.k_empty[s], parity));
+                const int id_next = look_up();
+                ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.k_empty[s], parity));
                 if (!ok) break;
-                const uint32_t absent = __ballot_sync(0xffffffffu, !there);
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (i < k_pieces) put(k_stage + s * k_groups * GROUP_BYTES, row, i, k_row[i]);
-                if (half == HALVES - 1) {
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.k_full[s]);
+                unsigned char* k_tile = k_stage + s * GROUPS * GROUP_BYTES;
+                unsigned char* v_tile = v_stage + s * GROUPS * GROUP_BYTES;
+                const uint32_t absent = __ballot_sync(0xffffffffu, at < 0);
+                uint32_t none = put(k_tile, buffer[0]);
+                const long at_next = row_of(id_next);
+                if (GROUPS == 2) {
+                    fetch(buffer[0], p.v_pages, p.vdim, 0, at);
+                    none |= put(k_tile + GROUP_BYTES, buffer[1]);
+                    fetch(buffer[1], p.v_pages, p.vdim, 1, at);
+                } else {
+                    fetch(buffer[0], p.k_pages, p.dim, 0, at_next);
                 }
+                go_on();
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.k_full[s]);
                 // What stands beside the tiles is read until the block's P is there, which its second product waits for: behind v_empty.
-                if (half == 0) ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.v_empty[s], parity));
+                ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.v_empty[s], parity));
                 if (!ok) break;
                 if ((t & 15) == 0) {
-                    sh.k_scale[s][row >> 4] = k_scale;
-                    sh.v_exponent[s][row >> 4] = (float)exponent_of(v_scale);
-                    sh.v_inverse[s][row >> 4] = 1.0f / v_scale;
+                    sh.k_scale[s][t >> 4] = k_scale;
+                    sh.v_exponent[s][t >> 4] = (float)exponent_of(v_scale);
+                    sh.v_inverse[s][t >> 4] = 1.0f / (E4M3_BITS_SCALE * v_scale);
                 }
-                const int id_now = id_after;
-                const long at = at_of(id_now, slot_after);
-                id_after = look_up(slot_after);
-                load_k(id_now, at);
-                // A value that is no number is so in its first entry; its row is left out, and the softmax puts it back in where it is seen.
-                const bool none = (v_row[0].x & 0x7fu) == 0x7fu;
-                const uint32_t nones = __ballot_sync(0xffffffffu, none);
-                if (lane == 0) {
-                    reinterpret_cast<uint32_t*>(&sh.absent[s])[row >> 5] = absent;
-                    reinterpret_cast<uint32_t*>(&sh.none[s])[row >> 5] = nones;
+                at = at_next;
+                scales();
+                if (GROUPS == 2) {
+                    none |= put(v_tile, buffer[0]);
+                    fetch(buffer[0], p.k_pages, p.dim, 0, at);
+                    none |= put(v_tile + GROUP_BYTES, buffer[1]);
+                    fetch(buffer[1], p.k_pages, p.dim, 1, at);
+                } else {
+                    none |= put(v_tile, buffer[1]);
+                    fetch(buffer[1], p.v_pages, p.vdim, 0, at);
                 }
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (i < v_pieces) put(v_stage + s * v_groups * GROUP_BYTES, row, i, none ? make_uint4(0u, 0u, 0u, 0u) : v_row[i]);
-                if (half == HALVES - 1) {
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.v_full[s]);
-                }
-                load_v(id_now, at);
-                if (half == HALVES - 1) ring = ring.next(stages);
+                const uint32_t nones = __ballot_sync(0xffffffffu, none != 0);
+                if (lane == 0) sh.absent[s][warp - SOFTMAX_WARPS] = absent, sh.none[s][warp - SOFTMAX_WARPS] = nones;
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.v_full[s]);
+                ring = ring.next(stages);
             }
-            if (!ok) {
-                if (lane == 0) give_up(sh, p, 31);
+            if (!ok) break;
+        }
+        if (!ok && lane == 0) give_up(sh, p, 31);
+    } else if (warp == MMA_WARP) {
+        // ---- products ----
+        const uint32_t elected = elected_lane();
+        const uint32_t idesc_s = f16_instr_desc(TILE, TILE), idesc_o = f16_instr_desc(TILE, p.vdim) | IDESC_B_MN_MAJOR;
+        const int k_steps = p.dim / UMMA_K;
+        const uint64_t q_desc = make_smem_desc(smem_u32(q_tile)), k_desc = make_smem_desc(smem_u32(k_stage));
+        const uint64_t v_desc = make_smem_desc_mn(smem_u32(v_stage), GROUP_BYTES);
+        const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t seen_blocks[2] = {0, 0}, seen_units[2] = {0, 0};
+        int q_place = 0;
+        auto issue_s = [&](int tile, int s) {
+            const uint64_t a = q_desc + (2 * q_place + tile) * GROUPS * (GROUP_BYTES >> 4), b = k_desc + s * GROUPS * (GROUP_BYTES >> 4);
+            int kk = 0;
+            for (; kk + 4 <= k_steps; kk += 4) {
+                const uint64_t group = (kk / 4) * (GROUP_BYTES >> 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) umma_by(elected, tmem0 + TILE * tile, a + group + 2 * i, b + group + 2 * i, idesc_s, kk + i > 0 ? 1u : 0u);
+            }
+#pragma unroll 1
+            for (; kk < k_steps; kk++) {
+                const uint64_t at = (kk / 4) * (GROUP_BYTES >> 4) + 2 * (kk % 4);
+                umma_by(elected, tmem0 + TILE * tile, a + at, b + at, idesc_s, kk > 0 ? 1u : 0u);
+            }
+            umma_commit_by(elected, &sh.s_ready[tile]);
+        };
+        auto issue_o = [&](int tile, int s, bool begins) {
+            const uint64_t b = v_desc + s * GROUPS * (GROUP_BYTES >> 4);
+            const uint32_t a = tmem0 + P_AT + P_STEP * tile, d = tmem0 + O_AT + O_STEP * tile;
+            umma_from_tmem_by(elected, d, a, b, idesc_o, begins ? 0u : 1u);
+#pragma unroll
+            for (int kk = 1; kk < TILE / UMMA_K; kk++)
+                umma_from_tmem_by(elected, d, a + (kk / 4) * P_HALF + (kk % 4) * (UMMA_K / 2), b + kk * (2048 >> 4), idesc_o, 1u);
+            umma_commit_by(elected, &sh.o_added[tile]);
+        };
+        bool ok = true;
+        for (int k = 0; next_unit(sh, k, u, ok); k++) {
+            const Blocks of_unit(u);
+            // (the same for all lanes, and the compiler knows it)
+            const int n0 = __shfl_sync(0xffffffffu, of_unit.n[0], 0), n1 = __shfl_sync(0xffffffffu, of_unit.n[1], 0), most = max(n0, n1);
+            q_place = k % Q_PLACES;
+            ok = wait_or_fail(sh, &sh.q_full[q_place], (k / Q_PLACES) & 1);
+            if (most > 0) {
+                ok = ok && wait_or_fail(sh, &sh.k_full[ring.stage], ring.parity);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tcgen05_after_sync();
+                if (n0 > 0) issue_s(0, ring.stage);
+                if (n1 > 0) issue_s(1, ring.stage);
+                umma_commit_by(elected, &sh.k_empty[ring.stage]);
+            }
+            for (int j = 0; j < most; j++) {
+                const Ring after = ring.next(stages);
+                ok = wait_or_fail(sh, &sh.v_full[ring.stage], ring.parity);
+                if (j + 1 < most) ok = ok && wait_or_fail(sh, &sh.k_full[after.stage], after.parity);
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++) {
+                    const int n = tile == 0 ? n0 : n1;
+                    if (j >= n) continue;
+                    const uint32_t parity = (seen_blocks[tile] + j) & 1;
+                    if (P_APART && j + 1 < n) {
+                        ok = __all_sync(0xffffffffu, ok && wait_or_fail(sh, &sh.s_read[tile], parity));
+                        if (!ok) break;
+                        tcgen05_after_sync();
+                        issue_s(tile, after.stage);
+                    }
+                    // the unit before has read its O
+                    if (j == 0) ok = ok && wait_or_fail(sh, &sh.o_free[tile], (seen_units[tile] & 1) ^ 1);
+                    ok = __all_sync(0xffffffffu, ok && wait_or_fail(sh, &sh.p_ready[tile], parity));
+                    if (!ok) break;
+                    tcgen05_after_sync();
+                    issue_o(tile, ring.stage, j == 0);
+                    if (!P_APART && j + 1 < n) issue_s(tile, after.stage);
+                }
+                if (!ok) break;
+                umma_commit_by(elected, &sh.v_empty[ring.stage]);
+                if (j + 1 < most) umma_commit_by(elected, &sh.k_empty[after.stage]);
+                ring = after;
+            }
+            if (!ok) break;
+            umma_commit_by(elected, &sh.q_empty[q_place]);
+            seen_blocks[0] += n0, seen_blocks[1] += n1;
+            seen_units[0] += n0 > 0 ? 1 : 0, seen_units[1] += n1 > 0 ? 1 : 0;
+        }
+        if (!ok && lane == 0) give_up(sh, p, 33);
+    } else {
+        // ---- the next unit, while the others work on this one ----
+        Schedule schedule(p, lane);
+        for (int k = 0;; k++) {
+            if (!__all_sync(0xffffffffu, wait_or_fail(sh, &sh.unit_empty[k & 1], ((k >> 1) & 1) ^ 1))) {
+                if (lane == 0) give_up(sh, p, 35);
                 break;
             }
-        }
-    } else {
-        if (warp == MMA_WARP) {
-            // ---- products: one lane issues them ----
-            const uint32_t idesc_s = f16_instr_desc(TILE, TILE), idesc_o = f16_instr_desc(TILE, p.vdim) | IDESC_B_MN_MAJOR;
-            const int k_steps = p.dim / UMMA_K;
-            const uint64_t q_desc = make_smem_desc(smem_u32(q_tile)), k_desc = make_smem_desc(smem_u32(k_stage));
-            const uint64_t v_desc = make_smem_desc_mn(smem_u32(v_stage), GROUP_BYTES);
-            uint32_t p_seen[2] = {0, 0}, o_units[2] = {0, 0};
-            Unit u;
-            int head;
-            for (int k = 0; next_unit(sh, k, u, head); k++) {
-                const Blocks blocks(u);
-                bool ok = true;
-                if (lane == 0) {
-                    auto issue_s = [&](int tile, int s) {
-                        const uint64_t a = q_desc + tile * k_groups * (GROUP_BYTES >> 4), b = k_desc + s * k_groups * (GROUP_BYTES >> 4);
-                        int kk = 0;
-                        for (; kk + 4 <= k_steps; kk += 4) {
-                            const uint64_t group = (kk / 4) * (GROUP_BYTES >> 4);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) umma(tmem + TILE * tile, a + group + 2 * i, b + group + 2 * i, idesc_s, kk + i > 0 ? 1u : 0u);
-                        }
-#pragma unroll 1
-                        for (; kk < k_steps; kk++) {
-                            const uint64_t at = (kk / 4) * (GROUP_BYTES >> 4) + 2 * (kk % 4);
-                            umma(tmem + TILE * tile, a + at, b + at, idesc_s, kk > 0 ? 1u : 0u);
-                        }
-                        umma_commit(&sh.s_ready[tile]);
-                    };
-                    auto issue_o = [&](int tile, int s, bool begins) {
-                        const uint64_t b = v_desc + s * v_groups * (GROUP_BYTES >> 4);
-                        umma_from_tmem(tmem + 256 + TILE * tile, tmem + TILE * tile, b, idesc_o, begins ? 0u : 1u);
-#pragma unroll
-                        for (int kk = 1; kk < TILE / UMMA_K; kk++)
-                            umma_from_tmem(tmem + 256 + TILE * tile, tmem + TILE * tile + kk * (UMMA_K / 2), b + kk * (2048 >> 4), idesc_o, 1u);
-                    };
-                    ok = wait_or_fail(sh, &sh.q_full, k & 1);
-                    if (ok && blocks.most > 0) {
-                        ok = wait_or_fail(sh, &sh.k_full[ring.stage], ring.parity);
-                        if (ok) {
-                            tcgen05_after_sync();
-                            for (int tile = 0; tile < 2; tile++)
-                                if (blocks.n[tile] > 0) issue_s(tile, ring.stage);
-                            umma_commit(&sh.k_empty[ring.stage]);
-                        }
-                    }
-                    for (int j = 0; ok && j < blocks.most; j++) {
-                        const Ring after = ring.next(stages);
-                        bool v_there = false, k_there = false;
-                        for (int tile = 0; ok && tile < 2; tile++) {
-                            if (j >= blocks.n[tile]) continue;
-                            if (!v_there) ok = wait_or_fail(sh, &sh.v_full[ring.stage], ring.parity), v_there = true;
-                            // the unit before has read its O
-                            if (ok && j == 0) ok = wait_or_fail(sh, &sh.o_free[tile], (o_units[tile] & 1) ^ 1);
-                            ok = ok && wait_or_fail(sh, &sh.p_ready[tile], (p_seen[tile] + j) & 1);
-                            if (!ok) break;
-                            tcgen05_after_sync();
-                            issue_o(tile, ring.stage, j == 0);
-                            if (j + 1 < blocks.n[tile]) {
-                                if (!k_there) ok = wait_or_fail(sh, &sh.k_full[after.stage], after.parity), k_there = true;
-                                if (!ok) break;
-                                tcgen05_after_sync();
-                                issue_s(tile, after.stage);
-                            } else {
-                                umma_commit(&sh.o_ready[tile]);
-                            }
-                        }
-                        if (!ok) break;
-                        umma_commit(&sh.v_empty[ring.stage]);
-                        if (j + 1 < blocks.most) umma_commit(&sh.k_empty[after.stage]);
-                        ring = after;
-                    }
-                    if (ok) umma_commit(&sh.q_empty);
-                    else give_up(sh, p, 33);
-                }
-                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-                for (int i = 0; i < 2; i++) p_seen[i] += blocks.n[i], o_units[i] += blocks.n[i] > 0 ? 1 : 0;
+            u.entry = -1;
+            const bool more = schedule.next(u);
+            if (lane == 0) {
+                sh.unit[k & 1] = u;
+                mbar_arrive(&sh.unit_full[k & 1]);
             }
-        } else if (warp == MMA_WARP + 1) {
-            // ---- the next unit, while the others work on this one ----
-            const Schedule schedule(p, n_sms);
-            for (int k = 0;; k++) {
-                if (!__all_sync(0xffffffffu, wait_or_fail(sh, &sh.unit_empty[k & 1], ((k >> 1) & 1) ^ 1))) {
-                    if (lane == 0) give_up(sh, p, 35);
-                    break;
-                }
-                int at = 0;
-                if (lane == 0) at = atomicAdd(work, 1);
-                at = __shfl_sync(0xffffffffu, at, 0);
-                Unit u;
-                u.entry = -1;
-                const bool more = schedule.find(at / p.n_heads, u);
-                if (lane == 0) {
-                    sh.unit[k & 1] = u;
-                    sh.head[k & 1] = at % p.n_heads;
-                    mbar_arrive(&sh.unit_full[k & 1]);
-                }
-                if (!more) break;
-            }
+            if (!more) break;
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        // the last CTA to leave puts the work counter back
-        if (atomicAdd(work + 1, 1) == (int)gridDim.x - 1) work[0] = work[1] = 0;
-    }
     if (warp == MMA_WARP) tmem_free(tmem, 512);
 }
 
 }  // namespace
 
-extern "C" int mllm_e4m3_tiles_attention(const E4m3Attention* p, int n_rows, int n_sms, int* work, void* stream) {
+extern "C" int mllm_e4m3_tiles_attention(const E4m3Attention* p, int n_rows, int n_sms, void* stream) {
     if (p->n_items <= 0 || n_rows <= 0) return 0;
     if (p->dim > 128 || p->vdim > 128) return fail("e4m3_attention_tiles: heads of more than 128 entries");
-    const int k_groups = (p->dim + 63) / 64, v_groups = (p->vdim + 63) / 64;
-    const int room = 220 * 1024 - 1024 - 2 * k_groups * GROUP_BYTES;
-    const int stages = min(MAX_STAGES, room / ((k_groups + v_groups) * GROUP_BYTES));
-    const size_t bytes = 1024 + (size_t)(2 * k_groups + stages * (k_groups + v_groups)) * GROUP_BYTES;
-    auto kernel = p->cap > 0.0f ? attention_tiles_kernel<true> : attention_tiles_kernel<false>;
+    const int groups = p->dim <= 64 && p->vdim <= 64 ? 1 : 2, stages = groups == 1 ? 4 : 2;
+    const size_t bytes = 1024 + (size_t)((groups == 1 ? 4 : 2) + 2 * stages) * groups * GROUP_BYTES;
+    auto kernel = p->cap > 0.0f ? (groups == 1 ? attention_tiles_kernel<true, 1> : attention_tiles_kernel<true, 2>)
+                                : (groups == 1 ? attention_tiles_kernel<false, 1> : attention_tiles_kernel<false, 2>);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) return launched(e, "e4m3_attention_tiles");
-    return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(n_sms), dim3(THREADS), bytes, (cudaStream_t)stream,
-                                  *p, stages, n_sms, work),
+    return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(n_sms), dim3(THREADS), bytes, (cudaStream_t)stream, *p, stages),
                     "e4m3_attention_tiles");
 }

@@ -1909,7 +1909,7 @@ _e4m3_store = Function("e4m3", "mllm_e4m3_store", [P, L, P, L, I, I, I, I, I, I,
 _e4m3_plain = Function("e4m3", "mllm_e4m3_attention_plain", [ctypes.POINTER(_E4m3Attention), I, I, P])
 _e4m3_step = Function("e4m3", "mllm_e4m3_attention_step", [ctypes.POINTER(_E4m3Attention), I, P])
 
-_e4m3_tiles = Function("e4m3_tiles", "mllm_e4m3_tiles_attention", [ctypes.POINTER(_E4m3Attention), I, I, P, P])
+_e4m3_tiles = Function("e4m3_tiles", "mllm_e4m3_tiles_attention", [ctypes.POINTER(_E4m3Attention), I, I, P])
 
 _sm_counts = {}
 
@@ -2029,7 +2029,7 @@ class E4m3Workspace:
         self.vdim = int(vdim)
         n_sms = _sm_count(torch.device(device))
         self.partial = torch.empty(2 * n_sms * 256 * (_padded_64(self.vdim) + 2), dtype=torch.float32, device=device)
-        self.counters = torch.zeros(4 * n_sms + 2, dtype=torch.int32, device=device)     # (the last two: the tiles' work counter)
+        self.counters = torch.zeros(2 * n_sms, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
 
     def reset(self) -> None:
@@ -2096,7 +2096,7 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
             return out
         n_sms, stream = _sm_count(q.device), _stream()
         if longest != 1:
-            _e4m3_tiles(ctypes.byref(params), q.shape[0], n_sms, params.counters + 4 * (workspace.counters.shape[0] - 2), stream)
+            _e4m3_tiles(ctypes.byref(params), q.shape[0], n_sms, stream)
         if longest == 1 or singles:
             _e4m3_step(ctypes.byref(params), n_sms, stream)
     return out
