@@ -29,20 +29,6 @@ __device__ __forceinline__ void e4m3_to_half2(uint32_t four, uint32_t& low, uint
     high = e4m3_to_half2((uint16_t)(four >> 16));
 }
 
-// Four codes to two pairs of 16-bit floats of 2^-8 their value, in order, by moving bits: sign, then exponent and fraction one place to
-// the right, and the float's smaller exponent bias does the rest, below the normal range too.  The conversion instruction shares the unit
-// of the exponentials (16 a clock and SM); this takes seven of the integer unit's 64.  What is no number comes out as 1.875 (of the sign):
-// codes_none finds it.
-__device__ __forceinline__ void e4m3_to_half2_by_bits(uint32_t four, uint32_t& low, uint32_t& high) {
-    const uint32_t a = __byte_perm(four, 0u, 0x1404), b = __byte_perm(four, 0u, 0x3424);        // codes in the halves' upper bytes
-    low = ((a >> 1) & 0x3f803f80u) | (a & 0x80008000u);
-    high = ((b >> 1) & 0x3f803f80u) | (b & 0x80008000u);
-}
-constexpr float E4M3_BITS_SCALE = 256.0f;
-
-// Bits that are set where one of four codes is no number.
-__device__ __forceinline__ uint32_t codes_none(uint32_t four) { return ((four & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
 __device__ __forceinline__ float2 half2_to_floats(uint32_t h) {
     float2 r;
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(h));

@@ -207,9 +207,9 @@ struct Shared {
     Unit unit[2];                                  // entry < 0: there are no more
     float q_factor[2][UNIT];
     float of_half[2][2][TILE];                     // what the two threads of a row tell one another
-    // of the blocks of 16 keys: the keys' scale, the values' scale's exponent, and one by what a value's 16-bit floats lack
+    // of the blocks of 16 keys: the keys' scale, the values' scale's exponent, and one by the values' scale
     float k_scale[MAX_STAGES][TILE / E4M3_BLOCK], v_exponent[MAX_STAGES][TILE / E4M3_BLOCK], v_inverse[MAX_STAGES][TILE / E4M3_BLOCK];
-    uint32_t absent[MAX_STAGES][4], none[MAX_STAGES][4];      // keys that are not there, and that or whose values are no numbers (a bit a key)
+    uint32_t absent[MAX_STAGES][4], none[MAX_STAGES][4];      // keys that are not there, and whose values are no numbers (a bit a key)
 };
 
 // (a role that gave up leaves its barriers as they are, so that the others' waits run out, or find out here)
@@ -573,22 +573,24 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
 #pragma unroll
                 for (int i = 0; i < 4; i++) to[i] = at >= 0 && 64 * group + 16 * i < size ? from[i] : make_uint4(0u, 0u, 0u, 0u);
             };
-            // 16 codes are two 16-byte chunks of a row in a swizzled tile; returns whether a code is no number (it has become one here: the
-            // softmax puts it back in where it is seen)
-            auto put = [&](unsigned char* group, const uint4 (&v)[4]) -> uint32_t {
-                uint32_t none = 0;
+            // 16 codes are two 16-byte chunks of a row in a swizzled tile
+            auto put = [&](unsigned char* group, const uint4 (&v)[4]) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     uint4 a, b;
-                    none |= codes_none(v[i].x) | codes_none(v[i].y) | codes_none(v[i].z) | codes_none(v[i].w);
-                    e4m3_to_half2_by_bits(v[i].x, a.x, a.y);
-                    e4m3_to_half2_by_bits(v[i].y, a.z, a.w);
-                    e4m3_to_half2_by_bits(v[i].z, b.x, b.y);
-                    e4m3_to_half2_by_bits(v[i].w, b.z, b.w);
+                    e4m3_to_half2(v[i].x, a.x, a.y);
+                    e4m3_to_half2(v[i].y, a.z, a.w);
+                    e4m3_to_half2(v[i].z, b.x, b.y);
+                    e4m3_to_half2(v[i].w, b.z, b.w);
                     *reinterpret_cast<uint4*>(group + t * 128 + (((2 * i) ^ (t & 7)) * 16)) = a;
                     *reinterpret_cast<uint4*>(group + t * 128 + (((2 * i + 1) ^ (t & 7)) * 16)) = b;
                 }
-                return none;
+            };
+            // A value that is no number is so from its first entry on.  Its row is left out of the tile, where a weight of zero would not keep it
+            // out of other rows, and the softmax puts it back in where it is seen.
+            auto put_value = [&](unsigned char* group, uint4 (&v)[4], bool none) {
+                if (none) v[0] = v[1] = v[2] = v[3] = make_uint4(0u, 0u, 0u, 0u);
+                put(group, v);
             };
             const int id_first = look_up();
             // The queries, eight or sixteen lanes a row, once the unit that had this place before has read its own for the last time.
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                         // (zeros, and what is not finite, stay as they are)
                         const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
                         const float factor = power_of_two(e);
-                        if (chunk == 0) sh.q_factor[k & 1][row] = p.scale * E4M3_BITS_SCALE * power_of_two(-e) * (CAP ? 1.0f : LOG2E);
+                        if (chunk == 0) sh.q_factor[k & 1][row] = p.scale * power_of_two(-e) * (CAP ? 1.0f : LOG2E);
                         uint32_t h[4];
 #pragma unroll
                         for (int c = 0; c < 4; c++) h[c] = half2_of(__uint_as_float(w[c] << 16) * factor, __uint_as_float(w[c] & 0xffff0000u) * factor);
@@ -652,11 +654,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 unsigned char* k_tile = k_stage + s * GROUPS * GROUP_BYTES;
                 unsigned char* v_tile = v_stage + s * GROUPS * GROUP_BYTES;
                 const uint32_t absent = __ballot_sync(0xffffffffu, at < 0);
-                uint32_t none = put(k_tile, buffer[0]);
+                put(k_tile, buffer[0]);
                 const long at_next = row_of(id_next);
                 if (GROUPS == 2) {
                     fetch(buffer[0], p.v_pages, p.vdim, 0, at);
-                    none |= put(k_tile + GROUP_BYTES, buffer[1]);
+                    put(k_tile + GROUP_BYTES, buffer[1]);
                     fetch(buffer[1], p.v_pages, p.vdim, 1, at);
                 } else {
                     fetch(buffer[0], p.k_pages, p.dim, 0, at_next);
@@ -671,20 +673,21 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 if ((t & 15) == 0) {
                     sh.k_scale[s][t >> 4] = k_scale;
                     sh.v_exponent[s][t >> 4] = (float)exponent_of(v_scale);
-                    sh.v_inverse[s][t >> 4] = 1.0f / (E4M3_BITS_SCALE * v_scale);
+                    sh.v_inverse[s][t >> 4] = 1.0f / v_scale;
                 }
                 at = at_next;
                 scales();
+                const bool none = (buffer[GROUPS == 2 ? 0 : 1][0].x & 0x7fu) == 0x7fu;
                 if (GROUPS == 2) {
-                    none |= put(v_tile, buffer[0]);
+                    put_value(v_tile, buffer[0], none);
                     fetch(buffer[0], p.k_pages, p.dim, 0, at);
-                    none |= put(v_tile + GROUP_BYTES, buffer[1]);
+                    put_value(v_tile + GROUP_BYTES, buffer[1], none);
                     fetch(buffer[1], p.k_pages, p.dim, 1, at);
                 } else {
-                    none |= put(v_tile, buffer[1]);
+                    put_value(v_tile, buffer[1], none);
                     fetch(buffer[1], p.v_pages, p.vdim, 0, at);
                 }
-                const uint32_t nones = __ballot_sync(0xffffffffu, none != 0);
+                const uint32_t nones = __ballot_sync(0xffffffffu, none);
                 if (lane == 0) sh.absent[s][warp - SOFTMAX_WARPS] = absent, sh.none[s][warp - SOFTMAX_WARPS] = nones;
                 fence_async_smem();
                 __syncwarp();
