@@ -2,6 +2,7 @@
 // over it for single tokens (mma.sync tiles) and, as a plain twin for every size and type, for any row.
 #include "common.cuh"
 #include "e4m3.cuh"
+#include "mma_tiles.cuh"
 
 MLLM_DEFINE_ERROR_API(mllm_e4m3)
 
@@ -322,376 +323,462 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attention_plain_kernel(const E4
 
 // ---- attention of single tokens -----------------------------------------------------------------
 //
-// The entries of one token.  What bounds them is the cache: every visible code is read once.  A CTA takes a token, a key/value head with
-// up to 16 of its query heads, and a part of the keys; its eight warps take the blocks of 16 keys in turn.  A warp reads a block straight into
-// registers in the layout of mma.sync m16n8k16, the codes as 16-bit floats (each is one exactly):
-//   S = Q K^T: key g (of 8) and columns 16 c .. 16 c + 15 of it lie with lane 4 g + c: one load of 16 bytes, four products; the order of
-//     the columns within a product does not matter as long as Q has the same;
-//   O = P V: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 and columns 8 g .. 8 g + 7 of each: the pairs of keys are put together byte by byte.
+// The entries of one token.  What bounds them is the cache: every visible code is read once.  A unit is a token, a key/value head and up to
+// eight (sixteen) of its query heads; the units stand in a row, each as long as its blocks of 16 keys and a few more for its set-up, and every
+// CTA takes an equal stretch of it: requests of all lengths fill the SMs evenly, and one request alone does too.  A unit that lies in several
+// stretches leaves 32-bit results of its parts, which the CTA that arrives last adds up in order.
+//
+// Within a CTA eight warps take a unit's blocks in turn.  A warp has its next blocks on their way into shared memory (cp.async; in
+// registers one block ahead was all that fitted, 3.6 TB/s) and reads them in the layout of mma.sync m16n8k16, with the
+// codes as 16-bit floats (each is one exactly) and the query heads as the eight columns:
+//   S^T = K Q^T: keys g and g + 8 and columns 16 c .. 16 c + 15 of them lie with lane 4 g + c: 16 bytes each, four products; the
+//     order of the columns within a product does not matter as long as Q has the same;
+//   O^T = V^T P^T: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 and columns 8 g .. 8 g + 7 of each: the pairs of keys are put together byte by byte.
+// (With the heads as rows half of the products' rows are empty for up to eight heads: 632 instructions a block of 128 columns, 113 us for
+// 131,072 keys of 8 heads of 128; this way ... us.)
 // Q is scaled by a power of two to lie below 2^15 in 16-bit floats (11 bits: bfloat16's 8 fit; an entry 2^29 below the largest of its head
 // begins to lose some, where the 32-bit sum has lost it already).  The weights: a block's value scale 2^t joins the score as t in
 // the exponent, p = 2^(s + t - m + 7), and the sum of the weights gets p / 2^t: no multiplication more, and p keeps the 11 bits of a 16-bit
 // float however far apart the scales lie.  m moves only where a score passes it by 8, so that p stays below 2^15.
-constexpr int STEP_WARPS = 8, STEP_THREADS = STEP_WARPS * 32;
-constexpr int STEP_MIN_BLOCKS = 8;             // a part has a block of keys at least for every warp
+constexpr int STEP_WARPS = 8, STEP_THREADS = STEP_WARPS * 32, STEP_CTAS = 2;
+constexpr int STEP_SET_UP = 8;                 // blocks that a unit's set-up counts as
+constexpr int STEP_RING_BYTES = 96 * 1024;     // of a CTA's blocks on their way
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The same where rows 8 to 15 are empty: their sums are not kept.
-__device__ __forceinline__ void mma_f16_upper(float& c0, float& c1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-    [[maybe_unused]] float none0, none1;
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %6, %5, %6}, {%7, %8}, {%0, %1, %9, %9};"
-                 : "+f"(c0), "+f"(c1), "=f"(none0), "=f"(none1)
-                 : "r"(a0), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(0.0f));
+// An 8 x 8 tile of 16-bit numbers turned over.
+__device__ __forceinline__ uint32_t turned_tile(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 
-// KG, VG: groups of 64 columns of a key and a value; HALVES 1: at most eight query heads, 2: sixteen.
-template <int KG, int VG, int HALVES>
-__global__ void __launch_bounds__(STEP_THREADS, HALVES * VG <= 2 ? 2 : 1) attention_step_kernel(const E4m3Attention p, int head_tiles, int max_parts) {
-    extern __shared__ float shared[];
+// All units in a row; every warp works out the same.
+struct StepSchedule {
+    const E4m3Attention& p;
+    const int units_of_entry;
+    long total, stretch, lo, hi, begin;
+    int entry, unit, length, first_block, blocks, row, pos;
+
+    __device__ void of_position(int position, int& lowest, int& count) const {
+        const int first = p.window > 0 ? max(0, position - p.window + 1) : 0;
+        lowest = first / E4M3_BLOCK;
+        count = position >= 0 ? min(position / E4M3_BLOCK + 1, p.max_blocks * (p.page / E4M3_BLOCK)) - lowest : 0;
+        count = max(count, 0);
+    }
+    __device__ int length_of(int e) const {        // of an entry's units; 0: it has none
+        if (e >= p.n_items || p.item_count[e] != 1) return 0;
+        int lowest, count;
+        of_position(p.item_start[e], lowest, count);
+        return count + STEP_SET_UP;
+    }
+    __device__ void take(int e) {                  // the next unit is this entry's first
+        entry = e, unit = 0, row = p.item_offset[e], pos = p.item_start[e];
+        of_position(pos, first_block, blocks);
+        length = blocks + STEP_SET_UP;
+    }
+    __device__ StepSchedule(const E4m3Attention& params, int units, int lane) : p(params), units_of_entry(units), total(0) {
+        int most = 0;
+        for (int base = 0; base < p.n_items; base += 32) {
+            const int n = length_of(base + lane);
+            total += __reduce_add_sync(0xffffffffu, n);
+            most = max(most, __reduce_max_sync(0xffffffffu, n));
+        }
+        total *= units_of_entry;
+        // (no shorter than a block a warp, where units are longer than that)
+        stretch = max((total + gridDim.x - 1) / gridDim.x, (long)min(most, STEP_WARPS + STEP_SET_UP));
+        lo = blockIdx.x * stretch, hi = min(total, lo + stretch);
+        begin = 0;
+        if (lo >= hi) return;
+        for (int base = 0;; base += 32) {
+            const int mine = length_of(base + lane);
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, begin + (long)upto * units_of_entry > lo);
+            if (past != 0) {
+                const int at = __ffs(past) - 1;
+                begin += (long)__shfl_sync(0xffffffffu, upto - mine, at) * units_of_entry;
+                take(base + at);
+                unit = (int)((lo - begin) / length);
+                begin += (long)unit * length;
+                return;
+            }
+            begin += (long)__shfl_sync(0xffffffffu, upto, 31) * units_of_entry;
+        }
+    }
+    __device__ bool more() const { return lo < hi && begin < hi; }      // (CTAs behind the row's end have nothing)
+    __device__ void next() {
+        begin += length;
+        if (++unit == units_of_entry && begin < hi) {
+            int e = entry + 1;
+            while (p.item_count[e] != 1) e++;      // (the row goes on, so there is one)
+            take(e);
+        }
+    }
+};
+
+// KG, VG: groups of 64 columns of a key and a value, which they fill where EXACT; TILES: of eight query heads.
+template <int KG, int VG, int TILES, bool EXACT>
+__global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel(const E4m3Attention p, int head_tiles, int stages) {
+    extern __shared__ __align__(128) float shared[];
+    __shared__ uint4 q_parts[TILES][KG][2][32];  // the queries in the products' layout, the same for all warps
+    __shared__ float q_factors[8 * TILES];       // what brings a score into powers of two
     __shared__ int ticket;
     dependents_may_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int entry = blockIdx.z, kv_head = blockIdx.y / head_tiles, head_tile = blockIdx.y % head_tiles, part = blockIdx.x;
-    const int group = p.n_heads / p.n_kv_heads;
-    const int n_rows = min(8 * HALVES, group - head_tile * 8 * HALVES);
-    const int head0 = kv_head * group + head_tile * 8 * HALVES;
+    const int dim = EXACT ? 64 * KG : p.dim, vdim = EXACT ? 64 * VG : p.vdim;
+    const int group = p.n_heads / p.n_kv_heads, per_page = p.page / E4M3_BLOCK;
+    constexpr float LOG2E = 1.4426950408889634f;
+    constexpr int WIDTH = 64 * VG, ROWS = 8 * TILES;
+    const bool has_cap = p.cap > 0.0f;
+    const float cap_factor = has_cap ? 2.0f * LOG2E / p.cap : 0.0f, cap_log2 = p.cap * LOG2E;
+    // a warp's ring: blocks, each behind its scales
+    const int stage_bytes = 128 + E4M3_BLOCK * (dim + vdim);
+    unsigned char* ring = reinterpret_cast<unsigned char*>(shared) + warp * stages * stage_bytes + 112;
     wait_for_earlier_kernels();
-    if (p.item_count[entry] != 1) return;
-    const int row = p.item_offset[entry], pos = p.item_start[entry];
-    const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-    const int block_lo = first / E4M3_BLOCK;
-    const int n_blocks = pos >= 0 ? min(pos / E4M3_BLOCK + 1, p.max_blocks * (p.page / E4M3_BLOCK)) - block_lo : 0;
-    const int per_part = max(STEP_MIN_BLOCKS, (n_blocks + max_parts - 1) / max_parts);
-    const int n_parts = max(1, (n_blocks + per_part - 1) / per_part);
-    if (part >= n_parts) return;
-    const int lo = block_lo + part * per_part, hi = min(lo + per_part, block_lo + n_blocks);
+    const uint8_t* k_pages = behind_the_wait(p.k_pages);
+    const uint8_t* v_pages = behind_the_wait(p.v_pages);
+    for (StepSchedule at(p, p.n_kv_heads * head_tiles, lane); at.more(); at.next()) {
+        const int kv_head = at.unit / head_tiles, head_tile = at.unit - kv_head * head_tiles;
+        const int n_rows = min(ROWS, group - head_tile * ROWS), head0 = kv_head * group + head_tile * ROWS;
+        const int pos = at.pos, first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        // places of the unit in this stretch: the set-up's, then a block each
+        const int from = (int)(max(at.lo, at.begin) - at.begin), to = (int)(min(at.hi, at.begin + at.length) - at.begin);
+        const int lo = at.first_block + max(0, from - STEP_SET_UP), hi = at.first_block + max(0, to - STEP_SET_UP);
+        const int first_cta = (int)(at.begin / at.stretch), n_parts = (int)((at.begin + at.length - 1) / at.stretch) - first_cta + 1;
+        const int part = (int)blockIdx.x - first_cta;
 
-    // the queries, as 16-bit floats of a power of two's size, in the order of the key's columns (in shared memory: all warps have the same)
-    const bf16* q = static_cast<const bf16*>(p.q) + row * p.ld_q;
-    __shared__ uint4 qa[HALVES][KG][2][32];
-    float q_factor[HALVES];                      // what brings a score into powers of two
-#pragma unroll
-    for (int h = 0; h < HALVES; h++) {
-        const int r = g + 8 * h;
-        float x[KG][16], top = 0.0f;
-#pragma unroll
-        for (int d = 0; d < KG; d++) {
-            const int col = 64 * d + 16 * c;
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[d][i] = 0.0f;
-            if (r < n_rows && col < p.dim) {
-                const uint4* at = reinterpret_cast<const uint4*>(q + (long)(head0 + r) * p.dim + col);
-                const uint4 u = at[0], v = at[1];
-                const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[d][2 * i] = __uint_as_float(w[i] << 16), x[d][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        // Lane i looks up the warp's next 32 blocks, and the 32 after them ahead: where block i lies (in blocks), and its scales.
+        const int* table = p.block_table + (long)at.entry * p.max_blocks;
+        struct Places {
+            int place;
+            float k_scale, v_scale;
+        } here, ahead;
+        auto look_up = [&](int begins) {
+            Places x = {-1, 0.0f, 0.0f};
+            const int b = begins + lane * STEP_WARPS;
+            if (b < hi) {
+                const int index = b / per_page, id = table[index];
+                if (id >= 0 && id < p.n_pages) {
+                    x.place = (id * p.n_kv_heads + kv_head) * per_page + b - index * per_page;
+                    x.k_scale = p.k_scales[x.place];
+                    x.v_scale = p.v_scales[x.place];
+                }
             }
+            return x;
+        };
+        const int mine = lo + warp < hi ? (hi - lo - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
+        here = look_up(lo + warp);
+        ahead = look_up(lo + warp + 32 * STEP_WARPS);
+        // A block on its way: 16-byte chunks, each row's in an order in which no two lanes below read the same banks.
+        auto fetch = [&](int i) {                        // the warp's i-th block, into the ring's place i % stages
+            if (i < mine) {
+                if (i > 0 && (i & 31) == 0) {
+                    here = ahead;
+                    ahead = look_up(lo + warp + (i + 32) * STEP_WARPS);
+                }
+                const int place = __shfl_sync(0xffffffffu, here.place, i & 31);
+                const float k_scale = __shfl_sync(0xffffffffu, here.k_scale, i & 31), v_scale = __shfl_sync(0xffffffffu, here.v_scale, i & 31);
+                unsigned char* to = ring + (i % stages) * stage_bytes;
+                if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(k_scale, place >= 0 ? v_scale : 0.0f);     // (no scale: not there)
+                if (place >= 0) {
+                    const uint8_t* k = k_pages + (long)place * E4M3_BLOCK * dim;
+                    const uint8_t* v = v_pages + (long)place * E4M3_BLOCK * vdim;
+                    to += 16;
+                    if constexpr (EXACT) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(x[d][i]));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // (zeros, and what is not finite, stay as they are)
-        const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
-        const float factor = power_of_two(e);
-        q_factor[h] = p.scale * power_of_two(-e);
-        if (warp == 0)
+                        for (int n = 0; n < 2 * KG; n++) {
+                            const int x = lane + 32 * n, key = x / (4 * KG);
+                            copy_16(to + 16 * (x ^ (KG == 2 ? (key & 1) << 2 : 0)), k + 16 * x, true);
+                        }
+                        to += E4M3_BLOCK * dim;
+#pragma unroll
+                        for (int n = 0; n < 2 * VG; n++) {
+                            const int x = lane + 32 * n, key = x / (4 * VG);
+                            copy_16(to + 16 * (x ^ (((key >> 1) & 3) << 1)), v + 16 * x, true);
+                        }
+                    } else {
+                        for (int x = lane; x < dim; x += 32) copy_16(to + 16 * x, k + 16 * x, true);
+                        to += E4M3_BLOCK * dim;
+                        for (int x = lane; x < vdim; x += 32) copy_16(to + 16 * x, v + 16 * x, true);
+                    }
+                }
+            }
+            copies_end();
+        };
+        for (int i = 0; i < stages - 1; i++) fetch(i);
+
+        // the queries of tile `warp`: 16-bit floats of a power of two's size, head g, in the order of the key's columns
+        if (warp < TILES) {
+            const int r = g + 8 * warp;
+            float x[KG][16], top = 0.0f;
+#pragma unroll
+            for (int d = 0; d < KG; d++) {
+                const int col = 64 * d + 16 * c;
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[d][i] = 0.0f;
+                if (r < n_rows && col < dim) {
+                    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + at.row * p.ld_q + (long)(head0 + r) * dim + col);
+                    const uint4 u = q[0], v = q[1];
+                    const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[d][2 * i] = __uint_as_float(w[i] << 16), x[d][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(x[d][i]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // (zeros, and what is not finite, stay as they are)
+            const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
+            const float factor = power_of_two(e);
+            if (c == 0) q_factors[r] = p.scale * power_of_two(-e) * (has_cap ? 1.0f : LOG2E);
 #pragma unroll
             for (int d = 0; d < KG; d++)
 #pragma unroll
                 for (int s = 0; s < 2; s++)
-                    qa[h][d][s][lane] = make_uint4(half2_of(x[d][8 * s] * factor, x[d][8 * s + 1] * factor),
-                                                   half2_of(x[d][8 * s + 2] * factor, x[d][8 * s + 3] * factor),
-                                                   half2_of(x[d][8 * s + 4] * factor, x[d][8 * s + 5] * factor),
-                                                   half2_of(x[d][8 * s + 6] * factor, x[d][8 * s + 7] * factor));
-    }
-    __syncthreads();
-    constexpr float LOG2E = 1.4426950408889634f;
-    const bool has_cap = p.cap > 0.0f;
-    if (!has_cap)
-        for (int h = 0; h < HALVES; h++) q_factor[h] *= LOG2E;
-    const float cap_factor = has_cap ? 2.0f * LOG2E / p.cap : 0.0f, cap_log2 = p.cap * LOG2E;
-
-    float acc[VG][8][2 * HALVES], m[HALVES], l[HALVES];
-#pragma unroll
-    for (int d = 0; d < VG; d++)
-#pragma unroll
-        for (int t = 0; t < 8; t++)
-#pragma unroll
-            for (int i = 0; i < 2 * HALVES; i++) acc[d][t][i] = 0.0f;
-#pragma unroll
-    for (int h = 0; h < HALVES; h++) m[h] = -INFINITY, l[h] = 0.0f;
-
-    const int per_page = p.page / E4M3_BLOCK;
-    const int* table = p.block_table + (long)entry * p.max_blocks;
-    const uint8_t* k_pages = behind_the_wait(p.k_pages);
-    const uint8_t* v_pages = behind_the_wait(p.v_pages);
-    // Lane i looks up the warp's next 32 blocks: where block i lies (in blocks), and its scales.
-    long of_lane = -1;
-    float k_scale_of_lane = 0.0f, v_scale_of_lane = 0.0f;
-    auto look_up = [&](int from) {
-        const int b = from + lane * STEP_WARPS;
-        of_lane = -1;
-        if (b < hi) {
-            const int id = table[b / per_page];
-            if (id >= 0 && id < p.n_pages) {
-                of_lane = ((long)id * p.n_kv_heads + kv_head) * per_page + b % per_page;
-                k_scale_of_lane = p.k_scales[of_lane];
-                v_scale_of_lane = p.v_scales[of_lane];
-            }
+                    q_parts[warp][d][s][lane] = make_uint4(half2_of(x[d][8 * s] * factor, x[d][8 * s + 1] * factor),
+                                                           half2_of(x[d][8 * s + 2] * factor, x[d][8 * s + 3] * factor),
+                                                           half2_of(x[d][8 * s + 4] * factor, x[d][8 * s + 5] * factor),
+                                                           half2_of(x[d][8 * s + 6] * factor, x[d][8 * s + 7] * factor));
         }
-    };
-    struct Block {
-        uint4 k[2][KG];
-        uint2 v[4][VG];
-        float k_scale, v_scale;
-        bool there;
-    };
-    auto fetch = [&](Block& b, int i) {                  // the i-th of the blocks that were looked up
-        const long at = __shfl_sync(0xffffffffu, of_lane, i);
-        b.k_scale = __shfl_sync(0xffffffffu, k_scale_of_lane, i);
-        b.v_scale = __shfl_sync(0xffffffffu, v_scale_of_lane, i);
-        b.there = at >= 0;
-        const uint8_t* k = k_pages + at * E4M3_BLOCK * p.dim;
-        const uint8_t* v = v_pages + at * E4M3_BLOCK * p.vdim;
+        __syncthreads();
+        // heads 2 c and 2 c + 1 of every tile are this lane's
+        float q_factor[TILES][2], m[TILES][2], l[TILES][2], acc[TILES][VG][4][4];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < TILES; h++) {
 #pragma unroll
-            for (int d = 0; d < KG; d++) {
-                const int col = 64 * d + 16 * c;
-                b.k[h][d] = make_uint4(0u, 0u, 0u, 0u);
-                if (b.there && col < p.dim) b.k[h][d] = __ldcs(reinterpret_cast<const uint4*>(k + (8 * h + g) * p.dim + col));
-            }
+            for (int e = 0; e < 2; e++) q_factor[h][e] = q_factors[8 * h + 2 * c + e], m[h][e] = -INFINITY, l[h][e] = 0.0f;
 #pragma unroll
-        for (int i4 = 0; i4 < 4; i4++)
+            for (int i = 0; i < 16 * VG; i++) acc[h][i / 16][(i / 4) & 3][i & 3] = 0.0f;
+        }
+
+        auto work = [&](const unsigned char* from, int index) {
+            const float2 scales = *reinterpret_cast<const float2*>(from);
+            const float k_scale = scales.x, v_scale = scales.y;
+            if (v_scale == 0.0f) return;
+            const unsigned char* k = from + 16;
+            const unsigned char* v = k + E4M3_BLOCK * dim;
+            float s[TILES][4];
 #pragma unroll
-            for (int d = 0; d < VG; d++) {
-                const int col = 64 * d + 8 * g, key = 2 * c + (i4 & 1) + 8 * (i4 >> 1);
-                b.v[i4][d] = make_uint2(0u, 0u);
-                if (b.there && col < p.vdim) b.v[i4][d] = __ldcs(reinterpret_cast<const uint2*>(v + key * p.vdim + col));
-            }
-    };
-    auto work = [&](Block& b, int index) {
-        if (!b.there) return;
-        float s[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.0f;
+            for (int h = 0; h < TILES; h++) s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.0f;
 #pragma unroll
             for (int d = 0; d < KG; d++) {
-                const uint32_t w[4] = {b.k[h][d].x, b.k[h][d].y, b.k[h][d].z, b.k[h][d].w};
+                uint4 rows[2];                           // columns 64 d + 16 c .. of keys g and g + 8
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const int key = g + 8 * n, col = 64 * d + 16 * c;
+                    if (EXACT) rows[n] = *reinterpret_cast<const uint4*>(k + key * dim + (col ^ (KG == 2 ? (key & 1) << 6 : 0)));
+                    else rows[n] = col < dim ? *reinterpret_cast<const uint4*>(k + key * dim + col) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                const uint32_t x[4] = {rows[0].x, rows[0].y, rows[0].z, rows[0].w}, y[4] = {rows[1].x, rows[1].y, rows[1].z, rows[1].w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const uint4 lower = qa[0][d][i >> 1][lane], upper = qa[HALVES - 1][d][i >> 1][lane];
-                    uint32_t b0, b1;
-                    e4m3_to_half2(w[i], b0, b1);
-                    if (HALVES == 1) mma_f16_upper(s[h][0], s[h][1], (i & 1) ? lower.z : lower.x, (i & 1) ? lower.w : lower.y, b0, b1);
-                    else mma_f16(s[h], (i & 1) ? lower.z : lower.x, (i & 1) ? upper.z : upper.x, (i & 1) ? lower.w : lower.y, (i & 1) ? upper.w : upper.y, b0, b1);
-                }
-            }
-        }
-        const float t = (float)exponent_of(b.v_scale), over = 1.0f / b.v_scale;
-        const int key0 = index * E4M3_BLOCK;
-        const bool partial = key0 + E4M3_BLOCK - 1 > pos || key0 < first;
-        // the weights of rows g and g + 8, keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-        uint32_t pa[HALVES][2];
-        float x[HALVES][4], top[HALVES];
-        bool moves = false;
+                    uint32_t a[4];
+                    e4m3_to_half2(x[i], a[0], a[2]);
+                    e4m3_to_half2(y[i], a[1], a[3]);
 #pragma unroll
-        for (int h = 0; h < HALVES; h++) {
-            const float factor = q_factor[h] * b.k_scale;
-            top[h] = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float y = s[i >> 1][2 * h + (i & 1)] * factor;
-                y = has_cap ? capped(y, cap_log2, cap_factor) + t : y + t;
-                const int key = key0 + 2 * c + (i & 1) + 8 * (i >> 1);
-                if (partial && (key > pos || key < first)) y = -INFINITY;
-                x[h][i] = y;
-                top[h] = fmaxf(top[h], y);
-            }
-            moves = moves || top[h] > m[h] + 8.0f;
-        }
-        if (__any_sync(0xffffffffu, moves)) {
-#pragma unroll
-            for (int h = 0; h < HALVES; h++) {
-                float most = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                most = fmaxf(m[h], fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)));
-                const float down = m[h] == -INFINITY ? 0.0f : exp2_fast(m[h] - most);
-                m[h] = most;
-                l[h] *= down;
-#pragma unroll
-                for (int d = 0; d < VG; d++)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc[d][i][2 * h] *= down, acc[d][i][2 * h + 1] *= down;
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < HALVES; h++) {
-            const float base = (m[h] == -INFINITY ? 0.0f : m[h]) - 7.0f;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[h][i] = exp2_fast(x[h][i] - base);
-                sum += x[h][i];
-            }
-            l[h] += sum * over;
-            pa[h][0] = half2_of(x[h][0], x[h][1]);
-            pa[h][1] = half2_of(x[h][2], x[h][3]);
-        }
-        if (partial) {
-            // a masked key's value may be no number, and its weight of zero would not keep it out
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int key = key0 + 2 * c + (i & 1) + 8 * (i >> 1);
-                if (key > pos || key < first)
-#pragma unroll
-                    for (int d = 0; d < VG; d++) b.v[i][d] = make_uint2(0u, 0u);
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < VG; d++)
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                const uint32_t v0 = w ? b.v[0][d].y : b.v[0][d].x, v1 = w ? b.v[1][d].y : b.v[1][d].x;
-                const uint32_t v2 = w ? b.v[2][d].y : b.v[2][d].x, v3 = w ? b.v[3][d].y : b.v[3][d].x;
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    // columns 2 half and 2 half + 1 of the four: (key a, key b) of the one, then of the other
-                    const uint32_t order = half ? 0x7362 : 0x5140;
-                    uint32_t b00, b01, b10, b11;
-                    e4m3_to_half2(__byte_perm(v0, v1, order), b00, b01);
-                    e4m3_to_half2(__byte_perm(v2, v3, order), b10, b11);
-                    float(&even)[2 * HALVES] = acc[d][4 * w + 2 * half];
-                    float(&odd)[2 * HALVES] = acc[d][4 * w + 2 * half + 1];
-                    if constexpr (HALVES == 1) {
-                        mma_f16_upper(even[0], even[1], pa[0][0], pa[0][1], b00, b10);
-                        mma_f16_upper(odd[0], odd[1], pa[0][0], pa[0][1], b01, b11);
-                    } else {
-                        mma_f16(even, pa[0][0], pa[1][0], pa[0][1], pa[1][1], b00, b10);
-                        mma_f16(odd, pa[0][0], pa[1][0], pa[0][1], pa[1][1], b01, b11);
+                    for (int h = 0; h < TILES; h++) {
+                        const uint4 q = q_parts[h][d][i >> 1][lane];
+                        mma_f16(s[h], a, (i & 1) ? q.z : q.x, (i & 1) ? q.w : q.y);
                     }
                 }
             }
-    };
-    // two blocks on their way while one is worked on
-    int taken = 0;
-    Block a, b;
-    const int mine = lo + warp < hi ? (hi - lo - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
-    auto next = [&](Block& x) {
-        if (taken >= mine) return;
-        if ((taken & 31) == 0) look_up(lo + warp + taken * STEP_WARPS);
-        fetch(x, taken & 31);
-        taken++;
-    };
-    next(a);
-    for (int i = 0; i < mine; i += 2) {
-        next(b);
-        work(a, lo + warp + i * STEP_WARPS);
-        next(a);
-        if (i + 1 < mine) work(b, lo + warp + (i + 1) * STEP_WARPS);
-    }
+            const float t = (float)exponent_of(v_scale), over = 1.0f / v_scale;
+            const int key0 = index * E4M3_BLOCK;
+            const bool partial = key0 + E4M3_BLOCK - 1 > pos || key0 < first;
+            // scores of key g, heads 2 c and 2 c + 1, then of key g + 8
+            float top[TILES][2];
+            bool moves = false;
+#pragma unroll
+            for (int h = 0; h < TILES; h++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float factor = q_factor[h][e] * k_scale;
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const float y = s[h][2 * n + e] * factor;
+                        s[h][2 * n + e] = has_cap ? capped(y, cap_log2, cap_factor) + t : y + t;
+                    }
+                    if (partial) {
+                        if (key0 + g > pos || key0 + g < first) s[h][e] = -INFINITY;
+                        if (key0 + g + 8 > pos || key0 + g + 8 < first) s[h][2 + e] = -INFINITY;
+                    }
+                    top[h][e] = fmaxf(s[h][e], s[h][2 + e]);
+                    moves = moves || top[h][e] > m[h][e] + 8.0f;
+                }
+            if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+                for (int h = 0; h < TILES; h++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float most = top[h][e];
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        most = fmaxf(m[h][e], most);
+                        const float down = m[h][e] == -INFINITY ? 0.0f : exp2_fast(m[h][e] - most);
+                        m[h][e] = most;
+                        l[h][e] *= down;
+#pragma unroll
+                        for (int d = 0; d < VG; d++)
+#pragma unroll
+                            for (int n = 0; n < 4; n++) acc[h][d][n][e] *= down, acc[h][d][n][2 + e] *= down;
+                    }
+            }
+            uint32_t weights[TILES][2];
+#pragma unroll
+            for (int h = 0; h < TILES; h++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float base = (m[h][e] == -INFINITY ? 0.0f : m[h][e]) - 7.0f;
+                    s[h][e] = exp2_fast(s[h][e] - base);
+                    s[h][2 + e] = exp2_fast(s[h][2 + e] - base);
+                    l[h][e] = fmaf(s[h][e] + s[h][2 + e], over, l[h][e]);
+                }
+                weights[h][0] = turned_tile(half2_of(s[h][0], s[h][1]));
+                weights[h][1] = turned_tile(half2_of(s[h][2], s[h][3]));
+            }
+#pragma unroll
+            for (int d = 0; d < VG; d++) {
+                uint2 rows[4];                           // columns 64 d + 8 g .. of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const int key = 2 * c + (n & 1) + 8 * (n >> 1), col = 64 * d + 8 * g;
+                    if (EXACT) rows[n] = *reinterpret_cast<const uint2*>(v + ((key * vdim + col) ^ (((key >> 1) & 3) << 5)));
+                    else rows[n] = col < vdim ? *reinterpret_cast<const uint2*>(v + key * vdim + col) : make_uint2(0u, 0u);
+                    // (a masked key's value may be no number, and its weight of zero would not keep it out)
+                    if (partial && (key0 + key > pos || key0 + key < first)) rows[n] = make_uint2(0u, 0u);
+                }
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    // columns 2 n and 2 n + 1 of the eight: keys a and b of the one, then of the other
+                    const uint32_t order = (n & 1) ? 0x7362 : 0x5140;
+                    uint32_t a[4];
+                    e4m3_to_half2(__byte_perm(n >> 1 ? rows[0].y : rows[0].x, n >> 1 ? rows[1].y : rows[1].x, order), a[0], a[1]);
+                    e4m3_to_half2(__byte_perm(n >> 1 ? rows[2].y : rows[2].x, n >> 1 ? rows[3].y : rows[3].x, order), a[2], a[3]);
+#pragma unroll
+                    for (int h = 0; h < TILES; h++) mma_f16(acc[h][d][n], a, weights[h][0], weights[h][1]);
+                }
+            }
+        };
+        for (int i = 0; i < mine; i++) {
+            // block i has landed (as many groups behind it are on their way as the ring has places but two), and all lanes have left block i - 1
+            if (stages == 4) copies_landed<2>();
+            else if (stages == 3) copies_landed<1>();
+            else copies_landed<4>();
+            __syncwarp();
+            fetch(i + stages - 1);
+            work(ring + (i % stages) * stage_bytes, lo + warp + i * STEP_WARPS);
+        }
+        copies_landed<0>();
+        __syncthreads();                                 // the ring's memory is the results' now
 
-    // the warps' results: rows of [vdim] sums, then the maxima and the sums of the weights
-    const int width = 64 * VG;
-    float* of_m = shared + STEP_WARPS * n_rows * width;
-    float* of_l = of_m + STEP_WARPS * n_rows;
+        // the warps' results: rows of sums, then the maxima and the sums of the weights
+        float* of_m = shared + STEP_WARPS * n_rows * WIDTH;
+        float* of_l = of_m + STEP_WARPS * n_rows;
 #pragma unroll
-    for (int h = 0; h < HALVES; h++) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        const int r = g + 8 * h;
-        // (lanes of a row agree on its maximum, but for rows whose scores never passed a warp's vote)
-        if (r < n_rows) {
-            if (c == 0) of_m[warp * n_rows + r] = m[h], of_l[warp * n_rows + r] = l[h];
-            float* to = shared + (warp * n_rows + r) * width;
+        for (int h = 0; h < TILES; h++)
 #pragma unroll
-            for (int d = 0; d < VG; d++)
+            for (int e = 0; e < 2; e++) {
 #pragma unroll
-                for (int t = 0; t < 8; t += 4)
+                for (int o = 4; o < 32; o <<= 1) l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], o);
+                const int r = 8 * h + 2 * c + e;
+                if (r < n_rows) {
+                    if (g == 0) of_m[warp * n_rows + r] = m[h][e], of_l[warp * n_rows + r] = l[h][e];
+                    float* sums = shared + (warp * n_rows + r) * WIDTH + 8 * g;
 #pragma unroll
-                    for (int e = 0; e < 2; e++)
-                        *reinterpret_cast<float4*>(to + 64 * d + 16 * c + 8 * e + t) =
-                            make_float4(acc[d][t][2 * h + e], acc[d][t + 1][2 * h + e], acc[d][t + 2][2 * h + e], acc[d][t + 3][2 * h + e]);
+                    for (int d = 0; d < VG; d++)
+#pragma unroll
+                        for (int n = 0; n < 4; n += 2)
+                            *reinterpret_cast<float4*>(sums + 64 * d + 2 * n) =
+                                make_float4(acc[h][d][n][e], acc[h][d][n][2 + e], acc[h][d][n + 1][e], acc[h][d][n + 1][2 + e]);
+                }
+            }
+        __syncthreads();
+        bf16* out = static_cast<bf16*>(p.out) + at.row * p.ld_out + (long)head0 * vdim;
+        // A part that begins a unit is its CTA's last and has the second of the CTA's two places; any other is its first.
+        constexpr int PART = ROWS * (WIDTH + 2);
+        auto cell = [&](int q) { return p.partial + (long)(2 * (first_cta + q) + (q == 0 ? 1 : 0)) * PART; };
+        for (int i = threadIdx.x; i < n_rows * WIDTH; i += STEP_THREADS) {
+            const int r = i / WIDTH, col = i - r * WIDTH;
+            float top = -INFINITY, sum = 0.0f, weight_sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < STEP_WARPS; w++) top = fmaxf(top, of_m[w * n_rows + r]);
+            const float anchor = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < STEP_WARPS; w++) {
+                const float weight = exp2_fast(of_m[w * n_rows + r] - anchor);
+                sum += weight * shared[(w * n_rows + r) * WIDTH + col];
+                weight_sum += weight * of_l[w * n_rows + r];
+            }
+            if (n_parts == 1) {
+                if (col < vdim) out[r * vdim + col] = __float2bfloat16_rn(weight_sum == 0.0f ? 0.0f : sum / weight_sum);
+            } else {
+                float* here = cell(part);
+                __stcg(here + i, sum);
+                if (col == 0) __stcg(here + ROWS * WIDTH + 2 * r, top), __stcg(here + ROWS * WIDTH + 2 * r + 1, weight_sum);
+            }
         }
-    }
-    __syncthreads();
-    bf16* out = static_cast<bf16*>(p.out) + row * p.ld_out + (long)head0 * p.vdim;
-    const int cell = entry * gridDim.y + blockIdx.y, part_floats = 8 * HALVES * (width + 2);
-    float* all = p.partial + (long)cell * max_parts * part_floats;
-    float* mine_out = all + (long)part * part_floats;
-    for (int i = threadIdx.x; i < n_rows * width; i += STEP_THREADS) {
-        const int r = i / width, col = i - r * width;
-        float top = -INFINITY, sum = 0.0f, total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < STEP_WARPS; w++) top = fmaxf(top, of_m[w * n_rows + r]);
-        const float anchor = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int w = 0; w < STEP_WARPS; w++) {
-            const float weight = exp2_fast(of_m[w * n_rows + r] - anchor);
-            sum += weight * shared[(w * n_rows + r) * width + col];
-            total += weight * of_l[w * n_rows + r];
-        }
-        if (n_parts == 1) {
-            if (col < p.vdim) out[r * p.vdim + col] = __float2bfloat16_rn(total == 0.0f ? 0.0f : sum / total);
-        } else {
-            __stcg(mine_out + i, sum);
-            if (col == 0) __stcg(mine_out + 8 * HALVES * width + 2 * r, top), __stcg(mine_out + 8 * HALVES * width + 2 * r + 1, total);
-        }
-    }
-    if (n_parts == 1) return;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) ticket = atomicAdd(p.counters + cell, 1);
-    __syncthreads();
-    if (ticket != n_parts - 1) return;
-    __threadfence();
-    // the last to arrive adds the parts up, in their order
-    for (int i = threadIdx.x; i < n_rows * width; i += STEP_THREADS) {
-        const int r = i / width, col = i - r * width;
-        const float* state = all + 8 * HALVES * width + 2 * r;
-        float top = -INFINITY, sum = 0.0f, total = 0.0f;
-        for (int q = 0; q < n_parts; q++) top = fmaxf(top, __ldcg(state + (long)q * part_floats));
-        const float anchor = top == -INFINITY ? 0.0f : top;
+        if (n_parts > 1) {
+            __threadfence();
+            __syncthreads();
+            int* counter = p.counters + first_cta;
+            if (threadIdx.x == 0) ticket = atomicAdd(counter, 1);
+            __syncthreads();
+            if (ticket == n_parts - 1) {
+                __threadfence();
+                // the last to arrive adds the parts up, in their order
+                for (int i = threadIdx.x; i < n_rows * WIDTH; i += STEP_THREADS) {
+                    const int r = i / WIDTH, col = i - r * WIDTH;
+                    float top = -INFINITY, sum = 0.0f, weight_sum = 0.0f;
+                    for (int q = 0; q < n_parts; q++) top = fmaxf(top, __ldcg(cell(q) + ROWS * WIDTH + 2 * r));
+                    const float anchor = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
-        for (int q = 0; q < n_parts; q++) {
-            const float weight = exp2_fast(__ldcg(state + (long)q * part_floats) - anchor);
-            sum += weight * __ldcg(all + (long)q * part_floats + i);
-            total += weight * __ldcg(state + (long)q * part_floats + 1);
+                    for (int q = 0; q < n_parts; q++) {
+                        const float* theirs = cell(q);
+                        const float weight = exp2_fast(__ldcg(theirs + ROWS * WIDTH + 2 * r) - anchor);
+                        sum += weight * __ldcg(theirs + i);
+                        weight_sum += weight * __ldcg(theirs + ROWS * WIDTH + 2 * r + 1);
+                    }
+                    if (col < vdim) out[r * vdim + col] = __float2bfloat16_rn(weight_sum == 0.0f ? 0.0f : sum / weight_sum);
+                }
+                if (threadIdx.x == 0) *counter = 0;
+            }
         }
-        if (col < p.vdim) out[r * p.vdim + col] = __float2bfloat16_rn(total == 0.0f ? 0.0f : sum / total);
+        __syncthreads();                                 // (shared memory is the next unit's)
     }
-    if (threadIdx.x == 0) p.counters[cell] = 0;
 }
 
-template <int KG, int VG, int HALVES>
+template <int KG, int VG, int TILES, bool EXACT>
 int launch_step(const E4m3Attention& p, int n_sms, cudaStream_t stream) {
-    const int group = p.n_heads / p.n_kv_heads, rows = min(group, 8 * HALVES);
-    const int head_tiles = (group + 8 * HALVES - 1) / (8 * HALVES);
-    const long cells = (long)p.n_items * p.n_kv_heads * head_tiles;
-    const int parts = (int)max(1L, min(64L, 2L * n_sms / cells));
-    const size_t bytes = STEP_WARPS * rows * (64 * VG + 2) * sizeof(float);
-    static_assert(STEP_WARPS * 16 * (128 + 2) * 4 <= 100 * 1024, "two CTAs of the largest size share an SM");
-    auto kernel = attention_step_kernel<KG, VG, HALVES>;
-    if (bytes > 48 * 1024) {
+    const int group = p.n_heads / p.n_kv_heads, rows = min(group, 8 * TILES);
+    const int head_tiles = (group + 8 * TILES - 1) / (8 * TILES);
+    const int stage_bytes = 128 + E4M3_BLOCK * (p.dim + p.vdim), of_all = STEP_WARPS * stage_bytes;
+    const int stages = of_all * 6 <= STEP_RING_BYTES ? 6 : of_all * 4 <= STEP_RING_BYTES ? 4 : 3;
+    const size_t bytes = max((size_t)stages * of_all, STEP_WARPS * rows * (64 * VG + 2) * sizeof(float));
+    static_assert(STEP_WARPS * 16 * (128 + 2) * 4 <= 100 * 1024 && 3 * STEP_WARPS * (128 + 16 * 256) <= 104 * 1024, "two CTAs of the largest size share an SM");
+    auto kernel = attention_step_kernel<KG, VG, TILES, EXACT>;
+    if (bytes > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e != cudaSuccess) return launched(e, "attention_step");
+        if (e != cudaSuccess) return launched(e, "e4m3_attention_step");
     }
-    return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(parts, p.n_kv_heads * head_tiles, p.n_items), dim3(STEP_THREADS),
-                                  bytes, stream, p, head_tiles, parts),
-                    "attention_step");
+    return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(STEP_CTAS * n_sms), dim3(STEP_THREADS), bytes, stream, p, head_tiles, stages),
+                    "e4m3_attention_step");
 }
 
-template <int HALVES>
+template <int TILES>
 int launch_step_of(const E4m3Attention& p, int n_sms, cudaStream_t stream) {
-    if (p.dim <= 64 && p.vdim <= 64) return launch_step<1, 1, HALVES>(p, n_sms, stream);
-    if (p.dim <= 64) return launch_step<1, 2, HALVES>(p, n_sms, stream);
-    if (p.vdim <= 64) return launch_step<2, 1, HALVES>(p, n_sms, stream);
-    return launch_step<2, 2, HALVES>(p, n_sms, stream);
+    if (p.dim == 64 && p.vdim == 64) return launch_step<1, 1, TILES, true>(p, n_sms, stream);
+    if (p.dim == 128 && p.vdim == 128) return launch_step<2, 2, TILES, true>(p, n_sms, stream);
+    if (p.dim <= 64 && p.vdim <= 64) return launch_step<1, 1, TILES, false>(p, n_sms, stream);
+    return launch_step<2, 2, TILES, false>(p, n_sms, stream);
 }
 
 }  // namespace
