@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attention_plain_kernel(const E4
 // float however far apart the scales lie.  m moves only where a score passes it by 8, so that p stays below 2^15.
 constexpr int STEP_WARPS = 8, STEP_THREADS = STEP_WARPS * 32, STEP_CTAS = 2;
 constexpr int STEP_SET_UP = 8;                 // blocks that a unit's set-up counts as
+constexpr int STEP_LEAST = 16;                 // places of a stretch, where a unit is that long
 constexpr int STEP_RING_BYTES = 96 * 1024;     // of a CTA's blocks on their way
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -349,11 +350,20 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// 4 bytes to shared memory, zero where there is nothing to copy.
+__device__ __forceinline__ void copy_4(void* to, const void* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
 // An 8 x 8 tile of 16-bit numbers turned over.
 __device__ __forceinline__ uint32_t turned_tile(uint32_t x) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
+}
+
+// a / b of numbers that are not negative (the 64-bit division costs some hundred clocks, and a row is hardly ever that long).
+__device__ __forceinline__ long divided(long a, long b) {
+    return ((a | b) >> 31) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 // All units in a row; every warp works out the same.
@@ -388,8 +398,7 @@ struct StepSchedule {
             most = max(most, __reduce_max_sync(0xffffffffu, n));
         }
         total *= units_of_entry;
-        // (no shorter than a block a warp, where units are longer than that)
-        stretch = max((total + gridDim.x - 1) / gridDim.x, (long)min(most, STEP_WARPS + STEP_SET_UP));
+        stretch = max(divided(total + gridDim.x - 1, gridDim.x), (long)min(most, STEP_LEAST));
         lo = blockIdx.x * stretch, hi = min(total, lo + stretch);
         begin = 0;
         if (lo >= hi) return;
@@ -406,7 +415,7 @@ struct StepSchedule {
                 const int at = __ffs(past) - 1;
                 begin += (long)__shfl_sync(0xffffffffu, upto - mine, at) * units_of_entry;
                 take(base + at);
-                unit = (int)((lo - begin) / length);
+                unit = (int)divided(lo - begin, length);
                 begin += (long)unit * length;
                 return;
             }
@@ -452,31 +461,31 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
         // places of the unit in this stretch: the set-up's, then a block each
         const int from = (int)(max(at.lo, at.begin) - at.begin), to = (int)(min(at.hi, at.begin + at.length) - at.begin);
         const int lo = at.first_block + max(0, from - STEP_SET_UP), hi = at.first_block + max(0, to - STEP_SET_UP);
-        const int first_cta = (int)(at.begin / at.stretch), n_parts = (int)((at.begin + at.length - 1) / at.stretch) - first_cta + 1;
+        const int first_cta = (int)divided(at.begin, at.stretch), n_parts = (int)divided(at.begin + at.length - 1, at.stretch) - first_cta + 1;
         const int part = (int)blockIdx.x - first_cta;
 
-        // Lane i looks up the warp's next 32 blocks, and the 32 after them ahead: where block i lies (in blocks), and its scales.
-        const int* table = p.block_table + (long)at.entry * p.max_blocks;
-        struct Places {
-            int place;
-            float k_scale, v_scale;
-        } here, ahead;
-        auto look_up = [&](int begins) {
-            Places x = {-1, 0.0f, 0.0f};
-            const int b = begins + lane * STEP_WARPS;
-            if (b < hi) {
-                const int index = b / per_page, id = table[index];
-                if (id >= 0 && id < p.n_pages) {
-                    x.place = (id * p.n_kv_heads + kv_head) * per_page + b - index * per_page;
-                    x.k_scale = p.k_scales[x.place];
-                    x.v_scale = p.v_scales[x.place];
-                }
+        // the queries of tile `warp` on their way: head g, in the order of the key's columns
+        uint4 q_row[KG][2];
+        if (warp < TILES) {
+#pragma unroll
+            for (int d = 0; d < KG; d++) {
+                const int col = 64 * d + 16 * c;
+                const bool there = g + 8 * warp < n_rows && col < dim;
+                const uint4* q = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + at.row * p.ld_q + (long)(head0 + (there ? g + 8 * warp : 0)) * dim + (there ? col : 0));
+                q_row[d][0] = there ? q[0] : make_uint4(0u, 0u, 0u, 0u);
+                q_row[d][1] = there ? q[1] : make_uint4(0u, 0u, 0u, 0u);
             }
-            return x;
+        }
+        // Lane i looks up the warp's next 32 blocks, and the 32 after them ahead: where block i lies (in blocks).
+        const int* table = p.block_table + (long)at.entry * p.max_blocks;
+        auto look_up = [&](int begins) -> int {
+            const int b = begins + lane * STEP_WARPS;
+            if (b >= hi) return -1;
+            const int index = b / per_page, id = table[index];
+            return id >= 0 && id < p.n_pages ? (id * p.n_kv_heads + kv_head) * per_page + b - index * per_page : -1;
         };
         const int mine = lo + warp < hi ? (hi - lo - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
-        here = look_up(lo + warp);
-        ahead = look_up(lo + warp + 32 * STEP_WARPS);
+        int here = look_up(lo + warp), ahead = look_up(lo + warp + 32 * STEP_WARPS);
         // A block on its way: 16-byte chunks, each row's in an order in which no two lanes below read the same banks.
         auto fetch = [&](int i) {                        // the warp's i-th block, into the ring's place i % stages
             if (i < mine) {
@@ -484,10 +493,9 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
                     here = ahead;
                     ahead = look_up(lo + warp + (i + 32) * STEP_WARPS);
                 }
-                const int place = __shfl_sync(0xffffffffu, here.place, i & 31);
-                const float k_scale = __shfl_sync(0xffffffffu, here.k_scale, i & 31), v_scale = __shfl_sync(0xffffffffu, here.v_scale, i & 31);
+                const int place = __shfl_sync(0xffffffffu, here, i & 31);
                 unsigned char* to = ring + (i % stages) * stage_bytes;
-                if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(k_scale, place >= 0 ? v_scale : 0.0f);     // (no scale: not there)
+                if (lane < 2) copy_4(to + 4 * lane, (lane == 0 ? p.k_scales : p.v_scales) + max(place, 0), place >= 0);     // (no scale: not there)
                 if (place >= 0) {
                     const uint8_t* k = k_pages + (long)place * E4M3_BLOCK * dim;
                     const uint8_t* v = v_pages + (long)place * E4M3_BLOCK * vdim;
@@ -515,24 +523,18 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
         };
         for (int i = 0; i < stages - 1; i++) fetch(i);
 
-        // the queries of tile `warp`: 16-bit floats of a power of two's size, head g, in the order of the key's columns
+        // the queries as 16-bit floats of a power of two's size
         if (warp < TILES) {
             const int r = g + 8 * warp;
             float x[KG][16], top = 0.0f;
 #pragma unroll
             for (int d = 0; d < KG; d++) {
-                const int col = 64 * d + 16 * c;
+                const uint32_t w[8] = {q_row[d][0].x, q_row[d][0].y, q_row[d][0].z, q_row[d][0].w, q_row[d][1].x, q_row[d][1].y, q_row[d][1].z, q_row[d][1].w};
 #pragma unroll
-                for (int i = 0; i < 16; i++) x[d][i] = 0.0f;
-                if (r < n_rows && col < dim) {
-                    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + at.row * p.ld_q + (long)(head0 + r) * dim + col);
-                    const uint4 u = q[0], v = q[1];
-                    const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[d][2 * i] = __uint_as_float(w[i] << 16), x[d][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                for (int i = 0; i < 8; i++) {
+                    x[d][2 * i] = __uint_as_float(w[i] << 16), x[d][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                    top = fmaxf(top, fmaxf(fabsf(x[d][2 * i]), fabsf(x[d][2 * i + 1])));
                 }
-#pragma unroll
-                for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(x[d][i]));
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -769,7 +771,11 @@ int launch_step(const E4m3Attention& p, int n_sms, cudaStream_t stream) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return launched(e, "e4m3_attention_step");
     }
-    return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(STEP_CTAS * n_sms), dim3(STEP_THREADS), bytes, stream, p, head_tiles, stages),
+    // as many CTAs as the SMs hold, or as the longest row that the tables allow has stretches
+    const long units = (long)p.n_items * p.n_kv_heads * head_tiles, most = (long)p.max_blocks * (p.page / E4M3_BLOCK) + STEP_SET_UP;
+    const long stretches = (units * most + STEP_LEAST - 1) / STEP_LEAST;
+    const int grid = (int)max(1L, min((long)STEP_CTAS * n_sms, stretches));
+    return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(grid), dim3(STEP_THREADS), bytes, stream, p, head_tiles, stages),
                     "e4m3_attention_step");
 }
 
