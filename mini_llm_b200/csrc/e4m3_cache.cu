@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attention_plain_kernel(const E4
 // the exponent, p = 2^(s + t - m + 7), and the sum of the weights gets p / 2^t: no multiplication more, and p keeps the 11 bits of a 16-bit
 // float however far apart the scales lie.  m moves only where a score passes it by 8, so that p stays below 2^15.
 constexpr int STEP_WARPS = 8, STEP_THREADS = STEP_WARPS * 32, STEP_CTAS = 2;
-constexpr int STEP_SET_UP = 8;                 // blocks that a unit's set-up counts as
+constexpr int STEP_SET_UP = 24;                // blocks that a unit's set-up counts as (some 6,500 clocks, at 150 to 250 a block)
 constexpr int STEP_LEAST = 16;                 // places of a stretch, where a unit is that long
 constexpr int STEP_RING_BYTES = 96 * 1024;     // of a CTA's blocks on their way
 
@@ -366,44 +366,66 @@ __device__ __forceinline__ long divided(long a, long b) {
     return ((a | b) >> 31) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-// All units in a row; every warp works out the same.
+// All units in a row; every warp works out the same, all its lanes together.
 struct StepSchedule {
     const E4m3Attention& p;
-    const int units_of_entry;
-    long total, stretch, lo, hi, begin;
-    int entry, unit, length, first_block, blocks, row, pos;
+    const int units_of_entry, lane;
+    long stretch, lo, hi, begin;                   // a CTA's share of the row, this CTA's, and where the unit that is next begins
+    int set_up;                                    // places that a unit's set-up takes
+    bool apart;                                    // every unit has CTAs of its own: it begins at a multiple of the stretch
+    int entry, unit, first_block, blocks, row, pos, length;
+    int base, count_of_lane, start_of_lane, row_of_lane;      // 32 entries, one a lane
 
+    __device__ void load(int from) {
+        base = from;
+        const int e = from + lane;
+        const bool there = e < p.n_items;
+        count_of_lane = there ? p.item_count[e] : 0, start_of_lane = there ? p.item_start[e] : 0, row_of_lane = there ? p.item_offset[e] : 0;
+    }
     __device__ void of_position(int position, int& lowest, int& count) const {
         const int first = p.window > 0 ? max(0, position - p.window + 1) : 0;
         lowest = first / E4M3_BLOCK;
-        count = position >= 0 ? min(position / E4M3_BLOCK + 1, p.max_blocks * (p.page / E4M3_BLOCK)) - lowest : 0;
-        count = max(count, 0);
+        count = position >= 0 ? max(0, min(position / E4M3_BLOCK + 1, p.max_blocks * (p.page / E4M3_BLOCK)) - lowest) : 0;
     }
-    __device__ int length_of(int e) const {        // of an entry's units; 0: it has none
-        if (e >= p.n_items || p.item_count[e] != 1) return 0;
+    __device__ int places(int of_blocks) const {
+        if (!apart) return of_blocks + set_up;
+        return (int)divided(max(of_blocks, 1) + stretch - 1, stretch) * (int)stretch;
+    }
+    __device__ int blocks_of_lane() const {        // -1: no unit
+        if (count_of_lane != 1) return -1;
         int lowest, count;
-        of_position(p.item_start[e], lowest, count);
-        return count + STEP_SET_UP;
+        of_position(start_of_lane, lowest, count);
+        return count;
     }
-    __device__ void take(int e) {                  // the next unit is this entry's first
-        entry = e, unit = 0, row = p.item_offset[e], pos = p.item_start[e];
+    __device__ void take(int at) {                 // the next unit is the first one of this lane's entry
+        entry = base + at, unit = 0;
+        row = __shfl_sync(0xffffffffu, row_of_lane, at), pos = __shfl_sync(0xffffffffu, start_of_lane, at);
         of_position(pos, first_block, blocks);
-        length = blocks + STEP_SET_UP;
+        length = places(blocks);
     }
-    __device__ StepSchedule(const E4m3Attention& params, int units, int lane) : p(params), units_of_entry(units), total(0) {
+    __device__ StepSchedule(const E4m3Attention& params, int units, int lane_) : p(params), units_of_entry(units), lane(lane_) {
+        long sum = 0, entries = 0;
         int most = 0;
-        for (int base = 0; base < p.n_items; base += 32) {
-            const int n = length_of(base + lane);
-            total += __reduce_add_sync(0xffffffffu, n);
+        for (int from = 0; from < p.n_items; from += 32) {
+            load(from);
+            const int n = blocks_of_lane();
+            sum += __reduce_add_sync(0xffffffffu, max(n, n == 0 ? 1 : 0));
+            entries += __popc(__ballot_sync(0xffffffffu, n >= 0));
             most = max(most, __reduce_max_sync(0xffffffffu, n));
         }
-        total *= units_of_entry;
-        stretch = max(divided(total + gridDim.x - 1, gridDim.x), (long)min(most, STEP_LEAST));
-        lo = blockIdx.x * stretch, hi = min(total, lo + stretch);
-        begin = 0;
-        if (lo >= hi) return;
-        for (int base = 0;; base += 32) {
-            const int mine = length_of(base + lane);
+        sum *= units_of_entry, entries *= units_of_entry;
+        // Equal stretches of the row of all units, or every unit cut by itself where that makes the longest stretch hardly longer (few units).
+        const long least = min(max(most, 1), STEP_LEAST), grid = gridDim.x;
+        const long together = max(divided(sum + entries * STEP_SET_UP + grid - 1, grid), least);
+        stretch = entries < grid ? max(divided(sum + grid - entries - 1, grid - entries), least) : 0;
+        apart = stretch > 0 && stretch <= together + STEP_SET_UP / 2;
+        set_up = apart ? 0 : STEP_SET_UP;
+        if (!apart) stretch = together;
+        lo = blockIdx.x * stretch, hi = lo + stretch, begin = 0;
+        // the unit in which the stretch begins
+        for (int from = 0; from < p.n_items; from += 32) {
+            if (base != from) load(from);
+            const int n = blocks_of_lane(), mine = n >= 0 ? places(n) : 0;
             int upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -414,22 +436,26 @@ struct StepSchedule {
             if (past != 0) {
                 const int at = __ffs(past) - 1;
                 begin += (long)__shfl_sync(0xffffffffu, upto - mine, at) * units_of_entry;
-                take(base + at);
+                take(at);
                 unit = (int)divided(lo - begin, length);
                 begin += (long)unit * length;
                 return;
             }
             begin += (long)__shfl_sync(0xffffffffu, upto, 31) * units_of_entry;
         }
+        hi = lo;                                   // the row ends before
     }
-    __device__ bool more() const { return lo < hi && begin < hi; }      // (CTAs behind the row's end have nothing)
+    __device__ bool more() const { return begin < hi && lo < hi; }
     __device__ void next() {
         begin += length;
-        if (++unit == units_of_entry && begin < hi) {
-            int e = entry + 1;
-            while (p.item_count[e] != 1) e++;      // (the row goes on, so there is one)
-            take(e);
+        if (++unit < units_of_entry || begin >= hi) return;
+        uint32_t left = __ballot_sync(0xffffffffu, count_of_lane == 1) & ~((2u << (entry - base)) - 1u);
+        while (left == 0 && base + 32 < p.n_items) {
+            load(base + 32);
+            left = __ballot_sync(0xffffffffu, count_of_lane == 1);
         }
+        if (left != 0) take(__ffs(left) - 1);
+        else hi = begin;                           // the row ends
     }
 };
 
@@ -454,46 +480,55 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
     wait_for_earlier_kernels();
     const uint8_t* k_pages = behind_the_wait(p.k_pages);
     const uint8_t* v_pages = behind_the_wait(p.v_pages);
-    for (StepSchedule at(p, p.n_kv_heads * head_tiles, lane); at.more(); at.next()) {
-        const int kv_head = at.unit / head_tiles, head_tile = at.unit - kv_head * head_tiles;
-        const int n_rows = min(ROWS, group - head_tile * ROWS), head0 = kv_head * group + head_tile * ROWS;
-        const int pos = at.pos, first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    StepSchedule at(p, p.n_kv_heads * head_tiles, lane);
+    // A unit, or what of it lies in this stretch, and what is on its way of it while the unit before is finished.
+    struct Piece {
+        int row, pos, first, kv_head, head0, n_rows, lo, hi, first_cta, part, n_parts, mine;
+        const int* table;
+        int here, ahead;                                 // lane i: where the warp's i-th block lies (in blocks), and its i + 32nd
+        uint4 q_row[KG][2];                              // the queries of tile `warp`: head g, in the order of the key's columns
+    };
+    // Lane i looks up 32 of the warp's blocks.
+    auto look_up = [&](const Piece& u, int begins) -> int {
+        const int b = begins + lane * STEP_WARPS;
+        if (b >= u.hi) return -1;
+        const int index = b / per_page, id = u.table[index];
+        return id >= 0 && id < p.n_pages ? (id * p.n_kv_heads + u.kv_head) * per_page + b - index * per_page : -1;
+    };
+    auto take = [&](Piece& u) {
+        u.kv_head = at.unit / head_tiles;
+        const int head_tile = at.unit - u.kv_head * head_tiles;
+        u.n_rows = min(ROWS, group - head_tile * ROWS), u.head0 = u.kv_head * group + head_tile * ROWS;
+        u.row = at.row, u.pos = at.pos, u.first = p.window > 0 ? max(0, at.pos - p.window + 1) : 0;
         // places of the unit in this stretch: the set-up's, then a block each
         const int from = (int)(max(at.lo, at.begin) - at.begin), to = (int)(min(at.hi, at.begin + at.length) - at.begin);
-        const int lo = at.first_block + max(0, from - STEP_SET_UP), hi = at.first_block + max(0, to - STEP_SET_UP);
-        const int first_cta = (int)divided(at.begin, at.stretch), n_parts = (int)divided(at.begin + at.length - 1, at.stretch) - first_cta + 1;
-        const int part = (int)blockIdx.x - first_cta;
-
-        // the queries of tile `warp` on their way: head g, in the order of the key's columns
-        uint4 q_row[KG][2];
+        u.lo = at.first_block + max(0, from - at.set_up), u.hi = at.first_block + min(at.blocks, max(0, to - at.set_up));
+        u.first_cta = (int)divided(at.begin, at.stretch), u.n_parts = (int)divided(at.begin + at.length - 1, at.stretch) - u.first_cta + 1;
+        u.part = (int)blockIdx.x - u.first_cta;
+        u.table = p.block_table + (long)at.entry * p.max_blocks;
+        u.mine = u.lo + warp < u.hi ? (u.hi - u.lo - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
+        u.here = look_up(u, u.lo + warp), u.ahead = look_up(u, u.lo + warp + 32 * STEP_WARPS);
         if (warp < TILES) {
 #pragma unroll
             for (int d = 0; d < KG; d++) {
                 const int col = 64 * d + 16 * c;
-                const bool there = g + 8 * warp < n_rows && col < dim;
-                const uint4* q = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + at.row * p.ld_q + (long)(head0 + (there ? g + 8 * warp : 0)) * dim + (there ? col : 0));
-                q_row[d][0] = there ? q[0] : make_uint4(0u, 0u, 0u, 0u);
-                q_row[d][1] = there ? q[1] : make_uint4(0u, 0u, 0u, 0u);
+                const bool there = g + 8 * warp < u.n_rows && col < dim;
+                const uint4* q = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + u.row * p.ld_q + (long)(u.head0 + (there ? g + 8 * warp : 0)) * dim + (there ? col : 0));
+                u.q_row[d][0] = there ? q[0] : make_uint4(0u, 0u, 0u, 0u);
+                u.q_row[d][1] = there ? q[1] : make_uint4(0u, 0u, 0u, 0u);
             }
         }
-        // Lane i looks up the warp's next 32 blocks, and the 32 after them ahead: where block i lies (in blocks).
-        const int* table = p.block_table + (long)at.entry * p.max_blocks;
-        auto look_up = [&](int begins) -> int {
-            const int b = begins + lane * STEP_WARPS;
-            if (b >= hi) return -1;
-            const int index = b / per_page, id = table[index];
-            return id >= 0 && id < p.n_pages ? (id * p.n_kv_heads + kv_head) * per_page + b - index * per_page : -1;
-        };
-        const int mine = lo + warp < hi ? (hi - lo - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
-        int here = look_up(lo + warp), ahead = look_up(lo + warp + 32 * STEP_WARPS);
+    };
+    if (!at.more()) return;
+    Piece u;
+    take(u);
+    for (;;) {
+        const int lo = u.lo, pos = u.pos, first = u.first, n_rows = u.n_rows, n_parts = u.n_parts;
         // A block on its way: 16-byte chunks, each row's in an order in which no two lanes below read the same banks.
         auto fetch = [&](int i) {                        // the warp's i-th block, into the ring's place i % stages
-            if (i < mine) {
-                if (i > 0 && (i & 31) == 0) {
-                    here = ahead;
-                    ahead = look_up(lo + warp + (i + 32) * STEP_WARPS);
-                }
-                const int place = __shfl_sync(0xffffffffu, here, i & 31);
+            if (i < u.mine) {
+                if (i > 0 && (i & 31) == 0) u.here = u.ahead, u.ahead = look_up(u, lo + warp + (i + 32) * STEP_WARPS);
+                const int place = __shfl_sync(0xffffffffu, u.here, i & 31);
                 unsigned char* to = ring + (i % stages) * stage_bytes;
                 if (lane < 2) copy_4(to + 4 * lane, (lane == 0 ? p.k_scales : p.v_scales) + max(place, 0), place >= 0);     // (no scale: not there)
                 if (place >= 0) {
@@ -529,7 +564,7 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
             float x[KG][16], top = 0.0f;
 #pragma unroll
             for (int d = 0; d < KG; d++) {
-                const uint32_t w[8] = {q_row[d][0].x, q_row[d][0].y, q_row[d][0].z, q_row[d][0].w, q_row[d][1].x, q_row[d][1].y, q_row[d][1].z, q_row[d][1].w};
+                const uint32_t w[8] = {u.q_row[d][0].x, u.q_row[d][0].y, u.q_row[d][0].z, u.q_row[d][0].w, u.q_row[d][1].x, u.q_row[d][1].y, u.q_row[d][1].z, u.q_row[d][1].w};
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     x[d][2 * i] = __uint_as_float(w[i] << 16), x[d][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
@@ -670,7 +705,7 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
                 }
             }
         };
-        for (int i = 0; i < mine; i++) {
+        for (int i = 0; i < u.mine; i++) {
             // block i has landed (as many groups behind it are on their way as the ring has places but two), and all lanes have left block i - 1
             if (stages == 4) copies_landed<2>();
             else if (stages == 3) copies_landed<1>();
@@ -704,7 +739,12 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
                 }
             }
         __syncthreads();
-        bf16* out = static_cast<bf16*>(p.out) + at.row * p.ld_out + (long)head0 * vdim;
+        // the next unit's pages and queries come while this one's results are put together
+        const int row = u.row, head0 = u.head0, first_cta = u.first_cta, part = u.part;
+        at.next();
+        const bool more = at.more();
+        if (more) take(u);
+        bf16* out = static_cast<bf16*>(p.out) + row * p.ld_out + (long)head0 * vdim;
         // A part that begins a unit is its CTA's last and has the second of the CTA's two places; any other is its first.
         constexpr int PART = ROWS * (WIDTH + 2);
         auto cell = [&](int q) { return p.partial + (long)(2 * (first_cta + q) + (q == 0 ? 1 : 0)) * PART; };
@@ -725,7 +765,7 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
             } else {
                 float* here = cell(part);
                 __stcg(here + i, sum);
-                if (col == 0) __stcg(here + ROWS * WIDTH + 2 * r, top), __stcg(here + ROWS * WIDTH + 2 * r + 1, weight_sum);
+                if (col == 0) __stcg(reinterpret_cast<float2*>(here + ROWS * WIDTH + 2 * r), make_float2(top, weight_sum));
             }
         }
         if (n_parts > 1) {
@@ -736,24 +776,41 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
             __syncthreads();
             if (ticket == n_parts - 1) {
                 __threadfence();
-                // the last to arrive adds the parts up, in their order
-                for (int i = threadIdx.x; i < n_rows * WIDTH; i += STEP_THREADS) {
+                // The last to arrive adds the parts up, in their order: two columns a thread, eight parts on their way at a time.
+                constexpr int AT_ONCE = 8;
+                for (int i = 2 * threadIdx.x; i < n_rows * WIDTH; i += 2 * STEP_THREADS) {
                     const int r = i / WIDTH, col = i - r * WIDTH;
-                    float top = -INFINITY, sum = 0.0f, weight_sum = 0.0f;
-                    for (int q = 0; q < n_parts; q++) top = fmaxf(top, __ldcg(cell(q) + ROWS * WIDTH + 2 * r));
-                    const float anchor = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-                    for (int q = 0; q < n_parts; q++) {
-                        const float* theirs = cell(q);
-                        const float weight = exp2_fast(__ldcg(theirs + ROWS * WIDTH + 2 * r) - anchor);
-                        sum += weight * __ldcg(theirs + i);
-                        weight_sum += weight * __ldcg(theirs + ROWS * WIDTH + 2 * r + 1);
+                    float top = -INFINITY, weight_sum = 0.0f;
+                    float2 sum = make_float2(0.0f, 0.0f);
+                    for (int q0 = 0; q0 < n_parts; q0 += AT_ONCE) {
+                        float2 of_part[AT_ONCE], state[AT_ONCE];
+#pragma unroll
+                        for (int n = 0; n < AT_ONCE; n++) {
+                            of_part[n] = make_float2(0.0f, 0.0f), state[n] = make_float2(-INFINITY, 0.0f);
+                            if (q0 + n < n_parts) {
+                                const float* theirs = cell(q0 + n);
+                                of_part[n] = __ldcg(reinterpret_cast<const float2*>(theirs + i));
+                                state[n] = __ldcg(reinterpret_cast<const float2*>(theirs + ROWS * WIDTH + 2 * r));
+                            }
+                        }
+                        float most = top;
+#pragma unroll
+                        for (int n = 0; n < AT_ONCE; n++) most = fmaxf(most, state[n].x);
+                        const float anchor = most == -INFINITY ? 0.0f : most, down = exp2_fast(top - anchor);
+                        sum.x *= down, sum.y *= down, weight_sum *= down, top = most;
+#pragma unroll
+                        for (int n = 0; n < AT_ONCE; n++) {
+                            const float weight = exp2_fast(state[n].x - anchor);
+                            sum.x += weight * of_part[n].x, sum.y += weight * of_part[n].y, weight_sum += weight * state[n].y;
+                        }
                     }
-                    if (col < vdim) out[r * vdim + col] = __float2bfloat16_rn(weight_sum == 0.0f ? 0.0f : sum / weight_sum);
+                    const float inverse = weight_sum == 0.0f ? 0.0f : 1.0f / weight_sum;
+                    if (col < vdim) *reinterpret_cast<__nv_bfloat162*>(out + r * vdim + col) = __floats2bfloat162_rn(sum.x * inverse, sum.y * inverse);
                 }
                 if (threadIdx.x == 0) *counter = 0;
             }
         }
+        if (!more) break;
         __syncthreads();                                 // (shared memory is the next unit's)
     }
 }
@@ -771,10 +828,9 @@ int launch_step(const E4m3Attention& p, int n_sms, cudaStream_t stream) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return launched(e, "e4m3_attention_step");
     }
-    // as many CTAs as the SMs hold, or as the longest row that the tables allow has stretches
-    const long units = (long)p.n_items * p.n_kv_heads * head_tiles, most = (long)p.max_blocks * (p.page / E4M3_BLOCK) + STEP_SET_UP;
-    const long stretches = (units * most + STEP_LEAST - 1) / STEP_LEAST;
-    const int grid = (int)max(1L, min((long)STEP_CTAS * n_sms, stretches));
+    // as many CTAs as the SMs hold, or as the longest row that the tables allow is cut into
+    const long units = (long)p.n_items * p.n_kv_heads * head_tiles, most = (long)p.max_blocks * (p.page / E4M3_BLOCK);
+    const int grid = (int)max(1L, min((long)STEP_CTAS * n_sms, units * ((most + STEP_LEAST - 1) / STEP_LEAST + 1)));
     return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(grid), dim3(STEP_THREADS), bytes, stream, p, head_tiles, stages),
                     "e4m3_attention_step");
 }
