@@ -1,7 +1,8 @@
 """Device memory of the caches, and the view of it each run entry gets.
 
 Per paged group: keys and values as ``[entries, n_pages, page_size, kv_heads,
-head_size]`` each (one page id covers every entry of the group, and every
+head_size]`` each (in 8 bits ``[entries, n_pages, kv_heads, page_size, head_size]``, with
+the scales of their blocks beside them) (one page id covers every entry of the group, and every
 entry's pages are one contiguous array), plus the device copy of the block
 tables of the step's items, ``[max_items, max_blocks]`` int32, refilled before
 each step.  Per fixed-state group: ``[entries, max_requests, *shape]``, zeroed
@@ -33,9 +34,10 @@ class LayerCache:
 class PagedLayerCache(LayerCache):
     kind = "paged"
 
-    def __init__(self, group, k_pages, v_pages, block_table, page_size, writes):
+    def __init__(self, group, k_pages, v_pages, block_table, page_size, writes, k_scales=None, v_scales=None):
         self.group = group
-        self.k_pages, self.v_pages = k_pages, v_pages      # [n_pages, page_size, kv_heads, head_size]
+        self.k_pages, self.v_pages = k_pages, v_pages      # [n_pages, page_size, kv_heads, head_size]; in 8 bits the heads come first
+        self.k_scales, self.v_scales = k_scales, v_scales  # in 8 bits: [n_pages, kv_heads, page_size / 16] fp32, else None
         self.block_table = block_table                     # [max_items, max_blocks] int32, rows = the step's items
         self.page_size = page_size
         self.writes = writes
@@ -70,11 +72,14 @@ class CompositeLayerCache(LayerCache):
 
 
 class CacheStorage:
-    def __init__(self, manager, order, dtype: torch.dtype, device, max_items: int, poison: float | None = None):
+    def __init__(self, manager, order, dtype: torch.dtype, device, max_items: int, poison: float | None = None, e4m3: bool = False):
         """``poison``: a debugging value.  Every page slot holds it until a token is stored
         there, and a page holds it again from the moment it is given back: a kernel that
         reads a slot past a request's length, or through a stale block-table row, then
-        reads ``poison`` instead of another request's plausible keys."""
+        reads ``poison`` instead of another request's plausible keys.  ``e4m3``: pages in 8 bits
+        (their poison is the code that is no number)."""
+        self.e4m3 = bool(e4m3)
+        self.key_scales, self.value_scales = {}, {}
         self.manager = manager
         self.device = device
         self.max_items = int(max_items)
@@ -87,6 +92,9 @@ class CacheStorage:
             if isinstance(group.need, PagedKV):
                 # one page beyond the pool's last: no request ever owns it; steps that are filled up
                 # to a round shape let their filler tokens store there
+                if self.e4m3:
+                    self._make_e4m3(group, n_entries, device)
+                    continue
                 shape = (n_entries, group.pool.n_pages + 1, manager.page_size, group.need.n_kv_heads,
                          group.need.head_size)
                 fill = 0.0 if poison is None else poison
@@ -105,7 +113,8 @@ class CacheStorage:
             g, position = manager.entry_group[key]
             if manager.groups[g].paged:
                 values = self.values[g][position] if g in self.values else None
-                return PagedLayerCache(g, self.keys[g][position], values, self.block_tables[g], manager.page_size, writes)
+                scales = (self.key_scales[g][position], self.value_scales[g][position]) if self.e4m3 else (None, None)
+                return PagedLayerCache(g, self.keys[g][position], values, self.block_tables[g], manager.page_size, writes, *scales)
             return StateLayerCache(g, self.states[g][position], writes)
 
         self.views = []
@@ -140,6 +149,19 @@ class CacheStorage:
         if poison is not None:
             manager.on_free = self.poison_pages
 
+    def _make_e4m3(self, group, n_entries: int, device) -> None:
+        need, page = group.need, self.manager.page_size
+        value_size = need.value_size or need.head_size
+        if not need.has_values or not ops.e4m3_sizes_take(need.head_size, value_size, page):
+            raise ValueError(f"a cache in 8 bits takes keys and values of 16 to 256 entries and pages, all multiples of 16, not heads of "
+                             f"{need.head_size} and {value_size if need.has_values else 'no'} entries in pages of {page}")
+        shape = (n_entries, group.pool.n_pages + 1, need.n_kv_heads, page)
+        code = 0 if self.poison is None else ops.E4M3_NONE
+        for pages, scales, size in ((self.keys, self.key_scales, need.head_size), (self.values, self.value_scales, value_size)):
+            pages[group.index] = torch.full((*shape, size), code, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+            scales[group.index] = torch.ones((*shape[:3], page // ops.E4M3_BLOCK), dtype=torch.float32, device=device)
+        self.block_tables[group.index] = torch.zeros((self.max_items, group.max_blocks), dtype=torch.int32, device=device)
+
     def paged_views(self):
         """Every paged view, also those inside the caches of entries with several."""
         for view in self.views:
@@ -151,7 +173,9 @@ class CacheStorage:
         """Overwrite pages that went back to their pool (debugging engines only)."""
         index = torch.tensor(list(pages), dtype=torch.int64, device=self.device)
         for store in (self.keys, self.values):
-            if group_index in store:
+            if group_index in store and self.e4m3:
+                store[group_index].view(torch.uint8).index_fill_(1, index, ops.E4M3_NONE)
+            elif group_index in store:
                 store[group_index].index_fill_(1, index, self.poison)
 
     def read_tokens(self, view_index: int, slot: int, first: int, count: int):
@@ -171,6 +195,10 @@ class CacheStorage:
         if count and int(pages.min()) < 0:
             raise ValueError(f"slot {slot} holds no page for some of tokens {first}..{first + count - 1}")
         pages, within = pages.to(self.device), (positions % page_size).to(self.device)
+        if self.e4m3:
+            # what the codes stand for, in 32-bit
+            return tuple(codes[pages, :, within].float() * scales[pages, :, within // ops.E4M3_BLOCK][..., None]
+                         for codes, scales in ((view.k_pages, view.k_scales), (view.v_pages, view.v_scales)))
         return (view.k_pages[pages, within].clone(),
                 view.v_pages[pages, within].clone() if view.v_pages is not None else None)
 
@@ -185,6 +213,6 @@ class CacheStorage:
 
     def bytes(self) -> int:
         total = 0
-        for store in (self.keys, self.values, self.states):
+        for store in (self.keys, self.values, self.key_scales, self.value_scales, self.states):
             total += sum(t.numel() * t.element_size() for t in store.values())
         return total

@@ -38,6 +38,7 @@ def parse_args(argv=None) -> argparse.Namespace:
                         help="a prompt as comma-separated token ids (may be given more than once)")
     parser.add_argument("--prompt", action="append", default=[], help="a prompt as text (needs a tokenizer.json)")
     parser.add_argument("--page-size", type=int, default=16)
+    parser.add_argument("--cache-dtype", default=None, choices=("e4m3",), help="hold keys and values in 8 bits (default: as --dtype)")
     parser.add_argument("--max-tokens-per-step", type=int, default=2048)
     parser.add_argument("--plain-kernels", action="store_true")
     parser.add_argument("--random", metavar="CONFIG.json",
@@ -109,7 +110,7 @@ def main(argv=None) -> int:
     from .generate import LLM
     if args.random:
         args.model = random_model_folder(args)
-    llm = LLM(args.model, dtype=args.dtype, device=device, page_size=args.page_size,
+    llm = LLM(args.model, dtype=args.dtype, device=device, page_size=args.page_size, cache_dtype=args.cache_dtype,
               max_tokens_per_step=args.max_tokens_per_step, plain_kernels=args.plain_kernels)
     tokenizer = load_tokenizer(args.model)
     prompts = [parse_ids(p) for p in args.prompt_ids]

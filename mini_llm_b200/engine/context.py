@@ -265,6 +265,7 @@ class StepContext:
         self.steps_apart = False      # no kernel of an earlier step still runs when this step's kernels start, but for its first one: what
                                       # earlier steps left (cached rows, states) may be read ahead of the wait for the kernels ahead
         self.decode_only = False      # every entry brings exactly one token
+        self.lone_tokens = False      # some entry of a step with prompt portions brings one token
         self.fused = False            # the step goes to the one-kernel decode step
         self.dump = None              # a list: the model appends the residual stream after every run entry
         self.att_tiles = None         # device work list (tiles of up to 128 tokens of one entry), or None

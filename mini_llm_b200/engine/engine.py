@@ -27,6 +27,7 @@ from ..config.registry import config_from_folder, describe_model
 from ..kernels import ops
 from ..kernels.lib import KernelError
 from ..kernels.dispatch import SPLIT_ATTENTION_MAX_ROWS, Kernels
+from ..parts.base import Mixer
 from ..sampling import SamplingParams
 from .context import ControlBlock, StepContext, Workspace
 from .fused_decode import FusedDecodePlan
@@ -59,23 +60,32 @@ class Engine:
     def __init__(self, model_dir: str, dtype: str = "bfloat16", device: str = "cuda:0", page_size: int = 64,
                  cache_tokens: int | None = None, n_pages: int | None = None, max_requests: int = 64,
                  max_tokens_per_step: int = 2048, plain_kernels: bool = False, cuda_graphs: bool = True,
-                 fused_decode: bool = True, debug_poison: bool = False):
+                 fused_decode: bool = True, debug_poison: bool = False, cache_dtype: str | None = None):
         """``debug_poison``: every cache slot that holds no live token holds a poison value
         (NaN on the 32-bit path; 1e30 on the bfloat16 path, whose tensor-core attention
         multiplies what lies in a masked slot by a weight of zero), so that a read past a
         request's length or through a stale block-table row ruins the logits instead of
-        passing for another request's keys."""
+        passing for another request's keys.
+
+        ``cache_dtype``: how the paged keys and values are held: None as ``dtype`` says, "e4m3" in 8
+        bits with a scale for each block of 16 tokens and head (a page is then half as many bytes as in
+        bfloat16; the model's attention must be of a kind that reads such pages, and ``page_size`` a
+        multiple of 16)."""
         if not torch.cuda.is_available():
             raise RuntimeError("mini_llm_b200 runs on a CUDA device (sm_100a) only; none is available "
                                "and there is no CPU path")
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {', '.join(sorted(DTYPES))}, got '{dtype}'")
-        self.dtype = DTYPES[dtype]
+        if cache_dtype not in (None, "e4m3"):
+            raise ValueError(f"cache_dtype must be None or 'e4m3', got {cache_dtype!r}")
+        self.dtype, self.cache_dtype = DTYPES[dtype], cache_dtype
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
         self.config = config_from_folder(model_dir)
         self.spec = describe_model(self.config)
         self.model = Model(self.spec)
+        if cache_dtype is not None:
+            self._check_e4m3()
         self.kernels = Kernels(self.dtype, plain_only=plain_kernels)
         self.model.load(model_dir, self.dtype, self.device, runtime=self)
         self.page_size = int(page_size)
@@ -97,7 +107,8 @@ class Engine:
         poison = None
         if debug_poison:
             poison = float("nan") if self.kernels.plain_only else 1e30
-        self.storage = CacheStorage(self.cache, self.spec.order, self.dtype, self.device, self.max_requests, poison)
+        self.storage = CacheStorage(self.cache, self.spec.order, self.dtype, self.device, self.max_requests, poison,
+                                    e4m3=cache_dtype is not None)
         self.workspace = Workspace(self.device, min_rows=min(self.max_tokens_per_step, 256))
         self.control = ControlBlock(self.device, self.cache.groups)
         self.ctx = StepContext(self.kernels, self.workspace, self.dtype, self.device)
@@ -117,8 +128,11 @@ class Engine:
         self._graph_stamp = None
         self.step_kinds = {"one_kernel": 0, "eager": 0, "captured": 0, "replayed": 0}      # how steps ran
         self._can_pad = self.storage.spare_page          # steps may be filled up to round shapes (see _step_reserved)
-        self.fused, self.fused_reason = (FusedDecodePlan.build(self) if fused_decode
-                                         else (None, "switched off by the caller"))
+        self.fused, self.fused_reason = None, "switched off by the caller"
+        if cache_dtype is not None:
+            self.fused_reason = "the cache is held in 8 bits"
+        elif fused_decode:
+            self.fused, self.fused_reason = FusedDecodePlan.build(self)
         if self.fused is None and fused_decode and self.dtype == torch.bfloat16 and not self.kernels.plain_only:
             # not an error, but a cliff in speed (a decode step is then some five launches a layer)
             print(f"[mini_llm_b200] decode steps run part by part, not as one kernel: {self.fused_reason}",
@@ -127,6 +141,14 @@ class Engine:
         self._status_address = ops.device_address(self._status_pinned)
         self._status_host = self._status_pinned.numpy()
         self.hidden_dump = None               # set by step(dump_hidden=True): the residual stream after every run entry
+
+    def _check_e4m3(self) -> None:
+        """Raises if some part of the model keeps pages that it cannot store and read in 8 bits, before anything is loaded."""
+        for part in self.model.parts():
+            if isinstance(part, Mixer) and not part.takes_e4m3_cache():
+                raise ValueError(f"{part.prefix}: {type(part).__name__} does not store and read a cache in 8 bits (cache_dtype='e4m3')")
+        # its attention makes out the prompt portions on the device: no work list is made for it
+        self.model.wants_attention_tiles = False
 
     def _make_ids_pinned(self, rows: int) -> None:
         """Room on the host for the draws of two steps of up to ``rows`` rows, which a step's last kernel writes."""
@@ -265,6 +287,7 @@ class Engine:
         ctx = self.ctx
         cache_length = self.cache.length
         decode_only = n_tokens == n_items
+        ctx.lone_tokens = not decode_only and any(len(e.tokens) == 1 for e in entries)
         slots = ctx.item_slots = [e.slot for e in entries]
         starts = ctx.item_starts = [cache_length(slot) for slot in slots]
         if decode_only:
@@ -507,6 +530,7 @@ class Engine:
             self._graph_stamp = stamp
         # (how many units come in parts is data; that some do decides whether the kernel gets scratch)
         key = (ctx.n_tokens, ctx.n_items, ctx.n_want, ctx.n_att_tiles, ctx.n_att_singles, ctx.att_parts > 1, ctx.att_units,
+               ctx.lone_tokens and self.cache_dtype is not None,
                sample_views is not None, self._any_nucleus, ctx.any_previous, self.control.parity, ctx.in_ring)
         held = self._graphs.get(key)
         # A shape runs eagerly the first time (every buffer it needs gets allocated) and is

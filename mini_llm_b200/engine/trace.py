@@ -33,6 +33,7 @@ def parse_args(argv=None):
     parser.add_argument("--max-tokens", type=int, required=True,
                         help="most tokens live requests hold at any time (each rounded up to a multiple of 64)")
     parser.add_argument("--page-size", type=int, default=16, help="tokens per cache page (a divisor of 64)")
+    parser.add_argument("--cache-dtype", default=None, choices=("e4m3",), help="hold keys and values in 8 bits (default: as --dtype)")
     parser.add_argument("--max-requests", type=int, default=4, help="most requests live at a time (state slots)")
     parser.add_argument("--plain-kernels", action="store_true", help="run the plain kernel of every operation")
     return parser.parse_args(argv)
@@ -46,7 +47,7 @@ def replay(args, lines, out=sys.stdout):
     os.makedirs(args.out, exist_ok=True)
     # a step of a trace may bring every token the cache holds at once
     engine = Engine(args.model, dtype=args.dtype, page_size=args.page_size, cache_tokens=args.max_tokens,
-                    max_requests=args.max_requests, plain_kernels=args.plain_kernels,
+                    cache_dtype=args.cache_dtype, max_requests=args.max_requests, plain_kernels=args.plain_kernels,
                     max_tokens_per_step=max(int(args.max_tokens), 1))
     slots = {}
     for line in lines:

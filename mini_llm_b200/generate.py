@@ -26,6 +26,7 @@ class EngineOptions:
     dtype: str = "bfloat16"               # "bfloat16" or "float32"
     device: str = "cuda:0"
     page_size: int = 64
+    cache_dtype: str | None = None        # how keys and values are held: None as ``dtype``, "e4m3" in 8 bits (pages of a multiple of 16)
     cache_tokens: int | None = None       # tokens the page pool holds; default: max_sessions full contexts
     max_sessions: int = 64                # most requests live at a time
     max_tokens_per_step: int = 2048       # token budget of one batch
@@ -46,7 +47,7 @@ class LLM:
         self.engine = Engine(model_dir, dtype=options.dtype, device=options.device, page_size=options.page_size,
                              cache_tokens=options.cache_tokens, max_requests=options.max_sessions,
                              max_tokens_per_step=options.max_tokens_per_step, plain_kernels=options.plain_kernels,
-                             cuda_graphs=options.cuda_graphs)
+                             cuda_graphs=options.cuda_graphs, cache_dtype=options.cache_dtype)
         self.scheduler = Scheduler(self.engine, options.max_tokens_per_step, options.max_prefill_chunk,
                                    options.max_sessions, run_ahead=options.run_ahead)
 

@@ -81,6 +81,7 @@ class Kernels:
         self._att_scratch = None
         self._att_work = None
         self._memory_readers = None
+        self._e4m3_workspace = None
 
     # ---- operations without a fast variant --------------------------------------------------
     def keep_tokens(self, kept, slots, tokens, to_host=None):
@@ -169,6 +170,32 @@ class Kernels:
         return ops.capped_attention(out, q, cache.k_pages, cache.v_pages, cache.block_table, ctx.positions, ctx.token_item,
                                     n_heads, n_kv_heads, dim, vdim, cache.page_size, scale, cap, window, tiled, chunk, gate, sink, keep,
                                     slopes, gate_wide)
+
+    # ---- a cache in 8 bits ------------------------------------------------------------------------
+    def e4m3_store(self, ctx, cache, q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims=0, inv_freq=None, amplitude=1.0):
+        self.launches += 1
+        return ops.e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, ctx.positions,
+                              ctx.token_item, cache.block_table, cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, cache.writes)
+
+    def e4m3_attention(self, ctx, out, q, cache, n_heads, n_kv_heads, scale, cap=0.0, window=0):
+        """Attention over pages in 8 bits: entries of single tokens go to one kernel, prompt portions to another (``ops.e4m3_attention``)."""
+        dim, vdim = cache.k_pages.shape[3], cache.v_pages.shape[3]
+        plain = self.plain_only or not ops.e4m3_fast_takes(q.dtype, dim, vdim)
+        singles, portions = bool(ctx.decode_only or ctx.lone_tokens), not ctx.decode_only
+        self.launches += 1 if plain else int(singles) + int(portions)
+        self.chose("e4m3_attention", "e4m3_attention_plain" if plain else "+".join(
+            (["e4m3_attention_tiles"] if portions else []) + (["e4m3_attention_step"] if singles else [])), q.shape[0], n_heads, dim, vdim)
+        workspace = None if plain else self._e4m3_space(ctx.device, vdim)
+        return ops.e4m3_attention(out, q, cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales, cache.block_table, ctx.item_offset,
+                                  ctx.item_count, ctx.item_start, n_heads, n_kv_heads, scale, cap, window, longest=None if portions else 1,
+                                  singles=singles, workspace=workspace, plain=plain)
+
+    def _e4m3_space(self, device, vdim):
+        held = self._e4m3_workspace
+        if held is None or held.vdim < vdim:
+            self._e4m3_workspace = held = ops.e4m3_workspace(device, vdim, self.status(device))
+            self.scratch_generation += 1
+        return held
 
     def linear_recurrence(self, ctx, out, q, k, v, gate_a, gate_b, log_rate, step_bias, state, heads, qk_heads, dim, vdim,
                           delta, unit_norm=False, q_scale=1.0, skip=None, writes=True, channel_decay=False):
@@ -489,6 +516,8 @@ class Kernels:
             self._split_scratch[2].zero_()
         if self._memory_readers is not None:
             self._memory_readers.zero_()
+        if self._e4m3_workspace is not None:
+            self._e4m3_workspace.reset()
         if self._sample_scratch is not None:
             self._sample_scratch[2].zero_()
 

@@ -1895,7 +1895,8 @@ def add_normed_norm(hidden, y, gain, eps, normed, next_gain, next_eps):
 # two, for each block of 16 positions and key/value head in scales [pages, kv_heads, page / 16]: an entry is code * scale.
 
 E4M3_BLOCK = 16
-E4M3_STEP_SIZES = 128          # entries of a key or value up to which the kernel for single tokens takes them
+E4M3_NONE = 0x7f               # the code that is no number
+E4M3_FAST_SIZES = 128          # entries of a key or value up to which the kernels on tensor cores take them
 
 
 class _E4m3Attention(ctypes.Structure):
@@ -1924,6 +1925,11 @@ def _sm_count(device) -> int:
 def e4m3_sizes_take(dim, vdim, page_size) -> bool:
     """Whether a cache in 8 bits takes the sizes: keys and values of 16 to 256 entries and pages of positions, all multiples of 16."""
     return all(n % 16 == 0 and n > 0 for n in (dim, vdim, page_size)) and dim <= 256 and vdim <= 256
+
+
+def e4m3_fast_takes(dtype, dim, vdim) -> bool:
+    """Whether the kernels on tensor cores take queries of this type and heads of these sizes (else the plain one does)."""
+    return dtype == torch.bfloat16 and max(dim, vdim) <= E4M3_FAST_SIZES
 
 
 def _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table):
@@ -2025,12 +2031,12 @@ class E4m3Workspace:
     parts (zero between launches) and a status word (0; a kernel that gives up a bounded wait leaves a code there, and its
     result is invalid).  Calls that may run at the same time need one each."""
 
-    def __init__(self, device, vdim: int):
+    def __init__(self, device, vdim: int, status=None):
         self.vdim = int(vdim)
         n_sms = _sm_count(torch.device(device))
         self.partial = torch.empty(2 * n_sms * 256 * (_padded_64(self.vdim) + 2), dtype=torch.float32, device=device)
         self.counters = torch.zeros(2 * n_sms, dtype=torch.int32, device=device)
-        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device) if status is None else status
 
     def reset(self) -> None:
         """After a kernel gave up: counters and status start over."""
@@ -2038,8 +2044,9 @@ class E4m3Workspace:
         self.status.zero_()
 
 
-def e4m3_workspace(device, vdim: int) -> E4m3Workspace:
-    return E4m3Workspace(device, vdim)
+def e4m3_workspace(device, vdim: int, status=None) -> E4m3Workspace:
+    """``status``: a zeroed int32 device word that other kernels report in too (its own, if none is given)."""
+    return E4m3Workspace(device, vdim, status)
 
 
 def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start, heads, kv_heads, scale,
@@ -2074,7 +2081,7 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
     if not (window >= 0 and cap >= 0 and scale >= 0):
         raise KernelError(f"{who}: a window and a cap are positive, or 0 for none, and no scale is negative")
     _check_same_device(who, q, out, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start)
-    fast = not plain and q.dtype == torch.bfloat16 and max(dim, vdim) <= E4M3_STEP_SIZES
+    fast = not plain and e4m3_fast_takes(q.dtype, dim, vdim)
     if fast and workspace is None:
         raise KernelError(f"{who}: a workspace is needed (e4m3_workspace)")
     if fast:

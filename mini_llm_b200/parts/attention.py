@@ -21,6 +21,9 @@ keys [T, kv_heads * head_size] in place, each row by its ``ctx.positions``.
 The projection then writes q, k and v side by side, the encoding rotates, and
 the keys and values are stored into the pages by a pass of their own (the
 fused projection, which scatters straight into the pages, knows no rotation).
+
+Where the engine holds its pages in 8 bits (``cache.k_scales`` is there) the same
+parts store with ``e4m3_store`` and read with ``e4m3_attention``.
 """
 
 from __future__ import annotations
@@ -81,6 +84,9 @@ class CausalSelfAttention(Mixer):
 
     accepts_deferred_norm = True
 
+    def takes_e4m3_cache(self) -> bool:
+        return True
+
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         if self.position is not None:
@@ -89,6 +95,10 @@ class CausalSelfAttention(Mixer):
 
     def forward(self, ctx, x, hidden, cache):
         k = ctx.kernels
+        if cache.k_scales is not None:
+            mixed = self._mixed_in_8_bits(ctx, x, cache)
+            k.linear(ctx, hidden, mixed, self.w(f"{self.out_name}.weight"), self.w(f"{self.out_name}.bias"), epilogue="add")
+            return
         if self.position is None:
             q = k.qkv_projection(ctx, x, self.w(f"{self.qkv_name}.weight"), self.w(f"{self.qkv_name}.bias"), cache,
                                  self.q_width, self.kv_width)
@@ -105,6 +115,20 @@ class CausalSelfAttention(Mixer):
                     self.window or 0)
         k.linear(ctx, hidden, mixed, self.w(f"{self.out_name}.weight"), self.w(f"{self.out_name}.bias"),
                  epilogue="add")
+
+    def _mixed_in_8_bits(self, ctx, x, cache):
+        """The concatenated heads over pages in 8 bits, ahead of the output projection."""
+        k = ctx.kernels
+        qkv = ctx.buffer("qkv", (x.shape[0], self.qkv_width), ctx.act_dtype)
+        k.linear(ctx, qkv, x, self.w(f"{self.qkv_name}.weight"), self.w(f"{self.qkv_name}.bias"))
+        q = qkv[:, :self.q_width]
+        if self.position is not None:
+            self.position.rotate(ctx, q, qkv[:, self.q_width:self.q_width + self.kv_width], self.n_heads, self.n_kv_heads, self.head_size)
+        if cache.writes:
+            k.e4m3_store(ctx, cache, None, qkv, self.q_width, self.q_width + self.kv_width, self.n_heads, self.n_kv_heads,
+                         self.head_size, self.head_size)
+        mixed = ctx.buffer("attn_out", (x.shape[0], self.q_width), ctx.act_dtype)
+        return k.e4m3_attention(ctx, mixed, q, cache, self.n_heads, self.n_kv_heads, self.score_scale, window=self.window or 0)
 
 
 class FilteredAttention(Mixer):
@@ -160,6 +184,9 @@ class FilteredAttention(Mixer):
             need["taps"] = FixedState((self.taps - 1, self.qkv_width), "float32")
         return need
 
+    def takes_e4m3_cache(self) -> bool:
+        return bool(getattr(self.position, "stores_e4m3", False))
+
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         n = self.names
@@ -185,8 +212,12 @@ class FilteredAttention(Mixer):
         self.position.rotate_store(ctx, pages, qkv, self.q_width, self.q_width + self.k_width, self.n_heads, self.n_kv_heads,
                                    self.dim, self.vdim)
         mixed = ctx.buffer("attn_out", (n, self.n_heads * self.vdim), ctx.act_dtype)
-        k.capped_attention(ctx, mixed, qkv[:, :self.q_width], pages, self.n_heads, self.n_kv_heads, self.dim, self.vdim,
-                           self.score_scale, self.softcap, self.window or 0)
+        if pages.k_scales is not None:
+            k.e4m3_attention(ctx, mixed, qkv[:, :self.q_width], pages, self.n_heads, self.n_kv_heads, self.score_scale, self.softcap,
+                             self.window or 0)
+        else:
+            k.capped_attention(ctx, mixed, qkv[:, :self.q_width], pages, self.n_heads, self.n_kv_heads, self.dim, self.vdim,
+                               self.score_scale, self.softcap, self.window or 0)
         out = ctx.buffer("mixer_out", (n, self.width), torch.float32)
         k.linear(ctx, out, mixed, self.w(self.names["o"]), self.w(self.names["o"] + self.names["bias"]))
         return out

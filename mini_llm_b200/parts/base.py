@@ -37,7 +37,7 @@ residual stream [T, width]; "act" tensors have the engine's element type):
 
 from __future__ import annotations
 
-from .spec import NoCache, PartSpec, WeightSpec
+from .spec import NoCache, PagedKV, PartSpec, WeightSpec
 
 
 class Part:
@@ -77,6 +77,11 @@ class Norm(Part):
 class Mixer(Part):
     def cache_need(self):
         return NoCache()
+
+    def takes_e4m3_cache(self) -> bool:
+        """Whether the part stores and reads pages in 8 bits, should the engine hold them so; one that keeps no pages does not mind."""
+        need = self.cache_need()
+        return not any(isinstance(one, PagedKV) for one in (need.values() if isinstance(need, dict) else (need,)))
 
     def forward(self, ctx, x, hidden, cache):
         raise NotImplementedError

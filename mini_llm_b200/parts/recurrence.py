@@ -383,6 +383,9 @@ class ParallelMixers(Mixer):
                 need[name] = mine
         return need
 
+    def takes_e4m3_cache(self) -> bool:
+        return all(part.takes_e4m3_cache() for _, part, _ in self.branches)
+
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         for _, part, _ in self.branches:

@@ -45,6 +45,7 @@ def rotary_frequencies(base: float, dims: int, scaling: dict | None = None):
 
 class InterleavedRotary(PositionEncoding):
     graph_safe = True
+    stores_e4m3 = True        # ``rotate_store`` also stores into pages in 8 bits
 
     def __init__(self, prefix, base: float, dims: int, scaling: dict | None = None):
         super().__init__(prefix)
@@ -69,6 +70,11 @@ class InterleavedRotary(PositionEncoding):
     def rotate_store(self, ctx, cache, qkv, k_off, v_off, n_heads, n_kv_heads, key_size, value_size):
         if self.dims > key_size:
             raise ValueError(f"{self.prefix}: {self.dims} rotated entries do not fit a head of {key_size}")
+        if cache.k_scales is not None:
+            # (in place, as below: each head's rows are read before they are written)
+            ctx.kernels.e4m3_store(ctx, cache, qkv[:, :n_heads * key_size], qkv, k_off, v_off, n_heads, n_kv_heads, key_size, value_size,
+                                   self.dims, self.inv_freq, self.amplitude)
+            return
         ctx.kernels.rotary_store(ctx, cache, qkv, k_off, v_off, n_heads, n_kv_heads, key_size, value_size, self.dims,
                                  self.inv_freq, self.amplitude)
 

@@ -35,3 +35,22 @@ def test_there_is_no_path_on_the_host():
         ops.e4m3_attention(q, q, pages, pages, scales, scales, ints[None], ints, ints, ints, 1, 1, 1.0, plain=True)
     with pytest.raises(KernelError, match="CUDA tensor"):
         ops.e4m3_store(None, torch.zeros((1, 192)), 64, 128, 1, 1, 64, 64, 0, None, 1.0, ints, ints, ints[None], pages, pages, scales, scales)
+
+
+def test_which_mixers_take_a_cache_in_8_bits():
+    import deluvik_helpers
+    import fuvolix_helpers
+    import lipulorn_helpers
+    import sumozen_helpers
+    from mini_llm_b200.config import config_from_dict, describe_model
+    from mini_llm_b200.engine.model import Model
+    from mini_llm_b200.parts.base import Mixer
+    from tiny_configs import TINY_A
+
+    def refused(raw):
+        return {type(p).__name__ for p in Model(describe_model(config_from_dict(raw))).parts() if isinstance(p, Mixer) and not p.takes_e4m3_cache()}
+
+    assert refused(TINY_A) == set() and refused(sumozen_helpers.full_stack()) == set()
+    assert refused(fuvolix_helpers.config([fuvolix_helpers.mlstm()])) == set()              # (keeps no pages)
+    assert refused(fuvolix_helpers.full_stack()) == {"LatentAttention"}
+    assert "GatedAttention" in refused(lipulorn_helpers.full_stack()) and "NormedAttention" in refused(deluvik_helpers.full_stack())
