@@ -61,6 +61,17 @@ __device__ __forceinline__ float capped(float x, float cap, float two_log2e_over
     return cap - 2.0f * cap * r;
 }
 
+// Raises a kernel's limit of dynamic shared memory to `bytes`, once on each device (`raised`: of this kernel, what each device's limit is).
+template <typename Kernel>
+static cudaError_t raise_shared_limit(Kernel kernel, size_t bytes, size_t (&raised)[64]) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && raised[device] >= bytes)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < 64) raised[device] = bytes;
+    return e;
+}
+
 // What attention over the cache gets.  An entry is a request's tokens of this step: rows item_offset .. + item_count of q, at
 // positions item_start, item_start + 1, ...; entries without tokens are allowed.
 struct E4m3Attention {

@@ -809,9 +809,11 @@ extern "C" int mllm_e4m3_tiles_attention(const E4m3Attention* p, int n_rows, int
     if (p->dim > 128 || p->vdim > 128) return fail("e4m3_attention_tiles: heads of more than 128 entries");
     const int groups = p->dim <= 64 && p->vdim <= 64 ? 1 : 2, stages = groups == 1 ? 4 : 2;
     const size_t bytes = 1024 + (size_t)((groups == 1 ? 4 : 2) + 2 * stages) * groups * GROUP_BYTES;
-    auto kernel = p->cap > 0.0f ? (groups == 1 ? attention_tiles_kernel<true, 1> : attention_tiles_kernel<true, 2>)
-                                : (groups == 1 ? attention_tiles_kernel<false, 1> : attention_tiles_kernel<false, 2>);
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    const int which = (p->cap > 0.0f ? 2 : 0) + groups - 1;
+    static size_t raised[4][64];
+    auto kernel = which == 0 ? attention_tiles_kernel<false, 1> : which == 1 ? attention_tiles_kernel<false, 2>
+                : which == 2 ? attention_tiles_kernel<true, 1> : attention_tiles_kernel<true, 2>;
+    const cudaError_t e = raise_shared_limit(kernel, bytes, raised[which]);
     if (e != cudaSuccess) return launched(e, "e4m3_attention_tiles");
     return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(n_sms), dim3(THREADS), bytes, (cudaStream_t)stream, *p, stages),
                     "e4m3_attention_tiles");

@@ -858,10 +858,9 @@ int launch_step(const E4m3Attention& p, int n_sms, cudaStream_t stream) {
     const size_t bytes = max((size_t)stages * of_all, STEP_WARPS * rows * (64 * VG + 2) * sizeof(float));
     static_assert(STEP_WARPS * 16 * (128 + 2) * 4 <= 100 * 1024 && 3 * STEP_WARPS * (128 + 16 * 256) <= 104 * 1024, "two CTAs of the largest size share an SM");
     auto kernel = attention_step_kernel<KG, VG, TILES, EXACT>;
-    if (bytes > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e != cudaSuccess) return launched(e, "e4m3_attention_step");
-    }
+    static size_t raised[64];
+    const cudaError_t e = raise_shared_limit(kernel, bytes, raised);
+    if (e != cudaSuccess) return launched(e, "e4m3_attention_step");
     // as many CTAs as the SMs hold, or as the longest row that the tables allow is cut into
     const long units = (long)p.n_items * p.n_kv_heads * head_tiles, most = (long)p.max_blocks * (p.page / E4M3_BLOCK);
     const int grid = (int)max(1L, min((long)STEP_CTAS * n_sms, units * ((most + STEP_LEAST - 1) / STEP_LEAST + 1)));

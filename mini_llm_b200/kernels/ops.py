@@ -1915,8 +1915,7 @@ _e4m3_tiles = Function("e4m3_tiles", "mllm_e4m3_tiles_attention", [ctypes.POINTE
 _sm_counts = {}
 
 
-def _sm_count(device) -> int:
-    index = device.index if device.index is not None else torch.cuda.current_device()
+def _sm_count(index: int) -> int:
     if index not in _sm_counts:
         _sm_counts[index] = torch.cuda.get_device_properties(index).multi_processor_count
     return _sm_counts[index]
@@ -1932,37 +1931,61 @@ def e4m3_fast_takes(dtype, dim, vdim) -> bool:
     return dtype == torch.bfloat16 and max(dim, vdim) <= E4M3_FAST_SIZES
 
 
-def _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table):
+# (These calls may be all that stands between two short kernels: a tensor is looked at once, in few words, and only a wrong one again, for the
+# error's text.)
+
+def _is(t, dtype, dims, index) -> bool:
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == dims
+
+
+def _refuse(t, name, dtype, dims, index):
+    """Raises what is wrong with a tensor that should be of this type on CUDA device ``index``."""
+    _check(t, name)
+    if t.dtype is not dtype or t.dim() != dims:
+        raise KernelError(f"{name}: expected {dtype} with {dims} dimensions, got {t.dtype} of shape {tuple(t.shape)}")
+    raise KernelError(f"{name}: on device {t.get_device()}, not with the others on {index}")
+
+
+def _rows_fit(t) -> bool:
+    """Rows of contiguous entries that begin on 16-byte boundaries."""
+    return t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0)
+
+
+def _on_device(index):
+    """The stream that a launch on CUDA device ``index`` goes to."""
+    return _pinned_stream if _pinned_stream is not None else torch._C._cuda_getCurrentRawStream(index)
+
+
+def _launch_on(index, launch, *args):
+    if torch._C._cuda_getDevice() == index:
+        launch(*args)
+    else:
+        with torch.cuda.device(index):
+            launch(*args)
+
+
+def _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, index):
     """The pages' sizes: (pages, kv_heads, page, dim, vdim)."""
-    for name, pages, scales in (("k", k_pages, k_scales), ("v", v_pages, v_scales)):
-        _check(pages, f"{who}.{name}_pages", torch.float8_e4m3fn, 4)
-        _check(scales, f"{who}.{name}_scales", torch.float32, 3)
-        if not pages.is_contiguous() or not scales.is_contiguous() or pages.data_ptr() % 16 != 0:
-            raise KernelError(f"{who}: pages and scales must be contiguous, pages on a 16-byte boundary")
+    code = torch.float8_e4m3fn
+    if not (_is(k_pages, code, 4, index) and _is(v_pages, code, 4, index) and _is(k_scales, torch.float32, 3, index)
+            and _is(v_scales, torch.float32, 3, index) and _is(block_table, torch.int32, 2, index)):
+        for name, t, dtype, dims in (("k_pages", k_pages, code, 4), ("v_pages", v_pages, code, 4), ("k_scales", k_scales, torch.float32, 3),
+                                     ("v_scales", v_scales, torch.float32, 3), ("block_table", block_table, torch.int32, 2)):
+            if not _is(t, dtype, dims, index):
+                _refuse(t, f"{who}.{name}", dtype, dims, index)
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()
+            and block_table.is_contiguous() and k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0):
+        raise KernelError(f"{who}: pages, scales and block table must be contiguous, pages on a 16-byte boundary")
     n_pages, kv_heads, page, dim = k_pages.shape
-    vdim = v_pages.shape[3]
-    if tuple(v_pages.shape[:3]) != (n_pages, kv_heads, page):
-        raise KernelError(f"{who}: keys {tuple(k_pages.shape)} and values {tuple(v_pages.shape)} are not of the same pages")
+    v_shape = v_pages.shape
+    vdim = v_shape[3]
+    if v_shape[:3] != (n_pages, kv_heads, page):
+        raise KernelError(f"{who}: keys {tuple(k_pages.shape)} and values {tuple(v_shape)} are not of the same pages")
     if not e4m3_sizes_take(dim, vdim, page):
         raise KernelError(f"{who} does not take heads of {dim} and {vdim} entries in pages of {page} (multiples of 16, heads up to 256)")
-    if tuple(k_scales.shape) != (n_pages, kv_heads, page // E4M3_BLOCK) or k_scales.shape != v_scales.shape:
+    if k_scales.shape != (n_pages, kv_heads, page // E4M3_BLOCK) or v_scales.shape != k_scales.shape:
         raise KernelError(f"{who}: scales must be [pages, kv_heads, page / {E4M3_BLOCK}]")
-    _check(block_table, f"{who}.block_table", torch.int32, 2)
-    if not block_table.is_contiguous():
-        raise KernelError(f"{who}: the block table must be contiguous")
     return n_pages, kv_heads, page, dim, vdim
-
-
-def _check_same_device(who, first, *others):
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise KernelError(f"{who}: tensors lie on {first.device} and {t.device}")
-
-
-def _rows_of_sixteen_bytes(t, who):
-    size = t.element_size()
-    if t.data_ptr() % 16 != 0 or (t.shape[0] > 1 and t.stride(0) * size % 16 != 0):
-        raise KernelError(f"{who}: rows must begin on 16-byte boundaries")
 
 
 def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, positions, token_item,
@@ -1981,44 +2004,41 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
     keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
     row that begins a block begins it anew, whatever was there.  A key or value head with an n that is not finite is stored as
     NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes."""
-    _check(qkv, "e4m3_store.qkv", None, 2)
-    n = qkv.shape[0]
-    if min(heads, kv_heads) <= 0 or dim % 16 != 0 or vdim % 16 != 0 or not 0 < dim <= 256 or not 0 < vdim <= 256:
-        raise KernelError(f"e4m3_store does not take heads of {dim} and {vdim} entries (multiples of 16 up to 256)")
-    if rot_dims < 0 or rot_dims % 2 != 0 or rot_dims > dim:
-        raise KernelError(f"e4m3_store: {rot_dims} turned entries do not fit a head of {dim}")
-    if min(k_off, v_off) < 0 or max(heads * dim, k_off + kv_heads * dim, v_off + kv_heads * vdim) > qkv.shape[1] or k_off % 8 or v_off % 8:
-        raise KernelError("e4m3_store: the columns do not hold queries, keys and values, or are not multiples of 8")
-    dtype = dtype_code(qkv.dtype)
-    _rows_of_sixteen_bytes(qkv, "e4m3_store.qkv")
-    if rot_dims:
-        _check(inv_freq, "e4m3_store.inv_freq", torch.float64, 1)
-        if inv_freq.shape[0] < rot_dims // 2:
-            raise KernelError("e4m3_store: fewer frequencies than turned pairs")
-    _check(positions, "e4m3_store.positions", torch.int32, 1)
-    _check(token_item, "e4m3_store.token_item", torch.int32, 1)
-    if positions.shape[0] < n or token_item.shape[0] < n:
-        raise KernelError("e4m3_store: fewer positions or entries than rows")
-    _check_same_device("e4m3_store", qkv, q_out, inv_freq if rot_dims else None, positions, token_item)
+    who = "e4m3_store"
+    _check(qkv, f"{who}.qkv", None, 2)
+    index, (n, columns), dtype = qkv.get_device(), qkv.shape, dtype_code(qkv.dtype)
+    if min(heads, kv_heads) <= 0 or dim % 16 or vdim % 16 or not 0 < dim <= 256 or not 0 < vdim <= 256:
+        raise KernelError(f"{who} does not take heads of {dim} and {vdim} entries (multiples of 16 up to 256)")
+    if rot_dims < 0 or rot_dims % 2 or rot_dims > dim:
+        raise KernelError(f"{who}: {rot_dims} turned entries do not fit a head of {dim}")
+    if min(k_off, v_off) < 0 or max(heads * dim, k_off + kv_heads * dim, v_off + kv_heads * vdim) > columns or k_off % 8 or v_off % 8:
+        raise KernelError(f"{who}: the columns do not hold queries, keys and values, or are not multiples of 8")
+    for name, t, kind in (("inv_freq", inv_freq, torch.float64), ("positions", positions, torch.int32), ("token_item", token_item, torch.int32)):
+        if not _is(t, kind, 1, index) and (rot_dims or kind is not torch.float64):
+            _refuse(t, f"{who}.{name}", kind, 1, index)
+    if rot_dims and (inv_freq.shape[0] < rot_dims // 2 or inv_freq.stride(0) != 1):
+        raise KernelError(f"{who}: fewer frequencies than turned pairs, or not side by side")
+    if positions.shape[0] < n or token_item.shape[0] < n or (n > 1 and (positions.stride(0) != 1 or token_item.stride(0) != 1)):
+        raise KernelError(f"{who}: fewer positions or entries than rows, or not side by side")
     if q_out is not None:
-        _check(q_out, "e4m3_store.q_out", qkv.dtype, 2)
-        if q_out.shape[0] != n or q_out.shape[1] != heads * dim:
-            raise KernelError("e4m3_store: q_out does not have heads * dim columns")
-        _rows_of_sixteen_bytes(q_out, "e4m3_store.q_out")
+        if not _is(q_out, qkv.dtype, 2, index):
+            _refuse(q_out, f"{who}.q_out", qkv.dtype, 2, index)
+        if q_out.shape != (n, heads * dim):
+            raise KernelError(f"{who}: q_out does not have heads * dim columns")
+    if n and not (_rows_fit(qkv) and (q_out is None or _rows_fit(q_out))):
+        raise KernelError(f"{who}: rows of qkv and q_out must begin on 16-byte boundaries, their entries side by side")
     n_pages = page = max_blocks = 0
+    pages = (None, None, None, None)
     if writes:
-        n_pages, held_heads, page, held_dim, held_vdim = _check_e4m3_pages("e4m3_store", k_pages, v_pages, k_scales, v_scales, block_table)
+        n_pages, held_heads, page, held_dim, held_vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, index)
         if (held_heads, held_dim, held_vdim) != (kv_heads, dim, vdim):
-            raise KernelError("e4m3_store: the pages hold heads of another number or size")
+            raise KernelError(f"{who}: the pages hold heads of another number or size")
         max_blocks = block_table.shape[1]
-        _check_same_device("e4m3_store", qkv, k_pages, v_pages, k_scales, v_scales, block_table)
-    with torch.cuda.device(qkv.device):
-        _e4m3_store(_ptr(q_out), q_out.stride(0) if q_out is not None else 0, qkv.data_ptr(), qkv.stride(0), k_off, v_off, heads, kv_heads,
-                    dim, vdim, rot_dims, inv_freq.data_ptr() if rot_dims else None, float(amplitude), positions.data_ptr(),
-                    token_item.data_ptr(), block_table.data_ptr() if writes else None, max_blocks, n_pages, page,
-                    k_pages.data_ptr() if writes else None, v_pages.data_ptr() if writes else None,
-                    k_scales.data_ptr() if writes else None, v_scales.data_ptr() if writes else None, n, dtype,
-                    _sm_count(qkv.device), _stream())
+        pages = (k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
+    _launch_on(index, _e4m3_store, _ptr(q_out), q_out.stride(0) if q_out is not None else 0, qkv.data_ptr(), qkv.stride(0), k_off, v_off, heads,
+               kv_heads, dim, vdim, rot_dims, inv_freq.data_ptr() if rot_dims else None, float(amplitude), positions.data_ptr(),
+               token_item.data_ptr(), block_table.data_ptr() if writes else None, max_blocks, n_pages, page, *pages, n, dtype,
+               _sm_count(index), _on_device(index))
     return q_out
 
 
@@ -2033,10 +2053,13 @@ class E4m3Workspace:
 
     def __init__(self, device, vdim: int, status=None):
         self.vdim = int(vdim)
-        n_sms = _sm_count(torch.device(device))
+        device = torch.device(device)
+        self.index = device.index if device.index is not None else torch.cuda.current_device()
+        n_sms = _sm_count(self.index)
         self.partial = torch.empty(2 * n_sms * 256 * (_padded_64(self.vdim) + 2), dtype=torch.float32, device=device)
         self.counters = torch.zeros(2 * n_sms, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device) if status is None else status
+        self.pointers = (self.partial.data_ptr(), self.counters.data_ptr(), self.status.data_ptr())
 
     def reset(self) -> None:
         """After a kernel gave up: counters and status start over."""
@@ -2062,48 +2085,44 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
     bring one token.  ``workspace`` (``e4m3_workspace``) is needed but with ``plain``: the kernel of every size and type, which 32-bit
     queries, and heads of more than 128 entries, take anyway."""
     who = "e4m3_attention"
-    n_pages, held_heads, page, dim, vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table)
     _check(q, f"{who}.q", None, 2)
-    _check(out, f"{who}.out", q.dtype, 2)
-    dtype = dtype_code(q.dtype)
-    if kv_heads != held_heads or heads <= 0 or heads % kv_heads != 0:
+    index, (n_rows, columns), dtype = q.get_device(), q.shape, dtype_code(q.dtype)
+    n_pages, held_heads, page, dim, vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, index)
+    if not _is(out, q.dtype, 2, index):
+        _refuse(out, f"{who}.out", q.dtype, 2, index)
+    if kv_heads != held_heads or heads <= 0 or heads % kv_heads:
         raise KernelError(f"{who}: {heads} heads over {kv_heads} key/value heads, pages hold {held_heads}")
-    if q.shape[1] != heads * dim or out.shape[0] != q.shape[0] or out.shape[1] != heads * vdim:
+    if columns != heads * dim or out.shape != (n_rows, heads * vdim):
         raise KernelError(f"{who}: q / out do not have heads * size columns")
-    _rows_of_sixteen_bytes(q, f"{who}.q")
-    _rows_of_sixteen_bytes(out, f"{who}.out")
-    n_items = block_table.shape[0]
+    if n_rows and not (_rows_fit(q) and _rows_fit(out)):
+        raise KernelError(f"{who}: rows of q and out must begin on 16-byte boundaries, their entries side by side")
+    n_items, max_blocks = block_table.shape
     for name, t in (("item_offset", item_offset), ("item_count", item_count), ("item_start", item_start)):
-        _check(t, f"{who}.{name}", torch.int32, 1)
-        n_items = min(n_items, t.shape[0])
-    if any(t.shape[0] > n_items for t in (item_offset, item_count, item_start)):
-        raise KernelError(f"{who}: offsets, counts and starts of the entries, and rows of the block table, differ in number")
+        if not _is(t, torch.int32, 1, index):
+            _refuse(t, f"{who}.{name}", torch.int32, 1, index)
+        if t.shape[0] != n_items or (n_items > 1 and t.stride(0) != 1):
+            raise KernelError(f"{who}: {name} does not hold a number for each of the block table's {n_items} rows, side by side")
     if not (window >= 0 and cap >= 0 and scale >= 0):
         raise KernelError(f"{who}: a window and a cap are positive, or 0 for none, and no scale is negative")
-    _check_same_device(who, q, out, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start)
     fast = not plain and e4m3_fast_takes(q.dtype, dim, vdim)
-    if fast and workspace is None:
-        raise KernelError(f"{who}: a workspace is needed (e4m3_workspace)")
+    pointers = (None, None, None)
     if fast:
-        _check_same_device(who, q, workspace.partial)
-        if _padded_64(vdim) > _padded_64(workspace.vdim):
-            raise KernelError(f"{who}: the workspace is for values of {workspace.vdim} entries, not {vdim}")
-    params = _E4m3Attention()
-    params.out, params.ld_out, params.q, params.ld_q = out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0)
-    params.k_pages, params.v_pages, params.k_scales, params.v_scales = (t.data_ptr() for t in (k_pages, v_pages, k_scales, v_scales))
-    params.block_table, params.max_blocks, params.n_pages, params.page = block_table.data_ptr(), block_table.shape[1], n_pages, page
-    params.item_offset, params.item_count, params.item_start = (t.data_ptr() for t in (item_offset, item_count, item_start))
-    params.n_items, params.n_heads, params.n_kv_heads, params.dim, params.vdim = n_items, heads, kv_heads, dim, vdim
-    params.scale, params.cap, params.window = float(scale), float(cap or 0.0), int(window or 0)
-    if fast:
-        params.partial, params.counters, params.status = (t.data_ptr() for t in (workspace.partial, workspace.counters, workspace.status))
-    with torch.cuda.device(q.device):
-        if not fast:
-            _e4m3_plain(ctypes.byref(params), q.shape[0], dtype, _stream())
-            return out
-        n_sms, stream = _sm_count(q.device), _stream()
-        if longest != 1:
-            _e4m3_tiles(ctypes.byref(params), q.shape[0], n_sms, stream)
-        if longest == 1 or singles:
-            _e4m3_step(ctypes.byref(params), n_sms, stream)
+        if workspace is None:
+            raise KernelError(f"{who}: a workspace is needed (e4m3_workspace)")
+        if workspace.index != index or _padded_64(vdim) > _padded_64(workspace.vdim):
+            raise KernelError(f"{who}: the workspace is for values of {workspace.vdim} entries on device {workspace.index}, not {vdim} on {index}")
+        pointers = workspace.pointers
+    params = ctypes.byref(_E4m3Attention(
+        out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+        block_table.data_ptr(), max_blocks, n_pages, page, item_offset.data_ptr(), item_count.data_ptr(), item_start.data_ptr(), n_items,
+        heads, kv_heads, dim, vdim, scale, cap or 0.0, window or 0, *pointers))
+    stream = _on_device(index)
+    if not fast:
+        _launch_on(index, _e4m3_plain, params, n_rows, dtype, stream)
+        return out
+    n_sms = _sm_count(index)
+    if longest != 1:
+        _launch_on(index, _e4m3_tiles, params, n_rows, n_sms, stream)
+    if longest == 1 or singles:
+        _launch_on(index, _e4m3_step, params, n_sms, stream)
     return out
