@@ -181,10 +181,13 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreParams 
         const double f = p.inv_freq[i] * 0.15915494309189535, of_turn = f - floor(f);
         const unsigned long long per_position = (unsigned long long)(of_turn * 18446744073709551616.0);
         for (int r = warp; r < rows; r += STORE_THREADS / 32) {
-            const int turns = (int)((per_position * (unsigned long long)(long long)row_pos[r + 1]) >> 32);      // in 2^-32, from -1/2 to 1/2
+            const uint32_t turns = (uint32_t)((per_position * (unsigned long long)(long long)row_pos[r + 1]) >> 32);      // in 2^-32
+            // the nearest quarter and what is left, an eighth at most: 2^-28 of a turn is lost where it becomes a 32-bit float
+            const uint32_t quarter = (turns + 0x20000000u) >> 30;
             float s, c;
-            sincospif((float)turns * 4.656612873077393e-10f, &s, &c);          // 2^-31: twice the turns
-            angles[r * pitch + i] = make_float2(c * p.amplitude, s * p.amplitude);
+            sincospif((float)(int)(turns - (quarter << 30)) * 4.656612873077393e-10f, &s, &c);                   // 2^-31: twice the turns
+            const float cosine = quarter & 1 ? -s : c, sine = quarter & 1 ? c : s, sign = quarter & 2 ? -p.amplitude : p.amplitude;
+            angles[r * pitch + i] = make_float2(cosine * sign, sine * sign);
         }
     }
     __syncthreads();
