@@ -101,11 +101,12 @@ def append(pages, scales, rows, rot, positions, items, table, inv_freq, amplitud
 
 def attention(q, k_pages, v_pages, k_scales, v_scales, table, entries, heads, scale, cap=0.0, window=0):
     """q [T, heads * dim]; entries (offset, count, start).  Returns (out [T, heads * vdim] with NaN-free zeros in rows of no entry,
-    weights' sums of |v| per entry of out, the largest sum of |q k| scale)."""
+    weights' sums of |v| per entry of out, the largest sum of |q k| scale, and per entry of out the number of keys times the largest
+    value a code may have times the largest weight times its value's scale)."""
     n_pages, kv_heads, page, dim = k_pages.shape
     vdim = v_pages.shape[3]
     out = np.zeros((q.shape[0], heads * vdim))
-    spread, most = np.zeros_like(out), 0.0
+    spread, edge, most = np.zeros_like(out), np.zeros_like(out), 0.0
     for item, (offset, count, start) in enumerate(entries):
         for i in range(count):
             position = start + i
@@ -130,8 +131,9 @@ def attention(q, k_pages, v_pages, k_scales, v_scales, table, entries, heads, sc
                     columns = slice(head * vdim, (head + 1) * vdim)
                     out[offset + i, columns] = p @ v
                     spread[offset + i, columns] = p @ np.abs(v)
+                    edge[offset + i, columns] = len(keys) * TOP * np.nanmax(np.append(p * v_scales[at, kv, slot // BLOCK], 0.0))
                     most = max(most, float(np.nan_to_num(np.abs(k) @ np.abs(row) * scale).max()))
-    return out, spread, most
+    return out, spread, most, edge
 
 
 def codes_of(pages):

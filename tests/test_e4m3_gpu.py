@@ -8,7 +8,9 @@ angle that is exact to 2^-24 turns: some 2^-21 of its pair, which is 448 scales 
 Attention in bfloat16: 2^-8 of the result for its own rounding, and of the sum of the weights times |v| 2^-11 for the
 weights, which are 16-bit floats, and 2^-20 (1 + size) for the scores: a score of products of sum `size` is some 8 sums cut off
 at 2^-23, its 32-bit arithmetic and the exponential a few units of 2^-24 of it, and an error of a score is as
-large a relative one of its weight.  With 32-bit queries sums of N terms, each rounded to 2^-24."""
+large a relative one of its weight.  A weight (times its value's scale) below 2^-14 of a 16-bit float's scale is off by half of 2^-24 whatever
+its size; the largest lies at 2^7 or above: 2^-32 of the largest for each key, times a code of 448 at most.  With 32-bit queries sums of
+N terms, each rounded to 2^-24, and weights down to 2^-126."""
 
 import numpy as np
 import pytest
@@ -280,20 +282,20 @@ def attend(pool, table, entries, q, heads, vdim, scale, dtype=torch.bfloat16, ou
 
 
 def check_attention(got, q, pool, table, entries, heads, scale, dtype, cap=0.0, window=0):
-    want, spread, most = plain.attention(q.float().cpu().numpy(), pool.codes["k"], pool.codes["v"], pool.scales["k"], pool.scales["v"], table,
+    want, spread, most, edge = plain.attention(q.float().cpu().numpy(), pool.codes["k"], pool.codes["v"], pool.scales["k"], pool.scales["v"], table,
                                          entries, heads, scale, cap, window)
     got = got.float().cpu().numpy().astype(np.float64)
     rows = np.zeros(got.shape[0], bool)
     for offset, count, _ in entries:
         rows[offset:offset + count] = True
     assert (got[~rows] == 3.0).all()
-    got, want, spread = got[rows], want[rows], spread[rows]
+    got, want, spread, edge = got[rows], want[rows], spread[rows], edge[rows]
     np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
     if dtype == torch.bfloat16:
-        bound = np.abs(want) * 2.0 ** -8 + spread * (2.0 ** -11 + 2.0 ** -20 * (1 + most))
+        bound = np.abs(want) * 2.0 ** -8 + spread * (2.0 ** -11 + 2.0 ** -20 * (1 + most)) + edge * 2.0 ** -32
     else:
         n = max(start + count for _, count, start in entries)
-        bound = np.abs(want) * 2.0 ** -24 + spread * 2.0 ** -24 * (n + 64 + 8 * (1 + most))
+        bound = np.abs(want) * 2.0 ** -24 + spread * 2.0 ** -24 * (n + 64 + 8 * (1 + most)) + edge * 2.0 ** -126
     off = np.abs(got - want)
     assert (off[~np.isnan(off)] <= bound[~np.isnan(off)]).all(), np.nanmax(off / np.maximum(bound, 1e-30))
 
@@ -353,3 +355,224 @@ def test_attention_of_portions(heads, kv_heads, dim, vdim, page, shapes, cap, wi
     got = attend(pool, table, entries, q, heads, vdim, scale, cap=cap, window=window, workspace=workspace)
     check_attention(got, q, pool, table, entries, heads, scale, torch.bfloat16, cap, window)
     assert int(workspace.status) == 0 and int(workspace.counters.abs().sum()) == 0
+
+
+# ---- what is no number, what lies elsewhere, and what the calls share ------------------------------
+
+def test_values_that_are_no_numbers_reach_only_the_rows_that_see_them():
+    """Position 70 of one request holds a key, position 150 a value that is none: queries before see numbers, queries from there on none, the
+    other request nothing of it; within a window only those that still see them."""
+    rng = np.random.default_rng(9)
+    heads, dim = 4, 64
+    for window in (0, 40):
+        pool, table = filled_pool(rng, [300, 300], 2, 32, dim, dim)
+        for name, position in (("k", 70), ("v", 150)):
+            pool.codes[name][table[0, position // 32], :, position % 32] = 127
+        pool.up()
+        for shapes in ([(200, 60), (100, 130)], [(1, 69), (1, 200)], [(1, 70), (1, 200)], [(1, 100), (1, 1)], [(1, 149), (1, 1)], [(1, 250), (30, 100)]):
+            entries = laid_out(shapes)
+            q = rows_of(rng, entries[-1][0] + entries[-1][1], heads * dim, torch.bfloat16)
+            got = attend(pool, table, entries, q, heads, dim, 0.05, window=window)
+            check_attention(got, q, pool, table, entries, heads, 0.05, torch.bfloat16, 0.0, window)
+            check_attention(attend(pool, table, entries, q, heads, dim, 0.05, window=window, plain=True), q, pool, table, entries, heads, 0.05,
+                            torch.bfloat16, 0.0, window)
+
+
+def test_queries_that_are_not_finite_stay_in_their_rows():
+    rng = np.random.default_rng(10)
+    pool, table = filled_pool(rng, [200], 1, 64, 64, 64)
+    q = rows_of(rng, 150, 2 * 64, torch.bfloat16)
+    bad = q.clone()
+    for row, value in ((3, float("nan")), (17, float("inf")), (140, -float("inf"))):
+        bad[row, 5] = value
+    for entries in ([(0, 150, 50)], [(3, 1, 100)], [(17, 1, 100)]):
+        clean, got = (attend(pool, table, entries, x, 2, 64, 0.1).float().cpu().numpy() for x in (q, bad))
+        rows = np.ones(150, bool)
+        rows[[3, 17, 140]] = False
+        np.testing.assert_array_equal(got[rows], clean[rows])
+        np.testing.assert_array_equal(got[:, 64:], clean[:, 64:])                 # (the other head)
+        offset, count, _ = entries[0]
+        assert np.isnan(got[[r for r in (3, 17, 140) if offset <= r < offset + count], :64]).all()
+
+
+def test_entries_without_tokens_or_keys_and_pages_that_are_none():
+    rng = np.random.default_rng(11)
+    pool, table = filled_pool(rng, [100, 100, 100, 100], 2, 16, 64, 64)
+    table[2, 1], table[3, 0] = -1, pool.codes["k"].shape[0] + 5                   # pages that the table does not name
+    # no tokens; a position before the first; keys missing in the middle and at the start
+    entries = [(0, 0, 50), (0, 1, -1), (1, 30, 40), (31, 1, 99), (32, 3, -2)]
+    table = np.concatenate((table, table[:1]))
+    q = rows_of(rng, 36, 4 * 64, torch.bfloat16)
+    for plain_kernel in (False, True):
+        got = attend(pool, table, entries, q, 4, 64, 0.1, plain=plain_kernel)
+        check_attention(got, q, pool, table, entries, 4, 0.1, torch.bfloat16)
+        assert (got[0] == 0).all() and (got[32:34] == 0).all() and not (got[34] == 0).all() and (got[35] == 3.0).all()
+    # an entry that reaches past its row of the table sees what the table names
+    entries = [(0, 1, 5000), (1, 40, 100), (41, 0, 0), (41, 0, 0), (41, 0, 0)]
+    q = rows_of(rng, 41, 4 * 64, torch.bfloat16)
+    check_attention(attend(pool, table, entries, q, 4, 64, 0.1), q, pool, table, entries, 4, 0.1, torch.bfloat16)
+
+
+def test_scales_far_apart_and_scores_far_apart():
+    """Blocks whose scales differ by 2^100, and queries that make scores of thousands: one block's values outweigh all others by far."""
+    rng = np.random.default_rng(12)
+    pool, table = filled_pool(rng, [400], 1, 16, 64, 64)
+    for block in range(25):
+        where = table[0, block]
+        pool.scales["v"][where, 0, 0] = 2.0 ** int(rng.integers(-64, 40))
+        pool.scales["k"][where, 0, 0] = 2.0 ** int(rng.integers(-12, -4))
+    pool.up()
+    q = rows_of(rng, 200, 3 * 64, torch.bfloat16)
+    for scale in (0.01, 3.0):
+        for entries in ([(0, 200, 200)], [(7, 1, 399)]):
+            got = attend(pool, table, entries, q, 3, 64, scale)
+            check_attention(got, q, pool, table, entries, 3, scale, torch.bfloat16)
+
+
+def test_results_do_not_depend_on_the_call_and_the_workspace_is_left_as_it_was():
+    """Twice the same bits, whatever the workspace held; rows of wider matrices; parts of units among many CTAs (long requests, few heads)."""
+    from mini_llm_b200.kernels import ops
+    rng = np.random.default_rng(13)
+    shapes = [(300, 3000), (1, 6000), (2, 0), (1, 17)]
+    pool, table = filled_pool(rng, [count + start for count, start in shapes], 1, 64, 128, 64)
+    entries = laid_out(shapes)
+    wide_q = rows_of(rng, 304, 2 * 128 + 16, torch.bfloat16)
+    q = wide_q[:, 8:8 + 256]
+    workspace = ops.e4m3_workspace("cuda", 128)
+    results = []
+    for fill in (0.0, float("nan")):
+        workspace.partial.fill_(fill)
+        wide_out = torch.full((304, 2 * 64 + 24), 5.0, dtype=torch.bfloat16, device="cuda")
+        attend(pool, table, entries, q, 2, 64, 0.05, out=wide_out[:, 16:16 + 128], workspace=workspace)
+        assert (wide_out[:, :16] == 5.0).all() and (wide_out[:, 144:] == 5.0).all()
+        results.append(wide_out[:, 16:144].clone())
+        assert int(workspace.status) == 0 and int(workspace.counters.abs().sum()) == 0
+    assert torch.equal(*results)
+    check_attention(results[0], q, pool, table, entries, 2, 0.05, torch.bfloat16)
+
+
+def test_another_stream_and_a_replayed_graph():
+    from mini_llm_b200.kernels import ops
+    rng = np.random.default_rng(14)
+    pool, table = filled_pool(rng, [700, 300, 40], 2, 32, 64, 64)
+    q = rows_of(rng, 300, 4 * 64, torch.bfloat16)
+    qkv = rows_of(rng, 300, 8 * 64, torch.bfloat16)
+    tables = ints(table)
+    plans = [[(0, 200, 300), (200, 1, 200), (201, 20, 3)], [(0, 1, 650), (1, 250, 10), (251, 40, 0)]]
+    offsets, counts, starts = (torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(3))
+    positions, items = (torch.zeros(300, dtype=torch.int32, device="cuda") for _ in range(2))
+    out, workspace = torch.zeros((300, 4 * 64), dtype=torch.bfloat16, device="cuda"), ops.e4m3_workspace("cuda", 64)
+
+    def step():
+        ops.e4m3_store(None, qkv, 4 * 64, 6 * 64, 4, 2, 64, 64, 0, None, 1.0, positions, items, tables, *pool.operands)
+        ops.e4m3_attention(out, q, *pool.operands, tables, offsets, counts, starts, 4, 2, 0.1, workspace=workspace)
+
+    def bring(plan):
+        for i, t in enumerate((offsets, counts, starts)):
+            t.copy_(ints([entry[i] for entry in plan]))
+        at, item = steps_arrays(plan)
+        positions.fill_(-1)
+        positions[:len(at)], items[:len(at)] = ints(at), ints(item)
+        out.fill_(3.0)
+
+    wanted, stores = [], []
+    first = [t.clone() for t in pool.operands]
+    for plan in plans:
+        bring(plan)
+        for t, before in zip(pool.operands, first):
+            t.copy_(before)
+        step()
+        wanted.append(out.clone())
+        stores.append([t.clone() for t in pool.operands])
+        pool.down()
+        check_attention(out, q, pool, table, plan, 4, 0.1, torch.bfloat16)
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for plan, want, store in list(zip(plans, wanted, stores)) * 2:
+        for run in ("graph", "stream"):
+            bring(plan)
+            for t, before in zip(pool.operands, first):
+                t.copy_(before)
+            if run == "graph":
+                graph.replay()
+            else:
+                stream.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(stream):
+                    step()
+                torch.cuda.current_stream().wait_stream(stream)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), run
+            for t, kept in zip(pool.operands, store):
+                assert torch.equal(t.view(torch.uint8), kept.view(torch.uint8))
+
+
+def test_offsets_past_four_gigabytes():
+    """Pages whose codes lie more than 2^32 bytes into the pool."""
+    from mini_llm_b200.kernels import ops
+    page, heads, dim = 128, 4, 128
+    pages = (5 << 30) // (heads * page * dim)
+    code = torch.float8_e4m3fn
+    k_pages, v_pages = (torch.zeros((pages, heads, page, dim), dtype=torch.uint8, device="cuda").view(code) for _ in range(2))
+    k_scales, v_scales = (torch.ones((pages, heads, page // 16), device="cuda") for _ in range(2))
+    rng = np.random.default_rng(15)
+    small = Pool(4, heads, page, dim, dim)
+    table = np.array([[3, 1, 2]], np.int32)
+    n = 300
+    qkv = rows_of(rng, n, 3 * heads * dim, torch.bfloat16)
+    inv_freq = torch.tensor(10000.0 ** (-np.arange(64) / 64), dtype=torch.float64, device="cuda")
+    results = []
+    for names, operands in ((table, small.operands), (table + pages - 4, (k_pages, v_pages, k_scales, v_scales))):
+        q = torch.empty((n, heads * dim), dtype=torch.bfloat16, device="cuda")
+        ops.e4m3_store(q, qkv, heads * dim, 2 * heads * dim, heads, heads, dim, dim, 128, inv_freq, 1.0, ints(np.arange(n)), ints([0] * n), ints(names), *operands)
+        for entry in ((0, n, 0), (0, 1, n - 1)):
+            out = torch.zeros((n, heads * dim), dtype=torch.bfloat16, device="cuda")
+            ops.e4m3_attention(out, q, *operands, ints(names), ints([entry[0]]), ints([entry[1]]), ints([entry[2]]), heads, heads, 0.01,
+                               workspace=ops.e4m3_workspace("cuda", dim))
+            results.append(out)
+    assert torch.equal(results[0], results[2]) and torch.equal(results[1], results[3]) and bool(results[0].abs().sum() > 0)
+
+
+def test_refusals():
+    from mini_llm_b200.kernels import ops
+    from mini_llm_b200.kernels.lib import KernelError
+    pool = Pool(3, 2, 32, 64, 64)
+    kp, vp, ks, vs = pool.operands
+    q, out = (torch.zeros((4, 4 * 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table, one, workspace = ints([[0, 1]]), ints([1]), ops.e4m3_workspace("cuda", 64)
+    good = dict(out=out, q=q, k_pages=kp, v_pages=vp, k_scales=ks, v_scales=vs, block_table=table, item_offset=ints([0]), item_count=one,
+                item_start=ints([0]), heads=4, kv_heads=2, scale=0.1, workspace=workspace)
+    ops.e4m3_attention(**good)
+    wide = torch.zeros((4, 4 * 64 + 4), dtype=torch.bfloat16, device="cuda")
+    for change, text in ((dict(q=q.cpu()), "CUDA tensor"), (dict(q=q.half()), "element type"), (dict(out=out.float()), "bfloat16"), (dict(out=out[:3]), "columns"),
+                         (dict(k_pages=kp.view(torch.uint8)), "float8"), (dict(k_pages=kp[:2]), "same pages"), (dict(v_pages=vp[:, :, :, ::2]), "contiguous"),
+                         (dict(k_scales=ks[:, :1]), "scales"), (dict(k_scales=ks.half()), "float32"), (dict(block_table=table.long()), "int32"),
+                         (dict(item_count=ints([1, 1])), "item_count"), (dict(item_start=ints([0]).long()), "int32"), (dict(heads=5), "heads over"),
+                         (dict(kv_heads=4), "heads over"), (dict(window=-1), "window"), (dict(cap=-1.0), "cap"), (dict(scale=-0.1), "scale"),
+                         (dict(scale=float("nan")), "scale"), (dict(workspace=None), "workspace"), (dict(q=wide[:, :256]), "16-byte"),
+                         (dict(out=wide[:, 2:258]), "16-byte")):
+        with pytest.raises(KernelError, match=text):
+            ops.e4m3_attention(**{**good, **change})
+    with pytest.raises(KernelError, match="workspace is for"):
+        big = Pool(2, 2, 32, 64, 128)
+        ops.e4m3_attention(**{**good, **dict(zip(("k_pages", "v_pages", "k_scales", "v_scales"), big.operands)),
+                              "out": torch.zeros((4, 4 * 128), dtype=torch.bfloat16, device="cuda")})
+    qkv = torch.zeros((4, 8 * 64), dtype=torch.bfloat16, device="cuda")
+    good = dict(q_out=out, qkv=qkv, k_off=256, v_off=384, heads=4, kv_heads=2, dim=64, vdim=64, rot_dims=64,
+                inv_freq=torch.ones(32, dtype=torch.float64, device="cuda"), amplitude=1.0, positions=ints([0, 1, 2, 3]), token_item=ints([0] * 4),
+                block_table=table, k_pages=kp, v_pages=vp, k_scales=ks, v_scales=vs)
+    ops.e4m3_store(**good)
+    for change, text in ((dict(qkv=qkv.cpu()), "CUDA tensor"), (dict(qkv=qkv.half()), "element type"), (dict(dim=60), "multiples of 16"), (dict(vdim=512), "multiples of 16"),
+                         (dict(rot_dims=63), "turned"), (dict(rot_dims=80), "turned"), (dict(v_off=400), "columns"), (dict(k_off=252), "multiples of 8"),
+                         (dict(inv_freq=torch.ones(31, dtype=torch.float64, device="cuda")), "frequencies"), (dict(inv_freq=None), "expected a CUDA"),
+                         (dict(inv_freq=torch.ones(32, device="cuda")), "float64"), (dict(positions=ints([0, 1])), "fewer positions"),
+                         (dict(token_item=ints([0] * 4).long()), "int32"), (dict(q_out=out[:, :128]), "columns"), (dict(q_out=out.float()), "bfloat16"),
+                         (dict(kv_heads=1), "another number"), (dict(k_pages=kp.view(torch.uint8)), "float8"), (dict(block_table=table[0]), "dimensions"),
+                         (dict(q_out=wide[:, 2:258]), "16-byte")):
+        with pytest.raises(KernelError, match=text):
+            ops.e4m3_store(**{**good, **change})
+    # nothing to do is no error
+    ops.e4m3_store(**{**good, "qkv": qkv[:0], "q_out": out[:0], "positions": ints([]), "token_item": ints([])})
+    none = torch.zeros((0, 2), dtype=torch.int32, device="cuda")
+    ops.e4m3_attention(out[:0], q[:0], kp, vp, ks, vs, none, ints([]), ints([]), ints([]), 4, 2, 0.1, workspace=workspace)
