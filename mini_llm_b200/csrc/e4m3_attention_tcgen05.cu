@@ -11,7 +11,11 @@
 // 16-bit float however far apart the scales lie.  Queries are scaled by a power of two to lie below 2^15.  O stays in tensor
 // memory; m moves, and O is scaled down, only where a score passes m by 8 (p stays below 2^15).
 //
-// What bounds it is the exponential (16 a clock and SM): 2,048 clocks a unit and block, against 1,024 of the products of heads of 64.
+// A unit and block takes the exponential's unit 2,048 clocks (16 a clock and SM), the tensor cores 1,024 with heads of 64 and 2,048 with 128, and reads
+// next to nothing from memory.  It takes 4,100 clocks with heads of 64 (a prompt of 16,000 tokens, 12 heads: 704 us, half of the exponential's rate) and
+// 5,200 with 128 (2,000 tokens behind 14,000, 32 heads: 573 us, 0.88 PFLOP/s): what lies between is the chain of a tile's turn, S, its largest, the
+// tile's meeting, the weights, P, which the other tile's turn fills in part, and the instruction fetch of four roles at once.  Without exponentials,
+// largest and conversion the chain alone still took 667 us of 766.
 //
 // The work is laid out on the device, from the entries alone (no list is made on the host, and a replayed graph takes any
 // entries): the units, each as long as its blocks and one more, stand in a row, and every CTA takes an equal stretch of it.  A unit that
@@ -27,7 +31,14 @@ namespace {
 constexpr int TILE = 128, UNIT = 2 * TILE;
 constexpr int GROUP_BYTES = TILE * 128;            // 128 rows of 64 16-bit floats
 constexpr int SOFTMAX_WARPS = 16, CONVERTER_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + CONVERTER_WARPS;
-constexpr int THREADS = (MMA_WARP + 2) * 32;       // 704: 88 registers each
+constexpr int THREADS = (MMA_WARP + 4) * 32;       // (the last two warps only make the fourth warp of their group up)
+// Registers a thread: all start with the same, and the last four warps, which need few, give up what the softmax warps take.  The shares never add up
+// to more than the block was launched with (`registers_suffice`).  790 us for 16,000 tokens of 12 heads of 64 without, 766 with it.
+constexpr int SOFTMAX_REGISTERS = 88, IDLE_REGISTERS = 48;
+constexpr bool registers_suffice(int at_launch) {
+    return THREADS / 32 * at_launch >= SOFTMAX_WARPS * SOFTMAX_REGISTERS + CONVERTER_WARPS * at_launch + 4 * IDLE_REGISTERS && at_launch >= IDLE_REGISTERS &&
+           at_launch <= SOFTMAX_REGISTERS;
+}
 constexpr int MAX_STAGES = 4;
 constexpr int MIN_STRETCH = 5;                     // of a CTA, where no unit is longer: its blocks and one more
 constexpr float LOG2E = 1.4426950408889634f;
@@ -213,9 +224,18 @@ struct Shared {
 };
 
 // (a role that gave up leaves its barriers as they are, so that the others' waits run out, or find out here)
+// By a whole warp, with one answer for all of its lanes: what follows does not branch apart, and the compiler knows it.  Code that is seldom reached
+// is kept out of the way here and in the softmax: 24 warps in four roles share the instruction caches, and what they fetch past, they wait for
+// (766 us and 612 us for 2,000 tokens at the end of 16,000 of 32 heads of 128 with all of it in line; 704 and 574 this way).
 __device__ __forceinline__ bool wait_or_fail(Shared& sh, uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait(bar, parity) && !*reinterpret_cast<volatile int*>(&sh.failed);
+    if (__builtin_expect(__any_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
+    const unsigned long long start = now_ns();
+    do {
+#pragma unroll 1
+        for (int i = 0; i < 256; i++)
+            if (__any_sync(0xffffffffu, mbar_try_wait(bar, parity))) return !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sh.failed));
+    } while (!__any_sync(0xffffffffu, now_ns() - start > WAIT_LIMIT_NS));
+    return false;
 }
 __device__ __forceinline__ void give_up(Shared& sh, const E4m3Attention& p, int code) {
     if (!*reinterpret_cast<volatile int*>(&sh.failed)) {
@@ -249,7 +269,7 @@ struct Blocks {
 
 // A warp's next unit (the k-th it asks for); false when there are none, or (`ok`) a wait ran out.
 __device__ __forceinline__ bool next_unit(Shared& sh, int k, Unit& u, bool& ok) {
-    ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.unit_full[k & 1], (k >> 1) & 1));
+    ok = wait_or_fail(sh, &sh.unit_full[k & 1], (k >> 1) & 1);
     if (!ok) return false;
     u = sh.unit[k & 1];
     __syncwarp();
@@ -342,6 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
     Unit u;
     if (warp < SOFTMAX_WARPS) {
         // ---- softmax: two threads a row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGISTERS));
         const int tile = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, row = tile * TILE + r;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_at = lanes + TILE * tile + 64 * half, o_at = lanes + O_AT + O_STEP * tile, p_at = lanes + P_AT + P_STEP * tile + P_HALF * half;
@@ -363,7 +384,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 const int s = ring.stage, key0 = (u.block_lo + j) * TILE + 64 * half;
                 // (the values' barrier too: what stands beside the tiles comes with it)
                 ok = wait_or_fail(sh, &sh.v_full[s], ring.parity) && wait_or_fail(sh, &sh.s_ready[tile], seen_blocks & 1);
-                ok = __all_sync(0xffffffffu, ok);
                 ring = ring.next(stages);
                 tcgen05_after_sync();
                 if (j == 0) q_factor = sh.q_factor[k & 1][row];
@@ -380,7 +400,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[i] = (bits >> i) & 1 ? v[i] : 0xff800000u;
                 };
-                // The row is read twice, 32 columns at a time (a loop body of all of them does not stay with the instructions near the warps).
+                // The row is read twice, 32 columns at a time (a loop body of all of them does not stay with the instructions near the warps: 4 %
+                // slower; 16 at a time are 3 % slower too, and so is the next chunk asked for before this one is worked on, 17 %).
                 // First its largest, in powers of two, with the values' scale (no factor is negative, and the cap keeps the order: the largest
                 // score is the largest product's).
                 float top = -INFINITY;
@@ -389,10 +410,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 for (int c = 0; ok && c < 64; c += 32) {
                     tmem_ask_32(s_at + c, v);
                     tmem_wait_32(v);
-                    if (needs_mask) {
+                    if (__builtin_expect(needs_mask, 0)) {
                         const uint32_t bits = seen(c);
                         if (((c == 0 ? none.x : none.y) & bits) != 0) sees_none = true;
                         mask(v, bits);
+                        tmem_store_bits_16(s_at + c, v), tmem_store_bits_16(s_at + c + 16, v + 16);      // (the second reading has no mask)
+                        tmem_stores_landed();
                     }
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
@@ -446,7 +469,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sh.s_read[tile]);
                     }
-                    if (needs_mask) mask(v, seen(c));
                     uint32_t packed[16];
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
@@ -595,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             const int id_first = look_up();
             // The queries, eight or sixteen lanes a row, once the unit that had this place before has read its own for the last time.
             unsigned char* q_here = q_tile + (k % Q_PLACES) * 2 * GROUPS * GROUP_BYTES;
-            ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.q_empty[k % Q_PLACES], ((k / Q_PLACES) & 1) ^ 1));
+            ok = wait_or_fail(sh, &sh.q_empty[k % Q_PLACES], ((k / Q_PLACES) & 1) ^ 1);
             if (!ok) break;
             {
                 constexpr int LANES = 8 * GROUPS, ROWS = 32 / LANES, AT_ONCE = 8, OF_WARP = UNIT / CONVERTER_WARPS;
@@ -649,7 +671,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 const int s = ring.stage;
                 const uint32_t parity = ring.parity ^ 1;
                 const int id_next = look_up();
-                ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.k_empty[s], parity));
+                ok = wait_or_fail(sh, &sh.k_empty[s], parity);
                 if (!ok) break;
                 unsigned char* k_tile = k_stage + s * GROUPS * GROUP_BYTES;
                 unsigned char* v_tile = v_stage + s * GROUPS * GROUP_BYTES;
@@ -668,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.k_full[s]);
                 // What stands beside the tiles is read until the block's P is there, which its second product waits for: behind v_empty.
-                ok = __all_sync(0xffffffffu, wait_or_fail(sh, &sh.v_empty[s], parity));
+                ok = wait_or_fail(sh, &sh.v_empty[s], parity);
                 if (!ok) break;
                 if ((t & 15) == 0) {
                     sh.k_scale[s][t >> 4] = k_scale;
@@ -697,105 +719,100 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             if (!ok) break;
         }
         if (!ok && lane == 0) give_up(sh, p, 31);
-    } else if (warp == MMA_WARP) {
-        // ---- products ----
-        const uint32_t elected = elected_lane();
-        const uint32_t idesc_s = f16_instr_desc(TILE, TILE), idesc_o = f16_instr_desc(TILE, p.vdim) | IDESC_B_MN_MAJOR;
-        const int k_steps = p.dim / UMMA_K;
-        const uint64_t q_desc = make_smem_desc(smem_u32(q_tile)), k_desc = make_smem_desc(smem_u32(k_stage));
-        const uint64_t v_desc = make_smem_desc_mn(smem_u32(v_stage), GROUP_BYTES);
-        const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0);
-        uint32_t seen_blocks[2] = {0, 0}, seen_units[2] = {0, 0};
-        int q_place = 0;
-        auto issue_s = [&](int tile, int s) {
-            const uint64_t a = q_desc + (2 * q_place + tile) * GROUPS * (GROUP_BYTES >> 4), b = k_desc + s * GROUPS * (GROUP_BYTES >> 4);
-            int kk = 0;
-            for (; kk + 4 <= k_steps; kk += 4) {
-                const uint64_t group = (kk / 4) * (GROUP_BYTES >> 4);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(IDLE_REGISTERS));
+        if (warp == MMA_WARP) {
+            // ---- products ----
+            const uint32_t elected = elected_lane();
+            const uint32_t idesc_s = f16_instr_desc(TILE, TILE), idesc_o = f16_instr_desc(TILE, p.vdim) | IDESC_B_MN_MAJOR;
+            const uint64_t q_desc = make_smem_desc(smem_u32(q_tile)), k_desc = make_smem_desc(smem_u32(k_stage));
+            const uint64_t v_desc = make_smem_desc_mn(smem_u32(v_stage), GROUP_BYTES);
+            const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0);
+            uint32_t seen_blocks[2] = {0, 0}, seen_units[2] = {0, 0};
+            int q_place = 0;
+            auto issue_s = [&](int tile, int s) {
+                const uint64_t a = q_desc + (2 * q_place + tile) * GROUPS * (GROUP_BYTES >> 4), b = k_desc + s * GROUPS * (GROUP_BYTES >> 4);
 #pragma unroll
-                for (int i = 0; i < 4; i++) umma_by(elected, tmem0 + TILE * tile, a + group + 2 * i, b + group + 2 * i, idesc_s, kk + i > 0 ? 1u : 0u);
-            }
-#pragma unroll 1
-            for (; kk < k_steps; kk++) {
-                const uint64_t at = (kk / 4) * (GROUP_BYTES >> 4) + 2 * (kk % 4);
-                umma_by(elected, tmem0 + TILE * tile, a + at, b + at, idesc_s, kk > 0 ? 1u : 0u);
-            }
-            umma_commit_by(elected, &sh.s_ready[tile]);
-        };
-        auto issue_o = [&](int tile, int s, bool begins) {
-            const uint64_t b = v_desc + s * GROUPS * (GROUP_BYTES >> 4);
-            const uint32_t a = tmem0 + P_AT + P_STEP * tile, d = tmem0 + O_AT + O_STEP * tile;
-            umma_from_tmem_by(elected, d, a, b, idesc_o, begins ? 0u : 1u);
+                for (int kk = 0; kk < 4 * GROUPS; kk++) {          // (entries behind `dim` are zeros on both sides)
+                    const uint64_t at = (kk / 4) * (GROUP_BYTES >> 4) + 2 * (kk % 4);
+                    umma_by(elected, tmem0 + TILE * tile, a + at, b + at, idesc_s, kk > 0 ? 1u : 0u);
+                }
+                umma_commit_by(elected, &sh.s_ready[tile]);
+            };
+            auto issue_o = [&](int tile, int s, bool begins) {
+                const uint64_t b = v_desc + s * GROUPS * (GROUP_BYTES >> 4);
+                const uint32_t a = tmem0 + P_AT + P_STEP * tile, d = tmem0 + O_AT + O_STEP * tile;
+                umma_from_tmem_by(elected, d, a, b, idesc_o, begins ? 0u : 1u);
 #pragma unroll
-            for (int kk = 1; kk < TILE / UMMA_K; kk++)
-                umma_from_tmem_by(elected, d, a + (kk / 4) * P_HALF + (kk % 4) * (UMMA_K / 2), b + kk * (2048 >> 4), idesc_o, 1u);
-            umma_commit_by(elected, &sh.o_added[tile]);
-        };
-        bool ok = true;
-        for (int k = 0; next_unit(sh, k, u, ok); k++) {
-            const Blocks of_unit(u);
-            // (the same for all lanes, and the compiler knows it)
-            const int n0 = __shfl_sync(0xffffffffu, of_unit.n[0], 0), n1 = __shfl_sync(0xffffffffu, of_unit.n[1], 0), most = max(n0, n1);
-            q_place = k % Q_PLACES;
-            ok = wait_or_fail(sh, &sh.q_full[q_place], (k / Q_PLACES) & 1);
-            if (most > 0) {
-                ok = ok && wait_or_fail(sh, &sh.k_full[ring.stage], ring.parity);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tcgen05_after_sync();
-                if (n0 > 0) issue_s(0, ring.stage);
-                if (n1 > 0) issue_s(1, ring.stage);
-                umma_commit_by(elected, &sh.k_empty[ring.stage]);
-            }
-            for (int j = 0; j < most; j++) {
-                const Ring after = ring.next(stages);
-                ok = wait_or_fail(sh, &sh.v_full[ring.stage], ring.parity);
-                if (j + 1 < most) ok = ok && wait_or_fail(sh, &sh.k_full[after.stage], after.parity);
-#pragma unroll
-                for (int tile = 0; tile < 2; tile++) {
-                    const int n = tile == 0 ? n0 : n1;
-                    if (j >= n) continue;
-                    const uint32_t parity = (seen_blocks[tile] + j) & 1;
-                    if (P_APART && j + 1 < n) {
-                        ok = __all_sync(0xffffffffu, ok && wait_or_fail(sh, &sh.s_read[tile], parity));
-                        if (!ok) break;
-                        tcgen05_after_sync();
-                        issue_s(tile, after.stage);
-                    }
-                    // the unit before has read its O
-                    if (j == 0) ok = ok && wait_or_fail(sh, &sh.o_free[tile], (seen_units[tile] & 1) ^ 1);
-                    ok = __all_sync(0xffffffffu, ok && wait_or_fail(sh, &sh.p_ready[tile], parity));
+                for (int kk = 1; kk < TILE / UMMA_K; kk++)
+                    umma_from_tmem_by(elected, d, a + (kk / 4) * P_HALF + (kk % 4) * (UMMA_K / 2), b + kk * (2048 >> 4), idesc_o, 1u);
+                umma_commit_by(elected, &sh.o_added[tile]);
+            };
+            bool ok = true;
+            for (int k = 0; next_unit(sh, k, u, ok); k++) {
+                const Blocks of_unit(u);
+                // (the same for all lanes, and the compiler knows it)
+                const int n0 = __shfl_sync(0xffffffffu, of_unit.n[0], 0), n1 = __shfl_sync(0xffffffffu, of_unit.n[1], 0), most = max(n0, n1);
+                q_place = k % Q_PLACES;
+                ok = wait_or_fail(sh, &sh.q_full[q_place], (k / Q_PLACES) & 1);
+                if (most > 0) {
+                    ok = ok && wait_or_fail(sh, &sh.k_full[ring.stage], ring.parity);
                     if (!ok) break;
                     tcgen05_after_sync();
-                    issue_o(tile, ring.stage, j == 0);
-                    if (!P_APART && j + 1 < n) issue_s(tile, after.stage);
+                    if (n0 > 0) issue_s(0, ring.stage);
+                    if (n1 > 0) issue_s(1, ring.stage);
+                    umma_commit_by(elected, &sh.k_empty[ring.stage]);
+                }
+                for (int j = 0; j < most; j++) {
+                    const Ring after = ring.next(stages);
+                    ok = wait_or_fail(sh, &sh.v_full[ring.stage], ring.parity);
+                    if (j + 1 < most) ok = ok && wait_or_fail(sh, &sh.k_full[after.stage], after.parity);
+#pragma unroll
+                    for (int tile = 0; tile < 2; tile++) {
+                        const int n = tile == 0 ? n0 : n1;
+                        if (j >= n) continue;
+                        const uint32_t parity = (seen_blocks[tile] + j) & 1;
+                        if (P_APART && j + 1 < n) {
+                            ok = ok && wait_or_fail(sh, &sh.s_read[tile], parity);
+                            if (!ok) break;
+                            tcgen05_after_sync();
+                            issue_s(tile, after.stage);
+                        }
+                        // the unit before has read its O
+                        if (j == 0) ok = ok && wait_or_fail(sh, &sh.o_free[tile], (seen_units[tile] & 1) ^ 1);
+                        ok = ok && wait_or_fail(sh, &sh.p_ready[tile], parity);
+                        if (!ok) break;
+                        tcgen05_after_sync();
+                        issue_o(tile, ring.stage, j == 0);
+                        if (!P_APART && j + 1 < n) issue_s(tile, after.stage);
+                    }
+                    if (!ok) break;
+                    umma_commit_by(elected, &sh.v_empty[ring.stage]);
+                    if (j + 1 < most) umma_commit_by(elected, &sh.k_empty[after.stage]);
+                    ring = after;
                 }
                 if (!ok) break;
-                umma_commit_by(elected, &sh.v_empty[ring.stage]);
-                if (j + 1 < most) umma_commit_by(elected, &sh.k_empty[after.stage]);
-                ring = after;
+                umma_commit_by(elected, &sh.q_empty[q_place]);
+                seen_blocks[0] += n0, seen_blocks[1] += n1;
+                seen_units[0] += n0 > 0 ? 1 : 0, seen_units[1] += n1 > 0 ? 1 : 0;
             }
-            if (!ok) break;
-            umma_commit_by(elected, &sh.q_empty[q_place]);
-            seen_blocks[0] += n0, seen_blocks[1] += n1;
-            seen_units[0] += n0 > 0 ? 1 : 0, seen_units[1] += n1 > 0 ? 1 : 0;
-        }
-        if (!ok && lane == 0) give_up(sh, p, 33);
-    } else {
-        // ---- the next unit, while the others work on this one ----
-        Schedule schedule(p, lane);
-        for (int k = 0;; k++) {
-            if (!__all_sync(0xffffffffu, wait_or_fail(sh, &sh.unit_empty[k & 1], ((k >> 1) & 1) ^ 1))) {
-                if (lane == 0) give_up(sh, p, 35);
-                break;
+            if (!ok && lane == 0) give_up(sh, p, 33);
+        } else if (warp == MMA_WARP + 1) {
+            // ---- the next unit, while the others work on this one ----
+            Schedule schedule(p, lane);
+            for (int k = 0;; k++) {
+                if (!wait_or_fail(sh, &sh.unit_empty[k & 1], ((k >> 1) & 1) ^ 1)) {
+                    if (lane == 0) give_up(sh, p, 35);
+                    break;
+                }
+                u.entry = -1;
+                const bool more = schedule.next(u);
+                if (lane == 0) {
+                    sh.unit[k & 1] = u;
+                    mbar_arrive(&sh.unit_full[k & 1]);
+                }
+                if (!more) break;
             }
-            u.entry = -1;
-            const bool more = schedule.next(u);
-            if (lane == 0) {
-                sh.unit[k & 1] = u;
-                mbar_arrive(&sh.unit_full[k & 1]);
-            }
-            if (!more) break;
         }
     }
     __syncthreads();
@@ -813,6 +830,14 @@ extern "C" int mllm_e4m3_tiles_attention(const E4m3Attention* p, int n_rows, int
     static size_t raised[4][64];
     auto kernel = which == 0 ? attention_tiles_kernel<false, 1> : which == 1 ? attention_tiles_kernel<false, 2>
                 : which == 2 ? attention_tiles_kernel<true, 1> : attention_tiles_kernel<true, 2>;
+    static bool suffices[4];
+    if (!suffices[which]) {
+        cudaFuncAttributes attributes;
+        const cudaError_t e = cudaFuncGetAttributes(&attributes, kernel);
+        if (e != cudaSuccess) return launched(e, "e4m3_attention_tiles");
+        if (!registers_suffice(attributes.numRegs)) return fail("e4m3_attention_tiles: built with other registers than its warps share out");
+        suffices[which] = true;
+    }
     const cudaError_t e = raise_shared_limit(kernel, bytes, raised[which]);
     if (e != cudaSuccess) return launched(e, "e4m3_attention_tiles");
     return launched(launch_kernel(g_dependent_launch != 0, kernel, dim3(n_sms), dim3(THREADS), bytes, (cudaStream_t)stream, *p, stages),

@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attention_plain_kernel(const E4
 //     order of the columns within a product does not matter as long as Q has the same;
 //   O^T = V^T P^T: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 and columns 8 g .. 8 g + 7 of each: the pairs of keys are put together byte by byte.
 // (With the heads as rows half of the products' rows are empty for up to eight heads: 632 instructions a block of 128 columns, 113 us for
-// 131,072 keys of 8 heads of 128; this way ... us.)
+// 131,072 keys of 8 heads of 128; this way 58 us.)
 // Q is scaled by a power of two to lie below 2^15 in 16-bit floats (11 bits: bfloat16's 8 fit; an entry 2^29 below the largest of its head
 // begins to lose some, where the 32-bit sum has lost it already).  The weights: a block's value scale 2^t joins the score as t in
 // the exponent, p = 2^(s + t - m + 7), and the sum of the weights gets p / 2^t: no multiplication more, and p keeps the 11 bits of a 16-bit
