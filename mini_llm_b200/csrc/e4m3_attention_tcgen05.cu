@@ -473,7 +473,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
                         const int group = 4 * half + c / 16 + g;
-                        const float from = sh.v_exponent[s][group] - base, factor = q_factor * sh.k_scale[s][group];
+                        // (never zero, which no hidden score's minus infinity would outlast: queries or a scale that small make scores of
+                        // nothing either way)
+                        const float from = sh.v_exponent[s][group] - base, factor = fmaxf(q_factor * sh.k_scale[s][group], 0x1p-126f);
                         float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {

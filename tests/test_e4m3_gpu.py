@@ -429,6 +429,21 @@ def test_scales_far_apart_and_scores_far_apart():
             check_attention(got, q, pool, table, entries, 3, scale, torch.bfloat16)
 
 
+@pytest.mark.parametrize("cap, window", [(0.0, 0), (7.0, 0), (0.0, 20)])
+@pytest.mark.parametrize("power, scale", [(0, 0.0), (-100, 0.25), (-126, 2.0 ** -126), (-30, 2.0 ** -120)])
+def test_scores_that_vanish(power, scale, cap, window):
+    """No scale, and queries or a scale so small that a product of factors is below every 32-bit number: all visible keys weigh the same, and
+    what is hidden stays hidden."""
+    rng = np.random.default_rng(14)
+    shapes = [(150, 70), (1, 99), (3, 0), (1, 0), (1, 300)]
+    pool, table = filled_pool(rng, [count + start for count, start in shapes], 2, 32, 64, 48)
+    entries = laid_out(shapes)
+    q = (rows_of(rng, entries[-1][0] + 1, 4 * 64, torch.bfloat16).float() * 2.0 ** power).to(torch.bfloat16)
+    for plain_kernel in (False, True):
+        got = attend(pool, table, entries, q, 4, 48, scale, cap=cap, window=window, plain=plain_kernel)
+        check_attention(got, q, pool, table, entries, 4, scale, torch.bfloat16, cap, window)
+
+
 def test_results_do_not_depend_on_the_call_and_the_workspace_is_left_as_it_was():
     """Twice the same bits, whatever the workspace held; rows of wider matrices; parts of units among many CTAs (long requests, few heads)."""
     from mini_llm_b200.kernels import ops
