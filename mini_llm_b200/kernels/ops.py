@@ -1896,6 +1896,8 @@ def add_normed_norm(hidden, y, gain, eps, normed, next_gain, next_eps):
 
 E4M3_BLOCK = 16
 E4M3_NONE = 0x7f               # the code that is no number
+E4M3_LEAST_CAP = 2.0 ** -100   # (its inverse is a 32-bit number)
+E4M3_MOST_CAP = 8192.0         # (a capped score is off by 2^-22 of the cap: here 2^-9, half of what a bfloat16 result is rounded by)
 E4M3_FAST_SIZES = 128          # entries of a key or value up to which the kernels on tensor cores take them
 
 
@@ -1995,10 +1997,12 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
     Rows of ``qkv`` (fp32 or bf16 [T, columns]) hold [q | k | v], k from column ``k_off``, v from ``v_off``.  The first ``rot_dims``
     entries of every query and key head turn in interleaved pairs by position * ``inv_freq`` [rot_dims / 2] (float64; None without
     turned entries), cosine and sine times ``amplitude``.  The turned queries go to ``q_out`` [T, heads * dim] (None: they are
-    not wanted); ``qkv`` stays as it is.  ``writes=False``: queries only.
+    not wanted), which may be the queries' own columns of ``qkv``, and no other part of it; all else of ``qkv`` stays as it is.
+    ``writes=False``: queries only.
 
-    Row t goes to position ``positions[t]`` of the request in row ``token_item[t]`` of the block table.  A request's rows stand side by
-    side at positions that grow by one; a row at a negative position, or whose page the table does not name (an index
+    Row t goes to position ``positions[t]`` of the request in row ``token_item[t]`` of the block table, which has that row.  A request's
+    rows stand side by side at positions that grow by one (rows of one request that repeat a position, as rows that fill a step up do, may
+    leave anything in the blocks that they name, and nothing elsewhere); no two requests of a step store into one page; a row at a negative position, or whose page the table does not name (an index
     outside the pages, a column outside the table), is stored nowhere.  The scale of a block of 16 positions is the least power of two
     s >= 2^-64 with n <= (448 s)^2 for all its rows so far, n being x^2 + y^2 of a pair that turns (times ``amplitude``^2; a turn
     keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
@@ -2076,13 +2080,13 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
                    cap=0.0, window=0, longest=None, singles=True, workspace=None, plain=False):
     """Causal attention over a cache in 8 bits.  Entry i of the step: rows ``item_offset[i]`` .. + ``item_count[i]`` of ``q`` (fp32 or bf16
     [T, heads * dim]) and ``out`` [T, heads * vdim], at positions ``item_start[i]``, ... of the request in row i of the block table, whose
-    keys and values are stored up to there; entries have rows of their own, and rows of no entry stay as they are.  score =
-    q . k * ``scale``, with ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if
+    keys and values are stored up to there; entries have rows of their own within ``q``, and rows of no entry stay as they are.  A stored
+    head is NaN throughout or nowhere and a scale a power of two from 2^-64 on, as ``e4m3_store`` leaves them.  score = q . k * ``scale``, with ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if
     given; softmax and the weighted sum in 32 bits; query head h reads key/value head h // (heads / kv_heads).  A row that sees no key (a
     negative position) is zero; pages that the table does not name are not seen.
 
-    ``longest``: the most tokens of an entry, where the caller knows (1: a step of single tokens); ``singles``: whether some entry may
-    bring one token.  ``workspace`` (``e4m3_workspace``) is needed but with ``plain``: the kernel of every size and type, which 32-bit
+    ``longest=1``: the caller knows that no entry brings more than one token (one that does is left out: its rows stay as they are);
+    ``singles=False``: that none brings just one (likewise).  Other values of ``longest`` change nothing.  ``workspace`` (``e4m3_workspace``) is needed but with ``plain``: the kernel of every size and type, which 32-bit
     queries, and heads of more than 128 entries, take anyway."""
     who = "e4m3_attention"
     _check(q, f"{who}.q", None, 2)
@@ -2102,8 +2106,9 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
             _refuse(t, f"{who}.{name}", torch.int32, 1, index)
         if t.shape[0] != n_items or (n_items > 1 and t.stride(0) != 1):
             raise KernelError(f"{who}: {name} does not hold a number for each of the block table's {n_items} rows, side by side")
-    if not (window >= 0 and cap >= 0 and scale >= 0):
-        raise KernelError(f"{who}: a window and a cap are positive, or 0 for none, and no scale is negative")
+    if not (window >= 0 and (cap == 0 or E4M3_LEAST_CAP <= cap <= E4M3_MOST_CAP) and 0 <= scale < float("inf")):
+        raise KernelError(f"{who}: a window is positive and a cap between {E4M3_LEAST_CAP} and {E4M3_MOST_CAP}, or 0 for none, and a scale is "
+                          "finite and not negative")
     fast = not plain and e4m3_fast_takes(q.dtype, dim, vdim)
     pointers = (None, None, None)
     if fast:

@@ -252,6 +252,26 @@ def test_rows_without_a_place_are_stored_nowhere():
     np.testing.assert_array_equal(q.float().cpu().numpy(), qkv[:, :64].float().cpu().numpy())
 
 
+def test_rows_that_fill_a_step_up_leave_the_others_alone():
+    """Rows of one more request, all at position 0, as a step filled up to a round number of rows has them: what the other requests store is the same."""
+    from mini_llm_b200.kernels import ops
+    rng = np.random.default_rng(16)
+    heads, dim, real, filler = 2, 64, 37, 27
+    qkv = rows_of(rng, real + filler, 3 * heads * dim, torch.bfloat16)
+    table = ints([[3, 1], [0, -1], [4, 4]])                                        # page 4: of no request
+    items, positions = [0] * 30 + [1] * 7 + [2] * filler, list(range(11, 41)) + list(range(7)) + [0] * filler
+    pages = []
+    for n in (real, real + filler):
+        pool = Pool(5, heads, 32, dim, dim)
+        for tensor in pool.operands[2:]:
+            tensor.fill_(2.0 ** -64)
+        ops.e4m3_store(None, qkv[:n], heads * dim, 2 * heads * dim, heads, heads, dim, dim, 0, None, 1.0, ints(positions[:n]), ints(items[:n]),
+                       table, *pool.operands)
+        pages.append([tensor[:4].contiguous().view(torch.uint8) for tensor in pool.operands])
+    for alone, beside in zip(*pages):
+        assert torch.equal(alone, beside)
+
+
 # ---- attention -----------------------------------------------------------------------------------
 
 def filled_pool(rng, reaches, kv_heads, page, dim, vdim, spare=2):
@@ -429,6 +449,25 @@ def test_scales_far_apart_and_scores_far_apart():
             check_attention(got, q, pool, table, entries, 3, scale, torch.bfloat16)
 
 
+@pytest.mark.parametrize("cap", [2.0 ** -100, 1e-3, 8192.0])
+def test_caps_at_their_borders(cap):
+    """The least cap leaves all keys alike.  With the largest the hardware's approximations show: in cap * (1 - 2 r), r = 1 / (1 + e), the
+    exponential's error of 2^-22 moves 2 r by 2^-23 (r' = -r^2, e = 1), the reciprocal's unit in the last place by 2^-23, the sum's rounding by
+    2^-24: 1.25 * 2^-22 of the cap together."""
+    rng = np.random.default_rng(15)
+    shapes = [(140, 60), (1, 150), (1, 0)]
+    pool, table = filled_pool(rng, [count + start for count, start in shapes], 2, 32, 64, 48)
+    entries = laid_out(shapes)
+    q = rows_of(rng, entries[-1][0] + 1, 4 * 64, torch.bfloat16)
+    want, spread, most, edge = plain.attention(q.float().cpu().numpy(), pool.codes["k"], pool.codes["v"], pool.scales["k"], pool.scales["v"], table,
+                                               entries, 4, 0.1, cap)
+    # the bound of other caps, and the capped scores' error: a weight is off by as much, their sum too, and so twice that of the sum of |v|
+    bound = np.abs(want) * 2.0 ** -8 + spread * (2.0 ** -11 + 2.0 ** -20 * (1 + most) + 2 * 1.25 * 2.0 ** -22 * cap) + edge * 2.0 ** -32
+    for plain_kernel in (False, True):
+        got = attend(pool, table, entries, q, 4, 48, 0.1, cap=cap, plain=plain_kernel).float().cpu().numpy()
+        assert (np.abs(got - want) <= bound).all()
+
+
 @pytest.mark.parametrize("cap, window", [(0.0, 0), (7.0, 0), (0.0, 20)])
 @pytest.mark.parametrize("power, scale", [(0, 0.0), (-100, 0.25), (-126, 2.0 ** -126), (-30, 2.0 ** -120)])
 def test_scores_that_vanish(power, scale, cap, window):
@@ -565,6 +604,8 @@ def test_refusals():
                          (dict(k_scales=ks[:, :1]), "scales"), (dict(k_scales=ks.half()), "float32"), (dict(block_table=table.long()), "int32"),
                          (dict(item_count=ints([1, 1])), "item_count"), (dict(item_start=ints([0]).long()), "int32"), (dict(heads=5), "heads over"),
                          (dict(kv_heads=4), "heads over"), (dict(window=-1), "window"), (dict(cap=-1.0), "cap"), (dict(scale=-0.1), "scale"),
+                         (dict(cap=float("inf")), "cap"), (dict(cap=1e-40), "cap"), (dict(cap=float("nan")), "cap"), (dict(cap=8193.0), "cap"),
+                         (dict(scale=float("inf")), "scale"),
                          (dict(scale=float("nan")), "scale"), (dict(workspace=None), "workspace"), (dict(q=wide[:, :256]), "16-byte"),
                          (dict(out=wide[:, 2:258]), "16-byte")):
         with pytest.raises(KernelError, match=text):
