@@ -372,13 +372,15 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attention_plain_kernel(const E4
 //     order of the columns within a product does not matter as long as Q has the same;
 //   O^T = V^T P^T: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 and columns 8 g .. 8 g + 7 of each: the pairs of keys are put together byte by byte.
 // (With the heads as rows half of the products' rows are empty for up to eight heads: 632 instructions a block of 128 columns, 113 us for
-// 131,072 keys of 8 heads of 128; this way 58 us.)
+// 131,072 keys of 8 heads of 128; this way 381, 58 us, and 54.5, 4.9 TB/s, since what is seldom reached is kept out of the way and no place in the
+// ring is divided for.  Half of the issue slots and of the integer unit's, which converts codes, are taken then, with 16 warps an SM.)
 // Q is scaled by a power of two to lie below 2^15 in 16-bit floats (11 bits: bfloat16's 8 fit; an entry 2^29 below the largest of its head
 // begins to lose some, where the 32-bit sum has lost it already).  The weights: a block's value scale 2^t joins the score as t in
 // the exponent, p = 2^(s + t - m + 7), and the sum of the weights gets p / 2^t: no multiplication more, and p keeps the 11 bits of a 16-bit
 // float however far apart the scales lie.  m moves only where a score passes it by 8, so that p stays below 2^15.
 constexpr int STEP_WARPS = 8, STEP_THREADS = STEP_WARPS * 32, STEP_CTAS = 2;
-constexpr int STEP_SET_UP = 24;                // blocks that a unit's set-up counts as (some 6,500 clocks, at 150 to 250 a block)
+constexpr int STEP_SET_UP = 28;                // blocks that a unit's set-up counts as (64 requests of 100 to 4,000 tokens, 8 heads of 128: 16 as many
+                                               // 42.1 us, 20 39.2, 24 38.7, 28 38.3, 34 38.8)
 constexpr int STEP_LEAST = 16;                 // places of a stretch, where a unit is that long
 constexpr int STEP_RING_BYTES = 96 * 1024;     // of a CTA's blocks on their way
 
@@ -514,6 +516,7 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
     // a warp's ring: blocks, each behind its scales
     const int stage_bytes = 128 + E4M3_BLOCK * (dim + vdim);
     unsigned char* ring = reinterpret_cast<unsigned char*>(shared) + warp * stages * stage_bytes + 112;
+    unsigned char* ring_end = ring + stages * stage_bytes;
     wait_for_earlier_kernels();
     const uint8_t* k_pages = behind_the_wait(p.k_pages);
     const uint8_t* v_pages = behind_the_wait(p.v_pages);
@@ -561,12 +564,13 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
     take(u);
     for (;;) {
         const int lo = u.lo, pos = u.pos, first = u.first, n_rows = u.n_rows, n_parts = u.n_parts;
+        unsigned char *put = ring, *got = ring;            // where the next block goes to, and the one that is next lies
         // A block on its way: 16-byte chunks, each row's in an order in which no two lanes below read the same banks.
-        auto fetch = [&](int i) {                        // the warp's i-th block, into the ring's place i % stages
+        auto fetch = [&](int i) {                        // the warp's i-th block, into the ring's next place
             if (i < u.mine) {
-                if (i > 0 && (i & 31) == 0) u.here = u.ahead, u.ahead = look_up(u, lo + warp + (i + 32) * STEP_WARPS);
+                if (__builtin_expect(i > 0 && (i & 31) == 0, 0)) u.here = u.ahead, u.ahead = look_up(u, lo + warp + (i + 32) * STEP_WARPS);
                 const int place = __shfl_sync(0xffffffffu, u.here, i & 31);
-                unsigned char* to = ring + (i % stages) * stage_bytes;
+                unsigned char* to = put;
                 if (lane < 2) copy_4(to + 4 * lane, (lane == 0 ? p.k_scales : p.v_scales) + max(place, 0), place >= 0);     // (no scale: not there)
                 if (place >= 0) {
                     const uint8_t* k = k_pages + (long)place * E4M3_BLOCK * dim;
@@ -592,6 +596,7 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
                 }
             }
             copies_end();
+            put = put + stage_bytes == ring_end ? ring : put + stage_bytes;
         };
         for (int i = 0; i < stages - 1; i++) fetch(i);
 
@@ -668,6 +673,7 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
             const float t = (float)exponent_of(v_scale), over = 1.0f / v_scale;
             const int key0 = index * E4M3_BLOCK;
             const bool partial = key0 + E4M3_BLOCK - 1 > pos || key0 < first;
+            const float after = has_cap ? 0.0f : t;
             // scores of key g, heads 2 c and 2 c + 1, then of key g + 8
             float top[TILES][2];
             bool moves = false;
@@ -678,17 +684,19 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
                     const float factor = q_factor[h][e] * k_scale;
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
-                        const float y = s[h][2 * n + e] * factor;
-                        s[h][2 * n + e] = has_cap ? capped(y, cap_log2, cap_factor) + t : y + t;
+                        s[h][2 * n + e] = fmaf(s[h][2 * n + e], factor, after);
                     }
-                    if (partial) {
+                    if (__builtin_expect(has_cap, 0)) {
+                        s[h][e] = capped(s[h][e], cap_log2, cap_factor) + t, s[h][2 + e] = capped(s[h][2 + e], cap_log2, cap_factor) + t;
+                    }
+                    if (__builtin_expect(partial, 0)) {
                         if (key0 + g > pos || key0 + g < first) s[h][e] = -INFINITY;
                         if (key0 + g + 8 > pos || key0 + g + 8 < first) s[h][2 + e] = -INFINITY;
                     }
                     top[h][e] = fmaxf(s[h][e], s[h][2 + e]);
                     moves = moves || top[h][e] > m[h][e] + 8.0f;
                 }
-            if (__any_sync(0xffffffffu, moves)) {
+            if (__builtin_expect(__any_sync(0xffffffffu, moves), 0)) {
 #pragma unroll
                 for (int h = 0; h < TILES; h++)
 #pragma unroll
@@ -727,8 +735,14 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
                     const int key = 2 * c + (n & 1) + 8 * (n >> 1), col = 64 * d + 8 * g;
                     if (EXACT) rows[n] = *reinterpret_cast<const uint2*>(v + ((key * vdim + col) ^ (((key >> 1) & 3) << 5)));
                     else rows[n] = col < vdim ? *reinterpret_cast<const uint2*>(v + key * vdim + col) : make_uint2(0u, 0u);
-                    // (a masked key's value may be no number, and its weight of zero would not keep it out)
-                    if (partial && (key0 + key > pos || key0 + key < first)) rows[n] = make_uint2(0u, 0u);
+                }
+                // (a masked key's value may be no number, and its weight of zero would not keep it out)
+                if (__builtin_expect(partial, 0)) {
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const int key = key0 + 2 * c + (n & 1) + 8 * (n >> 1);
+                        if (key > pos || key < first) rows[n] = make_uint2(0u, 0u);
+                    }
                 }
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
@@ -749,7 +763,8 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
             else copies_landed<4>();
             __syncwarp();
             fetch(i + stages - 1);
-            work(ring + (i % stages) * stage_bytes, lo + warp + i * STEP_WARPS);
+            work(got, lo + warp + i * STEP_WARPS);
+            got = got + stage_bytes == ring_end ? ring : got + stage_bytes;
         }
         copies_landed<0>();
         __syncthreads();                                 // the ring's memory is the results' now
