@@ -19,7 +19,8 @@
 //
 // The work is laid out on the device, from the entries alone (no list is made on the host, and a replayed graph takes any
 // entries): the units, each as long as its blocks and one more, stand in a row, and every CTA takes an equal stretch of it.  A unit that
-// lies in several stretches leaves 32-bit results of its parts, which the CTA that arrives last adds up in order.  Every wait is bounded.
+// lies in several stretches leaves 32-bit results of its parts, which the CTA that arrives last adds up in order.  Where there are few units each is cut
+// by itself instead, so that no CTA begins two.  Every wait is bounded.
 #include "common.cuh"
 #include "e4m3.cuh"
 #include "tcgen05.cuh"
@@ -41,6 +42,8 @@ constexpr bool registers_suffice(int at_launch) {
 }
 constexpr int MAX_STAGES = 4;
 constexpr int MIN_STRETCH = 5;                     // of a CTA, where no unit is longer: its blocks and one more
+constexpr int MIN_STRETCH_APART = 3;               // the same where every unit is cut by itself, in blocks (prompts of 300 and 700 tokens, 12 heads of
+                                                   // 64: 2 15.8 and 19.7 us, 3 13.8 and 22.2; one row for all units 22.6 and 26.3)
 constexpr float LOG2E = 1.4426950408889634f;
 
 // What one thread of the MMA warp does while all of its lanes run: a warp that does not branch apart keeps descriptors where the
@@ -121,7 +124,9 @@ struct Schedule {
     const E4m3Attention& p;
     long total, stretch, lo, hi;                   // the row's length, a CTA's share, this CTA's
     long begin;                                    // of the unit that is next
-    int entry, tile, head, length, start, count;
+    int entry, tile, head, blocks, length, start, count;
+    int set_up;                                    // places that a unit's set-up takes
+    bool apart;                                    // every unit has CTAs of its own: it begins at a multiple of the stretch
 
     __device__ int first_block(int s, int t) const {
         const int first = p.window > 0 ? s + t * UNIT - p.window + 1 : 0;
@@ -131,25 +136,36 @@ struct Schedule {
         const int last = s + min(c, (t + 1) * UNIT) - 1;
         return last < 0 ? 0 : last / TILE - first_block(s, t) + 1;
     }
-    __device__ int length_of(int s, int c, int t) const { return blocks_of(s, c, t) + 1; }
+    __device__ int places(int of_blocks) const {
+        return apart ? (max(of_blocks, 1) + (int)stretch - 1) / (int)stretch * (int)stretch : of_blocks + set_up;
+    }
     __device__ static int tiles_of(int c) { return (c + UNIT - 1) / UNIT; }
 
     __device__ Schedule(const E4m3Attention& params, int lane) : p(params), total(0), entry(-1) {
-        int sum = 0, most = 0;
+        int sum = 0, none = 0, most = 0, units = 0;         // blocks of this lane's units, those without any, the longest; all units
         for (int base = 0; base < p.n_items; base += 32) {
             const int e = base + lane;
             const int c_of = e < p.n_items ? p.item_count[e] : 0, s_of = e < p.n_items ? p.item_start[e] : 0;
             for (uint32_t bits = __ballot_sync(0xffffffffu, c_of > 1); bits != 0; bits &= bits - 1) {
                 const int c = __shfl_sync(0xffffffffu, c_of, __ffs(bits) - 1), s = __shfl_sync(0xffffffffu, s_of, __ffs(bits) - 1);
                 for (int t = lane; t < tiles_of(c); t += 32) {
-                    const int n = length_of(s, c, t);
-                    sum += n, most = max(most, n);
+                    const int n = blocks_of(s, c, t);
+                    sum += n, none += n == 0 ? 1 : 0, most = max(most, n);
                 }
+                units += tiles_of(c);
             }
         }
-        total = (long)__reduce_add_sync(0xffffffffu, sum) * p.n_heads;
+        // Equal stretches of the row of all units, or, where there are fewer units than CTAs, every unit cut by itself, if that makes the longest
+        // stretch no longer.
+        const long all = (long)__reduce_add_sync(0xffffffffu, sum) * p.n_heads, of_units = (long)units * p.n_heads, grid = gridDim.x;
+        const long cut = all + (long)__reduce_add_sync(0xffffffffu, none) * p.n_heads;
         most = __reduce_max_sync(0xffffffffu, most);
-        stretch = max((total + gridDim.x - 1) / gridDim.x, (long)min(most, MIN_STRETCH));
+        const long together = max((all + of_units + grid - 1) / grid, (long)min(most + 1, MIN_STRETCH));
+        const long by_itself = of_units < grid ? max((cut + grid - of_units - 1) / (grid - of_units), (long)min(max(most, 1), MIN_STRETCH_APART)) : 0;
+        apart = by_itself > 0 && by_itself <= together;
+        set_up = apart ? 0 : 1;
+        stretch = apart ? by_itself : together;
+        total = apart ? grid * stretch : all + of_units;         // (no longer than that, where the units stand apart)
         lo = blockIdx.x * stretch, hi = min(total, lo + stretch);
         if (lo >= hi) return;
         // the unit in which the stretch begins
@@ -162,7 +178,7 @@ struct Schedule {
                 const int c = __shfl_sync(0xffffffffu, c_of, src), s = __shfl_sync(0xffffffffu, s_of, src), n = tiles_of(c);
                 for (int first = 0; first < n; first += 32) {
                     const int t = n - 1 - first - lane;
-                    const int mine = t >= 0 ? length_of(s, c, t) : 0;
+                    const int of_lane = t >= 0 ? blocks_of(s, c, t) : 0, mine = t >= 0 ? places(of_lane) : 0;
                     int upto = mine;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
@@ -172,7 +188,7 @@ struct Schedule {
                     const uint32_t past = __ballot_sync(0xffffffffu, begin + (long)upto * p.n_heads > lo);
                     if (past != 0) {
                         const int at = __ffs(past) - 1;
-                        length = __shfl_sync(0xffffffffu, mine, at);
+                        length = __shfl_sync(0xffffffffu, mine, at), blocks = __shfl_sync(0xffffffffu, of_lane, at);
                         begin += (long)__shfl_sync(0xffffffffu, upto - mine, at) * p.n_heads;
                         head = (int)((lo - begin) / length);
                         begin += (long)head * length;
@@ -183,6 +199,7 @@ struct Schedule {
                 }
             }
         }
+        hi = lo;                                   // the row ends before
     }
     __device__ bool next(Unit& u) {
         if (lo >= hi || begin >= hi) return false;
@@ -190,8 +207,8 @@ struct Schedule {
         const int from = (int)(max(lo, begin) - begin), to = (int)(min(hi, end) - begin);      // place 0 is the unit's set-up
         u.entry = entry, u.head = head;
         u.row0 = p.item_offset[entry] + tile * UNIT, u.rows = min(UNIT, count - tile * UNIT), u.pos0 = start + tile * UNIT;
-        u.block_lo = first_block(start, tile) + max(0, from - 1);
-        u.blocks = max(0, to - 1) - max(0, from - 1);
+        u.block_lo = first_block(start, tile) + max(0, from - set_up);
+        u.blocks = min(blocks, max(0, to - set_up)) - max(0, from - set_up);
         u.first_cta = (int)(begin / stretch);
         u.parts = (int)((end - 1) / stretch) - u.first_cta + 1;
         u.part = (int)blockIdx.x - u.first_cta;
@@ -203,7 +220,7 @@ struct Schedule {
                 start = p.item_start[entry], count = p.item_count[entry];
                 tile = tiles_of(count) - 1;
             }
-            length = length_of(start, count, tile);
+            blocks = blocks_of(start, count, tile), length = places(blocks);
         }
         return true;
     }
