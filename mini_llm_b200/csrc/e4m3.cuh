@@ -52,6 +52,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// a / b of numbers that are not negative (the 64-bit division costs some hundred clocks, and a row is hardly ever that long).
+__device__ __forceinline__ long divided(long a, long b) {
+    return ((a | b) >> 31) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // cap * tanh(x / cap) = cap * (1 - 2 / (1 + e^(2x / cap))): two of the hardware's approximations with an error of some 2^-22 of the
 // cap, where its approximate tanh has 2^-11: of a cap of 50 that would be 2.4 % of a weight.
 __device__ __forceinline__ float capped(float x, float cap, float two_log2e_over_cap) {

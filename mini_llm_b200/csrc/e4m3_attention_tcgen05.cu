@@ -5,17 +5,18 @@
 //   converter warps  read a block's codes, page by page, and leave them as 16-bit floats in shared memory, swizzled like a TMA tile
 //                    (every code is one exactly; the scales stay outside); both tiles use them;
 //   MMA warp         S = Q K^T with tcgen05.mma into tensor memory, then O += P V, P from tensor memory;
-//   softmax warps    two threads a row, each with 64 of a block's columns: read S, apply scale, cap and mask, write P as 16-bit floats.
+//   softmax warps    two threads a row, each with 64 of a block's columns: read S, apply scale, cap and mask, write P as 16-bit floats; and, since they have
+//                    nothing else to do at a unit's start, its queries.
 // While one tile's softmax runs the other's products do.  Scales cost nothing an entry: a block of 16 keys has one factor for its scores, and
 // its values' scale 2^t goes into the exponent, p = 2^(s + t - m + 7), with the sum of the weights getting p / 2^t; p keeps the 11 bits of a
 // 16-bit float however far apart the scales lie.  Queries are scaled by a power of two to lie below 2^15.  O stays in tensor
 // memory; m moves, and O is scaled down, only where a score passes m by 8 (p stays below 2^15).
 //
 // A unit and block takes the exponential's unit 2,048 clocks (16 a clock and SM), the tensor cores 1,024 with heads of 64 and 2,048 with 128, and reads
-// next to nothing from memory.  It takes 4,100 clocks with heads of 64 (a prompt of 16,000 tokens, 12 heads: 704 us, half of the exponential's rate) and
-// 5,200 with 128 (2,000 tokens behind 14,000, 32 heads: 573 us, 0.88 PFLOP/s): what lies between is the chain of a tile's turn, S, its largest, the
+// next to nothing from memory.  It takes 4,250 clocks with heads of 64 (a prompt of 16,000 tokens, 12 heads: 732 us, half of the exponential's rate) and
+// 5,250 with 128 (2,000 tokens behind 14,000, 32 heads: 577 us, 0.87 PFLOP/s): what lies between is the chain of a tile's turn, S, its largest, the
 // tile's meeting, the weights, P, which the other tile's turn fills in part, and the instruction fetch of four roles at once.  Without exponentials,
-// largest and conversion the chain alone still took 667 us of 766.
+// largest and conversion the chain alone still took 667 us of 766 in an earlier state.
 //
 // The work is laid out on the device, from the entries alone (no list is made on the host, and a replayed graph takes any
 // entries): the units, each as long as its blocks and one more, stand in a row, and every CTA takes an equal stretch of it.  A unit that
@@ -160,8 +161,8 @@ struct Schedule {
         const long all = (long)__reduce_add_sync(0xffffffffu, sum) * p.n_heads, of_units = (long)units * p.n_heads, grid = gridDim.x;
         const long cut = all + (long)__reduce_add_sync(0xffffffffu, none) * p.n_heads;
         most = __reduce_max_sync(0xffffffffu, most);
-        const long together = max((all + of_units + grid - 1) / grid, (long)min(most + 1, MIN_STRETCH));
-        const long by_itself = of_units < grid ? max((cut + grid - of_units - 1) / (grid - of_units), (long)min(max(most, 1), MIN_STRETCH_APART)) : 0;
+        const long together = max(divided(all + of_units + grid - 1, grid), (long)min(most + 1, MIN_STRETCH));
+        const long by_itself = of_units < grid ? max(divided(cut + grid - of_units - 1, grid - of_units), (long)min(max(most, 1), MIN_STRETCH_APART)) : 0;
         apart = by_itself > 0 && by_itself <= together;
         set_up = apart ? 0 : 1;
         stretch = apart ? by_itself : together;
@@ -190,7 +191,7 @@ struct Schedule {
                         const int at = __ffs(past) - 1;
                         length = __shfl_sync(0xffffffffu, mine, at), blocks = __shfl_sync(0xffffffffu, of_lane, at);
                         begin += (long)__shfl_sync(0xffffffffu, upto - mine, at) * p.n_heads;
-                        head = (int)((lo - begin) / length);
+                        head = (int)divided(lo - begin, length);
                         begin += (long)head * length;
                         entry = base + src, tile = n - 1 - first - at, start = s, count = c;
                         return;
@@ -209,8 +210,8 @@ struct Schedule {
         u.row0 = p.item_offset[entry] + tile * UNIT, u.rows = min(UNIT, count - tile * UNIT), u.pos0 = start + tile * UNIT;
         u.block_lo = first_block(start, tile) + max(0, from - set_up);
         u.blocks = min(blocks, max(0, to - set_up)) - max(0, from - set_up);
-        u.first_cta = (int)(begin / stretch);
-        u.parts = (int)((end - 1) / stretch) - u.first_cta + 1;
+        u.first_cta = (int)divided(begin, stretch);
+        u.parts = (int)divided(end - 1, stretch) - u.first_cta + 1;
         u.part = (int)blockIdx.x - u.first_cta;
         begin = end;
         if (++head == p.n_heads && begin < hi) {
@@ -227,13 +228,13 @@ struct Schedule {
 };
 
 struct Shared {
-    uint64_t unit_full[2], unit_empty[2], q_full[2], q_empty[2];
+    uint64_t unit_full[2], unit_empty[2], q_full[2];
     uint64_t k_full[MAX_STAGES], k_empty[MAX_STAGES], v_full[MAX_STAGES], v_empty[MAX_STAGES];
     uint64_t s_ready[2], s_read[2], p_ready[2], o_added[2], o_free[2];
     uint32_t tmem;
     int failed, ticket[2];
     Unit unit[2];                                  // entry < 0: there are no more
-    float q_factor[2][UNIT];
+    float q_factor[UNIT];
     float of_half[2][2][TILE];                     // what the two threads of a row tell one another
     // of the blocks of 16 keys: the keys' scale, the values' scale's exponent, and one by the values' scale
     float k_scale[MAX_STAGES][TILE / E4M3_BLOCK], v_exponent[MAX_STAGES][TILE / E4M3_BLOCK], v_inverse[MAX_STAGES][TILE / E4M3_BLOCK];
@@ -330,6 +331,44 @@ __device__ __forceinline__ void store_sixteen(bf16* to, const float (&o)[16], fl
     *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
+// 16 rows of a unit's queries into shared memory, by a warp, eight or sixteen lanes a row: as 16-bit floats of a power of two's size, and what
+// brings a row's scores into powers of two.
+template <bool CAP, int GROUPS>
+__device__ __forceinline__ void put_queries(const E4m3Attention& p, const Unit& u, unsigned char* to, float* factors, int first_row, int lane) {
+    constexpr int LANES = 8 * GROUPS, ROWS = 32 / LANES, AT_ONCE = 4, OF_WARP = UNIT / SOFTMAX_WARPS;
+    const int chunk = lane % LANES, row0 = first_row + lane / LANES;
+    const bf16* from = static_cast<const bf16*>(p.q) + (long)u.row0 * p.ld_q + (long)u.head * p.dim + 8 * chunk;
+#pragma unroll 1
+    for (int base = 0; base < OF_WARP; base += AT_ONCE * ROWS) {
+        uint4 v[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const int row = row0 + base + i * ROWS;
+            v[i] = row < u.rows && 8 * chunk < p.dim ? *reinterpret_cast<const uint4*>(from + row * p.ld_q) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const int row = row0 + base + i * ROWS;
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            float top = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; c++) top = max_of_three(top, fabsf(__uint_as_float(w[c] << 16)), fabsf(__uint_as_float(w[c] & 0xffff0000u)));
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // (zeros, and what is not finite, stay as they are)
+            const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
+            const float factor = power_of_two(e);
+            if (chunk == 0) factors[row] = p.scale * power_of_two(-e) * (CAP ? 1.0f : LOG2E);
+            uint32_t h[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) h[c] = half2_of(__uint_as_float(w[c] << 16) * factor, __uint_as_float(w[c] & 0xffff0000u) * factor);
+            *reinterpret_cast<uint4*>(to + ((row / TILE) * GROUPS + chunk / 8) * GROUP_BYTES + (row % TILE) * 128 + (((chunk ^ row) & 7) * 16)) =
+                make_uint4(h[0], h[1], h[2], h[3]);
+        }
+    }
+    fence_async_smem();
+}
+
 // GROUPS: groups of 64 columns that a key and a value take in shared memory.
 // Tensor memory: S of the tiles from columns 0 and 128 on.  With one group O lies from 256 and 320 on, and P, which two 16-bit floats a column
 // make half as wide, from 384 and 448 on, so that S of the next block need not wait for the product with P; with two, O from 256 and
@@ -343,9 +382,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
     constexpr int O_AT = 2 * TILE, O_STEP = 64 * GROUPS, P_AT = P_APART ? 384 : 0, P_STEP = P_APART ? 64 : TILE, P_HALF = P_APART ? 32 : 64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned char* tiles = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
-    constexpr int Q_PLACES = GROUPS == 1 ? 2 : 1;                              // (there is room for the next unit's)
-    unsigned char* q_tile = tiles;                                             // [Q_PLACES][2][GROUPS]
-    unsigned char* k_stage = q_tile + Q_PLACES * 2 * GROUPS * GROUP_BYTES;                // [stages][GROUPS]
+    unsigned char* q_tile = tiles;                                             // [2][GROUPS]
+    unsigned char* k_stage = q_tile + 2 * GROUPS * GROUP_BYTES;                // [stages][GROUPS]
     unsigned char* v_stage = k_stage + stages * GROUPS * GROUP_BYTES;          // [stages][GROUPS]
     if (threadIdx.x == 0) {
         for (int s = 0; s < MAX_STAGES; s++) {
@@ -355,8 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             mbar_init(&sh.v_empty[s], 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.q_full[i], CONVERTER_WARPS);
-            mbar_init(&sh.q_empty[i], 1);
+            mbar_init(&sh.q_full[i], SOFTMAX_WARPS / 2);
             mbar_init(&sh.unit_full[i], 1);
             mbar_init(&sh.unit_empty[i], SOFTMAX_WARPS + CONVERTER_WARPS + 1);
             mbar_init(&sh.s_ready[i], 1);
@@ -392,9 +429,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             if (!ok || !more) break;
             const Blocks blocks(u);
             const int n = tile == 0 ? blocks.n[0] : blocks.n[1];
+            // The tile's queries: the last unit's have been read for the last time (its last S was there), and there is nothing else to do before there are
+            // some.  (The converter warps took 11,000 clocks for them with heads of 128, ahead of a unit's first keys: a prompt of 100 tokens 9.8 us
+            // for 8.1, 500 behind 3,000 67 for 61.  Where units are many and long they had them ready ahead: 16,000 tokens 707 us for 732.)
+            if (n > 0) {
+                put_queries<CAP, GROUPS>(p, u, q_tile, sh.q_factor, warp * (UNIT / SOFTMAX_WARPS), lane);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.q_full[tile]);
+            }
             const bool has_row = row < u.rows;
             const int pos = u.pos0 + (has_row ? row : u.rows - 1);
             const int first = p.window > 0 ? pos - p.window + 1 : 0;
+            const int unseen = p.window > 0 ? u.pos0 + (tile + 1) * TILE - 1 - p.window : -1;      // keys up to here some row of the tile does not see
             float m = -INFINITY, l = 0.0f, q_factor = 0.0f;
             bool sees_none = false;
             for (int j = 0; j < n; j++, seen_blocks++) {
@@ -403,9 +449,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 ok = wait_or_fail(sh, &sh.v_full[s], ring.parity) && wait_or_fail(sh, &sh.s_ready[tile], seen_blocks & 1);
                 ring = ring.next(stages);
                 tcgen05_after_sync();
-                if (j == 0) q_factor = sh.q_factor[k & 1][row];
+                if (j == 0) q_factor = sh.q_factor[row];
                 const uint2 absent = *reinterpret_cast<const uint2*>(&sh.absent[s][2 * half]), none = *reinterpret_cast<const uint2*>(&sh.none[s][2 * half]);
-                const bool needs_mask = key0 + 63 > u.pos0 + tile * TILE || p.window > 0 || (absent.x | absent.y | none.x | none.y) != 0;
+                const bool needs_mask = key0 + 63 > u.pos0 + tile * TILE || key0 <= unseen || (absent.x | absent.y | none.x | none.y) != 0;
                 // which of the columns c .. c + 31 this row sees
                 auto seen = [&](int c) -> uint32_t {
                     const int most = pos - key0 - c, least = first - key0 - c;
@@ -589,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
         }
         if (!ok && lane == 0) give_up(sh, p, 34);
     } else if (warp < MMA_WARP) {
-        // ---- converters: a thread a key (and two queries) ----
+        // ---- converters: a thread a key ----
         const int t = threadIdx.x - SOFTMAX_WARPS * 32;
         bool ok = true;
         for (int k = 0; next_unit(sh, k, u, ok); k++) {
@@ -634,46 +680,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 put(group, v);
             };
             const int id_first = look_up();
-            // The queries, eight or sixteen lanes a row, once the unit that had this place before has read its own for the last time.
-            unsigned char* q_here = q_tile + (k % Q_PLACES) * 2 * GROUPS * GROUP_BYTES;
-            ok = wait_or_fail(sh, &sh.q_empty[k % Q_PLACES], ((k / Q_PLACES) & 1) ^ 1);
-            if (!ok) break;
-            {
-                constexpr int LANES = 8 * GROUPS, ROWS = 32 / LANES, AT_ONCE = 8, OF_WARP = UNIT / CONVERTER_WARPS;
-                const int chunk = lane % LANES, first_row = (warp - SOFTMAX_WARPS) * OF_WARP + lane / LANES;
-                const bf16* from = static_cast<const bf16*>(p.q) + (long)u.row0 * p.ld_q + (long)u.head * p.dim + 8 * chunk;
-#pragma unroll 1
-                for (int base = 0; base < OF_WARP; base += AT_ONCE * ROWS) {
-                    uint4 v[AT_ONCE];
-#pragma unroll
-                    for (int i = 0; i < AT_ONCE; i++) {
-                        const int row = first_row + base + i * ROWS;
-                        v[i] = row < u.rows && 8 * chunk < p.dim ? *reinterpret_cast<const uint4*>(from + row * p.ld_q) : make_uint4(0u, 0u, 0u, 0u);
-                    }
-#pragma unroll
-                    for (int i = 0; i < AT_ONCE; i++) {
-                        const int row = first_row + base + i * ROWS;
-                        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                        float top = 0.0f;
-#pragma unroll
-                        for (int c = 0; c < 4; c++) top = max_of_three(top, fabsf(__uint_as_float(w[c] << 16)), fabsf(__uint_as_float(w[c] & 0xffff0000u)));
-#pragma unroll
-                        for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        // (zeros, and what is not finite, stay as they are)
-                        const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
-                        const float factor = power_of_two(e);
-                        if (chunk == 0) sh.q_factor[k & 1][row] = p.scale * power_of_two(-e) * (CAP ? 1.0f : LOG2E);
-                        uint32_t h[4];
-#pragma unroll
-                        for (int c = 0; c < 4; c++) h[c] = half2_of(__uint_as_float(w[c] << 16) * factor, __uint_as_float(w[c] & 0xffff0000u) * factor);
-                        *reinterpret_cast<uint4*>(q_here + ((row / TILE) * GROUPS + chunk / 8) * GROUP_BYTES + (row % TILE) * 128 + (((chunk ^ row) & 7) * 16)) =
-                            make_uint4(h[0], h[1], h[2], h[3]);
-                    }
-                }
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.q_full[k % Q_PLACES]);
             long at = row_of(id_first);
             go_on();
             float k_scale = 1.0f, v_scale = 1.0f;
@@ -748,9 +754,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             const uint64_t v_desc = make_smem_desc_mn(smem_u32(v_stage), GROUP_BYTES);
             const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0);
             uint32_t seen_blocks[2] = {0, 0}, seen_units[2] = {0, 0};
-            int q_place = 0;
-            auto issue_s = [&](int tile, int s) {
-                const uint64_t a = q_desc + (2 * q_place + tile) * GROUPS * (GROUP_BYTES >> 4), b = k_desc + s * GROUPS * (GROUP_BYTES >> 4);
+                auto issue_s = [&](int tile, int s) {
+                const uint64_t a = q_desc + tile * GROUPS * (GROUP_BYTES >> 4), b = k_desc + s * GROUPS * (GROUP_BYTES >> 4);
 #pragma unroll
                 for (int kk = 0; kk < 4 * GROUPS; kk++) {          // (entries behind `dim` are zeros on both sides)
                     const uint64_t at = (kk / 4) * (GROUP_BYTES >> 4) + 2 * (kk % 4);
@@ -772,14 +777,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 const Blocks of_unit(u);
                 // (the same for all lanes, and the compiler knows it)
                 const int n0 = __shfl_sync(0xffffffffu, of_unit.n[0], 0), n1 = __shfl_sync(0xffffffffu, of_unit.n[1], 0), most = max(n0, n1);
-                q_place = k % Q_PLACES;
-                ok = wait_or_fail(sh, &sh.q_full[q_place], (k / Q_PLACES) & 1);
                 if (most > 0) {
-                    ok = ok && wait_or_fail(sh, &sh.k_full[ring.stage], ring.parity);
+                    ok = wait_or_fail(sh, &sh.k_full[ring.stage], ring.parity);
+#pragma unroll
+                    for (int tile = 0; tile < 2; tile++) {
+                        if ((tile == 0 ? n0 : n1) == 0) continue;
+                        ok = ok && wait_or_fail(sh, &sh.q_full[tile], seen_units[tile] & 1);
+                        if (!ok) break;
+                        tcgen05_after_sync();
+                        issue_s(tile, ring.stage);
+                    }
                     if (!ok) break;
-                    tcgen05_after_sync();
-                    if (n0 > 0) issue_s(0, ring.stage);
-                    if (n1 > 0) issue_s(1, ring.stage);
                     umma_commit_by(elected, &sh.k_empty[ring.stage]);
                 }
                 for (int j = 0; j < most; j++) {
@@ -811,7 +819,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                     ring = after;
                 }
                 if (!ok) break;
-                umma_commit_by(elected, &sh.q_empty[q_place]);
                 seen_blocks[0] += n0, seen_blocks[1] += n1;
                 seen_units[0] += n0 > 0 ? 1 : 0, seen_units[1] += n1 > 0 ? 1 : 0;
             }
@@ -844,7 +851,7 @@ extern "C" int mllm_e4m3_tiles_attention(const E4m3Attention* p, int n_rows, int
     if (p->n_items <= 0 || n_rows <= 0) return 0;
     if (p->dim > 128 || p->vdim > 128) return fail("e4m3_attention_tiles: heads of more than 128 entries");
     const int groups = p->dim <= 64 && p->vdim <= 64 ? 1 : 2, stages = groups == 1 ? 4 : 2;
-    const size_t bytes = 1024 + (size_t)((groups == 1 ? 4 : 2) + 2 * stages) * groups * GROUP_BYTES;
+    const size_t bytes = 1024 + (size_t)(2 + 2 * stages) * groups * GROUP_BYTES;
     const int which = (p->cap > 0.0f ? 2 : 0) + groups - 1;
     static size_t raised[4][64];
     auto kernel = which == 0 ? attention_tiles_kernel<false, 1> : which == 1 ? attention_tiles_kernel<false, 2>

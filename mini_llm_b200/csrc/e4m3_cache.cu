@@ -400,11 +400,6 @@ __device__ __forceinline__ uint32_t turned_tile(uint32_t x) {
     return r;
 }
 
-// a / b of numbers that are not negative (the 64-bit division costs some hundred clocks, and a row is hardly ever that long).
-__device__ __forceinline__ long divided(long a, long b) {
-    return ((a | b) >> 31) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
-}
-
 // All units in a row; every warp works out the same, all its lanes together.
 struct StepSchedule {
     const E4m3Attention& p;
