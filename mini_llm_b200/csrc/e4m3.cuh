@@ -77,6 +77,23 @@ static cudaError_t raise_shared_limit(Kernel kernel, size_t bytes, size_t (&rais
     return e;
 }
 
+// What storing gets.
+struct E4m3Store {
+    void* q_out;                   // [n, heads * dim] or null: the queries stay as they are
+    long ld_q;
+    const void* qkv;
+    long ld;
+    int k_off, v_off, heads, kv_heads, dim, vdim, rot_dims;
+    const double* inv_freq;
+    float amplitude;
+    const int *positions, *token_item, *block_table;
+    int max_blocks, n_pages, page;
+    uint8_t *k_pages, *v_pages;    // null: nothing is stored
+    float *k_scales, *v_scales;
+    int n;
+};
+static_assert(sizeof(E4m3Store) == 160, "packed by the caller field by field, with C's alignment");
+
 // What attention over the cache gets.  An entry is a request's tokens of this step: rows item_offset .. + item_count of q, at
 // positions item_start, item_start + 1, ...; entries without tokens are allowed.
 struct E4m3Attention {
@@ -97,3 +114,4 @@ struct E4m3Attention {
     int* counters;
     int* status;                   // where a bounded wait that ran out leaves its code
 };
+static_assert(sizeof(E4m3Attention) == 168, "packed by the caller field by field, with C's alignment");

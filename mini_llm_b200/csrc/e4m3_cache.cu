@@ -22,21 +22,6 @@ namespace {
 // a step that is run again leaves the same bytes.  A CTA takes G rows and the blocks that begin in them, and a share of the heads; its
 // table of cosines and sines serves all of them.  What bounds it is bytes, rows once in, codes and queries once out, for long
 // portions (8,192 rows of 6,144 columns: 54 us, 3.4 TB/s), and the chain of positions, page and rows for single tokens (2.9 us).
-struct StoreParams {
-    void* q_out;                   // [n, heads * dim] or null: the queries stay as they are
-    long ld_q;
-    const void* qkv;
-    long ld;
-    int k_off, v_off, heads, kv_heads, dim, vdim, rot_dims;
-    const double* inv_freq;
-    float amplitude;
-    const int *positions, *token_item, *block_table;
-    int max_blocks, n_pages, page;
-    uint8_t *k_pages, *v_pages;    // null: nothing is stored
-    float *k_scales, *v_scales;
-    int n;
-};
-
 constexpr int STORE_THREADS = 256, STORE_ROWS = 16;
 
 // Eight numbers of a row, as they lie in memory.
@@ -137,7 +122,7 @@ __device__ __forceinline__ int scale_exponent(float square) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(STORE_THREADS) store_kernel(const StoreParams p, int G) {
+__global__ void __launch_bounds__(STORE_THREADS) store_kernel(const E4m3Store p, int G) {
     __shared__ int row_pos[STORE_ROWS + 16], row_item[STORE_ROWS + 16];        // of rows first - 1, first, ...
     __shared__ int row_page[STORE_ROWS];                                       // a leading row's page, -1: it has no place
     extern __shared__ __align__(16) float2 angles[];                           // [rows, rot_dims / 2]
@@ -891,14 +876,11 @@ int launch_step_of(const E4m3Attention& p, int n_sms, cudaStream_t stream) {
 
 }  // namespace
 
-extern "C" int mllm_e4m3_store(void* q_out, long ld_q, const void* qkv, long ld, int k_off, int v_off, int heads, int kv_heads, int dim,
-                               int vdim, int rot_dims, const double* inv_freq, double amplitude, const int* positions,
-                               const int* token_item, const int* block_table, int max_blocks, int n_pages, int page, void* k_pages,
-                               void* v_pages, float* k_scales, float* v_scales, int n, int dtype, int n_sms, void* stream) {
+extern "C" int mllm_e4m3_store(const E4m3Store* operands, int dtype, int n_sms, void* stream) {
+    const E4m3Store& p = *operands;
+    const int n = p.n, rot_dims = p.rot_dims;
     if (n <= 0) return 0;
-    StoreParams p = {q_out, ld_q, qkv, ld, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, (float)amplitude, positions,
-                     token_item, block_table, max_blocks, n_pages, page, (uint8_t*)k_pages, (uint8_t*)v_pages, k_scales, v_scales, n};
-    const int slots = (q_out != nullptr ? heads : 0) + (k_pages != nullptr ? 2 * kv_heads : 0);
+    const int slots = (p.q_out != nullptr ? p.heads : 0) + (p.k_pages != nullptr ? 2 * p.kv_heads : 0);
     if (slots == 0) return 0;
     // Rows a CTA, and the heads shared among as many CTAs as fill the SMs.  Single tokens, of which each begins a block, want few rows a CTA,
     // long portions many, whose angles are then made once (rows a CTA 4, 8, 16: a portion of 1,500 with shorter ones and 40 single tokens

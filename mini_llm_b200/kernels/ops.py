@@ -9,6 +9,7 @@ take every size; a fast kernel either takes a size or is not chosen for it.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -1898,21 +1899,22 @@ E4M3_BLOCK = 16
 E4M3_NONE = 0x7f               # the code that is no number
 E4M3_LEAST_CAP = 2.0 ** -100   # (its inverse is a 32-bit number)
 E4M3_MOST_CAP = 8192.0         # (a capped score is off by 2^-22 of the cap: here 2^-9, half of what a bfloat16 result is rounded by)
+E4M3_MOST_SCALE = 2.0 ** 127   # of scores, and the most amplitude: numbers that 32 bits hold
 E4M3_FAST_SIZES = 128          # entries of a key or value up to which the kernels on tensor cores take them
 
 
-class _E4m3Attention(ctypes.Structure):
-    _fields_ = [("out", P), ("ld_out", L), ("q", P), ("ld_q", L), ("k_pages", P), ("v_pages", P), ("k_scales", P), ("v_scales", P),
-                ("block_table", P), ("max_blocks", I), ("n_pages", I), ("page", I), ("item_offset", P), ("item_count", P),
-                ("item_start", P), ("n_items", I), ("n_heads", I), ("n_kv_heads", I), ("dim", I), ("vdim", I), ("scale", F), ("cap", F),
-                ("window", I), ("partial", P), ("counters", P), ("status", P)]
+# struct E4m3Attention: out, ld_out, q, ld_q, k_pages, v_pages, k_scales, v_scales, block_table; max_blocks, n_pages, page; item_offset, item_count,
+# item_start; n_items, n_heads, n_kv_heads, dim, vdim; scale, cap; window; partial, counters, status
+# struct E4m3Store: q_out, ld_q, qkv, ld; k_off, v_off, heads, kv_heads, dim, vdim, rot_dims; inv_freq, amplitude; positions, token_item, block_table;
+# max_blocks, n_pages, page; k_pages, v_pages, k_scales, v_scales; n
+_e4m3_rows = struct.Struct("@PlPl7iPf3P3i4Pi0P").pack
+_e4m3_operands = struct.Struct("@PlPlPPPPP3iPPP5i2fiPPP").pack
 
+_e4m3_store = Function("e4m3", "mllm_e4m3_store", [ctypes.c_char_p, I, I, P])
+_e4m3_plain = Function("e4m3", "mllm_e4m3_attention_plain", [ctypes.c_char_p, I, I, P])
+_e4m3_step = Function("e4m3", "mllm_e4m3_attention_step", [ctypes.c_char_p, I, P])
 
-_e4m3_store = Function("e4m3", "mllm_e4m3_store", [P, L, P, L, I, I, I, I, I, I, I, P, ctypes.c_double, P, P, P, I, I, I, P, P, P, P, I, I, I, P])
-_e4m3_plain = Function("e4m3", "mllm_e4m3_attention_plain", [ctypes.POINTER(_E4m3Attention), I, I, P])
-_e4m3_step = Function("e4m3", "mllm_e4m3_attention_step", [ctypes.POINTER(_E4m3Attention), I, P])
-
-_e4m3_tiles = Function("e4m3_tiles", "mllm_e4m3_tiles_attention", [ctypes.POINTER(_E4m3Attention), I, I, P])
+_e4m3_tiles = Function("e4m3_tiles", "mllm_e4m3_tiles_attention", [ctypes.c_char_p, I, I, P])
 
 _sm_counts = {}
 
@@ -1933,8 +1935,8 @@ def e4m3_fast_takes(dtype, dim, vdim) -> bool:
     return dtype == torch.bfloat16 and max(dim, vdim) <= E4M3_FAST_SIZES
 
 
-# (These calls may be all that stands between two short kernels: a tensor is looked at once, in few words, and only a wrong one again, for the
-# error's text.)
+# (These calls may be all that stands between two short kernels: all that they ask of their operands is asked in one expression, and only where
+# something does not hold again, one by one, for the error's text.)
 
 def _is(t, dtype, dims, index) -> bool:
     return isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == dims
@@ -1990,31 +1992,34 @@ def _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, in
     return n_pages, kv_heads, page, dim, vdim
 
 
-def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, positions, token_item,
-               block_table, k_pages, v_pages, k_scales, v_scales, writes=True):
-    """Append a step's keys and values to a cache in 8 bits, with the rotation of queries and keys on the way.
+_NO_PAGES = (0, 0, 0, 0)
 
-    Rows of ``qkv`` (fp32 or bf16 [T, columns]) hold [q | k | v], k from column ``k_off``, v from ``v_off``.  The first ``rot_dims``
-    entries of every query and key head turn in interleaved pairs by position * ``inv_freq`` [rot_dims / 2] (float64; None without
-    turned entries), cosine and sine times ``amplitude``.  The turned queries go to ``q_out`` [T, heads * dim] (None: they are
-    not wanted), which may be the queries' own columns of ``qkv``, and no other part of it; all else of ``qkv`` stays as it is.
-    ``writes=False``: queries only.
 
-    Row t goes to position ``positions[t]`` of the request in row ``token_item[t]`` of the block table, which has that row.  A request's
-    rows stand side by side at positions that grow by one (rows of one request that repeat a position, as rows that fill a step up do, may
-    leave anything in the blocks that they name, and nothing elsewhere); no two requests of a step store into one page; a row at a negative position, or whose page the table does not name (an index
-    outside the pages, a column outside the table), is stored nowhere.  The scale of a block of 16 positions is the least power of two
-    s >= 2^-64 with n <= (448 s)^2 for all its rows so far, n being x^2 + y^2 of a pair that turns (times ``amplitude``^2; a turn
-    keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
-    row that begins a block begins it anew, whatever was there.  A key or value head with an n that is not finite is stored as
-    NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes."""
+_INT32, _FP32, _FP64, _BF16, _E4M3 = torch.int32, torch.float32, torch.float64, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _are_pages(k_pages, v_pages, k_scales, v_scales, block_table, index, scales) -> bool:
+    """``_check_e4m3_pages``, but for the pages' shapes and alignment, in one expression."""
+    return (k_pages.dtype is _E4M3 and v_pages.dtype is _E4M3 and k_scales.dtype is _FP32 and v_scales.dtype is _FP32
+            and block_table.dtype is _INT32 and k_scales.shape == scales and v_scales.shape == scales
+            and k_pages.get_device() == index and v_pages.get_device() == index and k_scales.get_device() == index
+            and v_scales.get_device() == index and block_table.get_device() == index and k_pages.is_contiguous() and v_pages.is_contiguous()
+            and k_scales.is_contiguous() and v_scales.is_contiguous() and block_table.is_contiguous())
+
+
+def _check_e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, positions, token_item, block_table,
+                      k_pages, v_pages, k_scales, v_scales, writes):
+    """Raises what is wrong with the operands of ``e4m3_store``."""
     who = "e4m3_store"
     _check(qkv, f"{who}.qkv", None, 2)
-    index, (n, columns), dtype = qkv.get_device(), qkv.shape, dtype_code(qkv.dtype)
+    index, (n, columns) = qkv.get_device(), qkv.shape
+    dtype_code(qkv.dtype)
     if min(heads, kv_heads) <= 0 or dim % 16 or vdim % 16 or not 0 < dim <= 256 or not 0 < vdim <= 256:
         raise KernelError(f"{who} does not take heads of {dim} and {vdim} entries (multiples of 16 up to 256)")
     if rot_dims < 0 or rot_dims % 2 or rot_dims > dim:
         raise KernelError(f"{who}: {rot_dims} turned entries do not fit a head of {dim}")
+    if not -E4M3_MOST_SCALE <= amplitude <= E4M3_MOST_SCALE:
+        raise KernelError(f"{who}: an amplitude of {amplitude} is not finite in 32 bits")
     if min(k_off, v_off) < 0 or max(heads * dim, k_off + kv_heads * dim, v_off + kv_heads * vdim) > columns or k_off % 8 or v_off % 8:
         raise KernelError(f"{who}: the columns do not hold queries, keys and values, or are not multiples of 8")
     for name, t, kind in (("inv_freq", inv_freq, torch.float64), ("positions", positions, torch.int32), ("token_item", token_item, torch.int32)):
@@ -2031,18 +2036,70 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
             raise KernelError(f"{who}: q_out does not have heads * dim columns")
     if n and not (_rows_fit(qkv) and (q_out is None or _rows_fit(q_out))):
         raise KernelError(f"{who}: rows of qkv and q_out must begin on 16-byte boundaries, their entries side by side")
-    n_pages = page = max_blocks = 0
-    pages = (None, None, None, None)
     if writes:
-        n_pages, held_heads, page, held_dim, held_vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, index)
+        _, held_heads, _, held_dim, held_vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, index)
         if (held_heads, held_dim, held_vdim) != (kv_heads, dim, vdim):
             raise KernelError(f"{who}: the pages hold heads of another number or size")
-        max_blocks = block_table.shape[1]
-        pages = (k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
-    _launch_on(index, _e4m3_store, _ptr(q_out), q_out.stride(0) if q_out is not None else 0, qkv.data_ptr(), qkv.stride(0), k_off, v_off, heads,
-               kv_heads, dim, vdim, rot_dims, inv_freq.data_ptr() if rot_dims else None, float(amplitude), positions.data_ptr(),
-               token_item.data_ptr(), block_table.data_ptr() if writes else None, max_blocks, n_pages, page, *pages, n, dtype,
-               _sm_count(index), _on_device(index))
+
+
+def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, positions, token_item,
+               block_table, k_pages, v_pages, k_scales, v_scales, writes=True):
+    """Append a step's keys and values to a cache in 8 bits, with the rotation of queries and keys on the way.
+
+    Rows of ``qkv`` (fp32 or bf16 [T, columns]) hold [q | k | v], k from column ``k_off``, v from ``v_off``.  The first ``rot_dims``
+    entries of every query and key head turn in interleaved pairs by position * ``inv_freq`` [rot_dims / 2] (float64; None without
+    turned entries), cosine and sine times ``amplitude``.  The turned queries go to ``q_out`` [T, heads * dim] (None: they are
+    not wanted), which may be the queries' own columns of ``qkv``, and no other part of it; all else of ``qkv`` stays as it is.
+    ``writes=False``: queries only.
+
+    Row t goes to position ``positions[t]`` of the request in row ``token_item[t]`` of the block table, which has that row.  A request's
+    rows stand side by side at positions that grow by one (rows of one request that repeat a position, as rows that fill a step up do, may
+    leave anything in the blocks that they name, and nothing elsewhere); no two requests of a step store into one page; a row at a negative
+    position, or whose page the table does not name (an index outside the pages, a column outside the table), is stored nowhere.  The scale of a block of 16
+    positions is the least power of two s >= 2^-64 with n <= (448 s)^2 for all its rows so far, n being x^2 + y^2 of a pair that turns (times ``amplitude``^2; a turn
+    keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
+    row that begins a block begins it anew, whatever was there.  A key or value head with an n that is not finite is stored as
+    NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes."""
+    n_pages = page = max_blocks = ld_q = 0
+    q_at = freq_at = table_at = 0
+    pages = _NO_PAGES
+    try:
+        index, dtype, (n, columns), (ld, step), at = qkv.get_device(), qkv.dtype, qkv.shape, qkv.stride(), qkv.data_ptr()
+        (n_positions,), (n_places,), bits = positions.shape, token_item.shape, 2 if dtype is _FP32 else 1
+        fits = (index >= 0 and (bits == 2 or dtype is _BF16) and step == 1 and not (at | (ld << bits)) & 15
+                and heads > 0 and kv_heads > 0 and 0 < dim <= 256 and 0 < vdim <= 256 and not (dim | vdim) & 15
+                and 0 <= rot_dims <= dim and not rot_dims & 1 and -E4M3_MOST_SCALE <= amplitude <= E4M3_MOST_SCALE
+                and k_off >= 0 and v_off >= 0 and not (k_off | v_off) & 7
+                and heads * dim <= columns and k_off + kv_heads * dim <= columns and v_off + kv_heads * vdim <= columns
+                and n_positions >= n and n_places >= n and positions.dtype is _INT32 and token_item.dtype is _INT32
+                and positions.get_device() == index and token_item.get_device() == index and positions.is_contiguous() and token_item.is_contiguous())
+        if rot_dims:
+            freq_at, (n_frequencies,) = inv_freq.data_ptr(), inv_freq.shape
+            fits = (fits and 2 * n_frequencies >= rot_dims and inv_freq.dtype is _FP64 and inv_freq.get_device() == index
+                    and inv_freq.is_contiguous())
+        if q_out is not None:
+            q_at, (ld_q, step) = q_out.data_ptr(), q_out.stride()
+            fits = (fits and q_out.dtype is dtype and q_out.get_device() == index and q_out.shape == (n, heads * dim) and step == 1
+                    and not (q_at | (ld_q << bits)) & 15)
+        if writes:
+            n_pages, held_heads, page, held_dim = k_pages.shape
+            _, max_blocks = block_table.shape
+            table_at = block_table.data_ptr()
+            pages = k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr()
+            fits = (fits and held_heads == kv_heads and held_dim == dim and v_pages.shape == (n_pages, kv_heads, page, vdim) and page > 0
+                    and not (page | pages[0] | pages[1]) & 15
+                    and _are_pages(k_pages, v_pages, k_scales, v_scales, block_table, index, (n_pages, kv_heads, page >> 4)))
+        known = True
+    except (AttributeError, TypeError, ValueError):
+        fits = known = False
+    if not fits:
+        _check_e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, positions, token_item, block_table,
+                          k_pages, v_pages, k_scales, v_scales, writes)
+        if not known:
+            raise KernelError("e4m3_store: operands of other kinds than it takes")
+    params = _e4m3_rows(q_at, ld_q, at, ld, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, freq_at, amplitude, positions.data_ptr(),
+                        token_item.data_ptr(), table_at, max_blocks, n_pages, page, *pages, n)
+    _launch_on(index, _e4m3_store, params, dtype_code(dtype), _sm_count(index), _on_device(index))
     return q_out
 
 
@@ -2076,22 +2133,14 @@ def e4m3_workspace(device, vdim: int, status=None) -> E4m3Workspace:
     return E4m3Workspace(device, vdim, status)
 
 
-def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start, heads, kv_heads, scale,
-                   cap=0.0, window=0, longest=None, singles=True, workspace=None, plain=False):
-    """Causal attention over a cache in 8 bits.  Entry i of the step: rows ``item_offset[i]`` .. + ``item_count[i]`` of ``q`` (fp32 or bf16
-    [T, heads * dim]) and ``out`` [T, heads * vdim], at positions ``item_start[i]``, ... of the request in row i of the block table, whose
-    keys and values are stored up to there; entries have rows of their own within ``q``, and rows of no entry stay as they are.  A stored
-    head is NaN throughout or nowhere and a scale a power of two from 2^-64 on, as ``e4m3_store`` leaves them.  score = q . k * ``scale``, with ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if
-    given; softmax and the weighted sum in 32 bits; query head h reads key/value head h // (heads / kv_heads).  A row that sees no key (a
-    negative position) is zero; pages that the table does not name are not seen.
-
-    ``longest=1``: the caller knows that no entry brings more than one token (one that does is left out: its rows stay as they are);
-    ``singles=False``: that none brings just one (likewise).  Other values of ``longest`` change nothing.  ``workspace`` (``e4m3_workspace``) is needed but with ``plain``: the kernel of every size and type, which 32-bit
-    queries, and heads of more than 128 entries, take anyway."""
+def _check_e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start, heads, kv_heads, scale, cap,
+                          window):
+    """Raises what is wrong with the operands of ``e4m3_attention``."""
     who = "e4m3_attention"
     _check(q, f"{who}.q", None, 2)
-    index, (n_rows, columns), dtype = q.get_device(), q.shape, dtype_code(q.dtype)
-    n_pages, held_heads, page, dim, vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, index)
+    index, (n_rows, columns) = q.get_device(), q.shape
+    dtype_code(q.dtype)
+    _, held_heads, _, dim, vdim = _check_e4m3_pages(who, k_pages, v_pages, k_scales, v_scales, block_table, index)
     if not _is(out, q.dtype, 2, index):
         _refuse(out, f"{who}.out", q.dtype, 2, index)
     if kv_heads != held_heads or heads <= 0 or heads % kv_heads:
@@ -2100,30 +2149,66 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
         raise KernelError(f"{who}: q / out do not have heads * size columns")
     if n_rows and not (_rows_fit(q) and _rows_fit(out)):
         raise KernelError(f"{who}: rows of q and out must begin on 16-byte boundaries, their entries side by side")
-    n_items, max_blocks = block_table.shape
+    n_items = block_table.shape[0]
     for name, t in (("item_offset", item_offset), ("item_count", item_count), ("item_start", item_start)):
         if not _is(t, torch.int32, 1, index):
             _refuse(t, f"{who}.{name}", torch.int32, 1, index)
         if t.shape[0] != n_items or (n_items > 1 and t.stride(0) != 1):
             raise KernelError(f"{who}: {name} does not hold a number for each of the block table's {n_items} rows, side by side")
-    if not (window >= 0 and (cap == 0 or E4M3_LEAST_CAP <= cap <= E4M3_MOST_CAP) and 0 <= scale < float("inf")):
+    if not (0 <= window < 2 ** 31 and (cap == 0 or E4M3_LEAST_CAP <= cap <= E4M3_MOST_CAP) and 0 <= scale <= E4M3_MOST_SCALE):
         raise KernelError(f"{who}: a window is positive and a cap between {E4M3_LEAST_CAP} and {E4M3_MOST_CAP}, or 0 for none, and a scale is "
                           "finite and not negative")
-    fast = not plain and e4m3_fast_takes(q.dtype, dim, vdim)
-    pointers = (None, None, None)
+
+
+def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start, heads, kv_heads, scale,
+                   cap=0.0, window=0, longest=None, singles=True, workspace=None, plain=False):
+    """Causal attention over a cache in 8 bits.  Entry i of the step: rows ``item_offset[i]`` .. + ``item_count[i]`` of ``q`` (fp32 or bf16
+    [T, heads * dim]) and ``out`` [T, heads * vdim], at positions ``item_start[i]``, ... of the request in row i of the block table, whose
+    keys and values are stored up to there; entries have rows of their own within ``q``, and rows of no entry stay as they are.  A stored
+    head is NaN throughout or nowhere and a scale a power of two from 2^-64 on, as ``e4m3_store`` leaves them.  score = q . k * ``scale``, with
+    ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if given; softmax and the weighted sum
+    in 32 bits; query head h reads key/value head h // (heads / kv_heads).  A row that sees no key (a negative position) is zero; pages that the table does not name are not seen.
+
+    ``longest=1``: the caller knows that no entry brings more than one token (one that does is left out: its rows stay as they are);
+    ``singles=False``: that none brings just one (likewise).  Other values of ``longest`` change nothing.  ``workspace``
+    (``e4m3_workspace``) is needed but with ``plain``: the kernel of every size and type, which 32-bit queries, and heads of more than 128
+    entries, take anyway."""
+    try:
+        index, dtype, (n_rows, columns), (ld_q, q_step), q_at = q.get_device(), q.dtype, q.shape, q.stride(), q.data_ptr()
+        n_pages, held_heads, page, dim = k_pages.shape
+        (n_items, max_blocks), vdim, (ld_out, out_step), out_at = block_table.shape, v_pages.shape[-1], out.stride(), out.data_ptr()
+        k_at, v_at, bits, items = k_pages.data_ptr(), v_pages.data_ptr(), 2 if dtype is _FP32 else 1, (n_items,)
+        fits = (index >= 0 and (bits == 2 or dtype is _BF16) and out.dtype is dtype and out.get_device() == index
+                and kv_heads == held_heads and heads > 0 and not heads % kv_heads and columns == heads * dim and out.shape == (n_rows, heads * vdim)
+                and q_step == 1 and out_step == 1 and not (q_at | out_at | (ld_q << bits) | (ld_out << bits) | k_at | v_at | dim | vdim | page) & 15
+                and 0 < dim <= 256 and 0 < vdim <= 256 and page > 0 and v_pages.shape == (n_pages, held_heads, page, vdim)
+                and _are_pages(k_pages, v_pages, k_scales, v_scales, block_table, index, (n_pages, held_heads, page >> 4))
+                and item_offset.shape == items and item_count.shape == items and item_start.shape == items
+                and item_offset.dtype is _INT32 and item_count.dtype is _INT32 and item_start.dtype is _INT32
+                and item_offset.get_device() == index and item_count.get_device() == index and item_start.get_device() == index
+                and item_offset.is_contiguous() and item_count.is_contiguous() and item_start.is_contiguous()
+                and 0 <= window < 2 ** 31 and (cap == 0 or E4M3_LEAST_CAP <= cap <= E4M3_MOST_CAP) and 0 <= scale <= E4M3_MOST_SCALE)
+        known = True
+    except (AttributeError, TypeError, ValueError, IndexError):
+        fits = known = False
+    if not fits:
+        _check_e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start, heads, kv_heads, scale,
+                              cap, window)
+        if not known:
+            raise KernelError("e4m3_attention: operands of other kinds than it takes")
+    fast = not plain and dtype is _BF16 and dim <= E4M3_FAST_SIZES and vdim <= E4M3_FAST_SIZES
     if fast:
         if workspace is None:
-            raise KernelError(f"{who}: a workspace is needed (e4m3_workspace)")
+            raise KernelError("e4m3_attention: a workspace is needed (e4m3_workspace)")
         if workspace.index != index or _padded_64(vdim) > _padded_64(workspace.vdim):
-            raise KernelError(f"{who}: the workspace is for values of {workspace.vdim} entries on device {workspace.index}, not {vdim} on {index}")
-        pointers = workspace.pointers
-    params = ctypes.byref(_E4m3Attention(
-        out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-        block_table.data_ptr(), max_blocks, n_pages, page, item_offset.data_ptr(), item_count.data_ptr(), item_start.data_ptr(), n_items,
-        heads, kv_heads, dim, vdim, scale, cap or 0.0, window or 0, *pointers))
+            raise KernelError(f"e4m3_attention: the workspace is for values of {workspace.vdim} entries on device {workspace.index}, not {vdim} on {index}")
+    params = _e4m3_operands(
+        out_at, ld_out, q_at, ld_q, k_at, v_at, k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), max_blocks, n_pages, page,
+        item_offset.data_ptr(), item_count.data_ptr(), item_start.data_ptr(), n_items, heads, kv_heads, dim, vdim, scale, cap, window,
+        *(workspace.pointers if fast else (0, 0, 0)))
     stream = _on_device(index)
     if not fast:
-        _launch_on(index, _e4m3_plain, params, n_rows, dtype, stream)
+        _launch_on(index, _e4m3_plain, params, n_rows, dtype_code(dtype), stream)
         return out
     n_sms = _sm_count(index)
     if longest != 1:

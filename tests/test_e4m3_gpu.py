@@ -605,7 +605,8 @@ def test_refusals():
                          (dict(item_count=ints([1, 1])), "item_count"), (dict(item_start=ints([0]).long()), "int32"), (dict(heads=5), "heads over"),
                          (dict(kv_heads=4), "heads over"), (dict(window=-1), "window"), (dict(cap=-1.0), "cap"), (dict(scale=-0.1), "scale"),
                          (dict(cap=float("inf")), "cap"), (dict(cap=1e-40), "cap"), (dict(cap=float("nan")), "cap"), (dict(cap=8193.0), "cap"),
-                         (dict(scale=float("inf")), "scale"),
+                         (dict(scale=float("inf")), "scale"), (dict(scale=1e39), "scale"), (dict(window=2 ** 31), "window"), (dict(item_count=[1]), "item_count"),
+                         (dict(q=q[0]), "dimensions"), (dict(v_pages=vp[0]), "v_pages"),
                          (dict(scale=float("nan")), "scale"), (dict(workspace=None), "workspace"), (dict(q=wide[:, :256]), "16-byte"),
                          (dict(out=wide[:, 2:258]), "16-byte")):
         with pytest.raises(KernelError, match=text):
@@ -620,6 +621,7 @@ def test_refusals():
                 block_table=table, k_pages=kp, v_pages=vp, k_scales=ks, v_scales=vs)
     ops.e4m3_store(**good)
     for change, text in ((dict(qkv=qkv.cpu()), "CUDA tensor"), (dict(qkv=qkv.half()), "element type"), (dict(dim=60), "multiples of 16"), (dict(vdim=512), "multiples of 16"),
+                         (dict(amplitude=1e39), "amplitude"), (dict(amplitude=float("nan")), "amplitude"), (dict(positions=[0, 1, 2, 3]), "positions"),
                          (dict(rot_dims=63), "turned"), (dict(rot_dims=80), "turned"), (dict(v_off=400), "columns"), (dict(k_off=252), "multiples of 8"),
                          (dict(inv_freq=torch.ones(31, dtype=torch.float64, device="cuda")), "frequencies"), (dict(inv_freq=None), "expected a CUDA"),
                          (dict(inv_freq=torch.ones(32, device="cuda")), "float64"), (dict(positions=ints([0, 1])), "fewer positions"),
