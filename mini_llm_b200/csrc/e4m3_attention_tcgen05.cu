@@ -308,6 +308,58 @@ __device__ __forceinline__ void add_pair(float& x, float& y, float a, float b) {
         : "f"(a), "f"(b));
 }
 
+__device__ __forceinline__ void mul_pair(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma_pairs(float& x, float& y, float a, float b, float from) {
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %4};\n\t"
+        "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b), "f"(from));
+}
+
+// A factor of scores is never zero, which no hidden score's minus infinity would outlast: queries or a scale that small make scores of nothing either way.
+__device__ __forceinline__ float never_zero(float factor) { return fmaxf(factor, 0x1p-126f); }
+
+// 32 products (two blocks of 16 keys) to capped scores.  Up to a quarter of the cap, where scores mostly lie, by the series of tanh u / u in u^2 to its
+// third power (the next term is 2^-23.5 of the cap there): otherwise the exponential's unit, which the weights need, has two more operations a score (a
+// portion of 1,024 behind 1,345 and two short prompts, 12 heads of 64: 48.0 us, and 41.3).
+__device__ __forceinline__ void cap_scores(uint32_t (&v)[32], float q_factor, const float* k_scale, float cap_log2, float cap_factor, float by_cap) {
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        float x = __uint_as_float(v[i]), y = __uint_as_float(v[i + 1]);
+        const float factor = never_zero(q_factor * k_scale[i / 16]);
+        mul_pair(x, y, factor, factor);
+        far = max_of_three(far, fabsf(x), fabsf(y));
+        v[i] = __float_as_uint(x), v[i + 1] = __float_as_uint(y);
+    }
+    if (__builtin_expect(__any_sync(0xffffffffu, far > 0.25f * cap_log2), 0)) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            // (what is hidden stays hidden: its score is minus infinity, not minus the cap)
+            const float x = __uint_as_float(v[i]);
+            v[i] = __float_as_uint(x == -INFINITY ? x : capped(x, cap_log2, cap_factor));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float x = __uint_as_float(v[i]), y = __uint_as_float(v[i + 1]);
+        float a = x, b = y;
+        mul_pair(a, b, by_cap, by_cap);
+        mul_pair(a, b, a, b);
+        float p = a, q = b;
+        fma_pair(p, q, -17.0f / 315.0f, 2.0f / 15.0f);
+        fma_pairs(p, q, a, b, -1.0f / 3.0f);
+        fma_pairs(p, q, a, b, 1.0f);
+        mul_pair(p, q, x, y);
+        v[i] = __float_as_uint(p), v[i + 1] = __float_as_uint(q);
+    }
+}
+
 // The 256 threads of a tile meet; whether any of them says yes.  (Where a wait ran out for some of them only, they leave together all the same,
 // from a meeting in which one said so: one that left alone would keep the others waiting here for good.)
 __device__ __forceinline__ bool any_of_tile(int tile, bool yes) {
@@ -333,7 +385,7 @@ __device__ __forceinline__ void store_sixteen(bf16* to, const float (&o)[16], fl
 
 // 16 rows of a unit's queries into shared memory, by a warp, eight or sixteen lanes a row: as 16-bit floats of a power of two's size, and what
 // brings a row's scores into powers of two.
-template <bool CAP, int GROUPS>
+template <int GROUPS>
 __device__ __forceinline__ void put_queries(const E4m3Attention& p, const Unit& u, unsigned char* to, float* factors, int first_row, int lane) {
     constexpr int LANES = 8 * GROUPS, ROWS = 32 / LANES, AT_ONCE = 4, OF_WARP = UNIT / SOFTMAX_WARPS;
     const int chunk = lane % LANES, row0 = first_row + lane / LANES;
@@ -358,7 +410,7 @@ __device__ __forceinline__ void put_queries(const E4m3Attention& p, const Unit& 
             // (zeros, and what is not finite, stay as they are)
             const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
             const float factor = power_of_two(e);
-            if (chunk == 0) factors[row] = p.scale * power_of_two(-e) * (CAP ? 1.0f : LOG2E);
+            if (chunk == 0) factors[row] = p.scale * power_of_two(-e) * LOG2E;
             uint32_t h[4];
 #pragma unroll
             for (int c = 0; c < 4; c++) h[c] = half2_of(__uint_as_float(w[c] << 16) * factor, __uint_as_float(w[c] & 0xffff0000u) * factor);
@@ -420,7 +472,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
         const int tile = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, row = tile * TILE + r;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_at = lanes + TILE * tile + 64 * half, o_at = lanes + O_AT + O_STEP * tile, p_at = lanes + P_AT + P_STEP * tile + P_HALF * half;
-        const float cap_factor = CAP ? 2.0f * LOG2E / p.cap : 0.0f, cap_log2 = p.cap * LOG2E;
+        // (scores are in powers of two from the first on, and so is the cap)
+        const float cap_log2 = p.cap * LOG2E, cap_factor = CAP ? 2.0f / p.cap : 0.0f, by_cap = CAP ? 1.0f / cap_log2 : 0.0f;
         uint32_t seen_blocks = 0;                    // of this tile, over all units
         bool ok = true;
         for (int k = 0;; k++) {
@@ -433,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             // some.  (The converter warps took 11,000 clocks for them with heads of 128, ahead of a unit's first keys: a prompt of 100 tokens 9.8 us
             // for 8.1, 500 behind 3,000 67 for 61.  Where units are many and long they had them ready ahead: 16,000 tokens 707 us for 732.)
             if (n > 0) {
-                put_queries<CAP, GROUPS>(p, u, q_tile, sh.q_factor, warp * (UNIT / SOFTMAX_WARPS), lane);
+                put_queries<GROUPS>(p, u, q_tile, sh.q_factor, warp * (UNIT / SOFTMAX_WARPS), lane);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.q_full[tile]);
             }
@@ -533,23 +586,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                         if (lane == 0) mbar_arrive(&sh.s_read[tile]);
                     }
                     uint32_t packed[16];
+                    if (CAP) cap_scores(v, q_factor, &sh.k_scale[s][4 * half + c / 16], cap_log2, cap_factor, by_cap);
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
                         const int group = 4 * half + c / 16 + g;
-                        // (never zero, which no hidden score's minus infinity would outlast: queries or a scale that small make scores of
-                        // nothing either way)
-                        const float from = sh.v_exponent[s][group] - base, factor = fmaxf(q_factor * sh.k_scale[s][group], 0x1p-126f);
+                        const float from = sh.v_exponent[s][group] - base, factor = CAP ? 1.0f : never_zero(q_factor * sh.k_scale[s][group]);
                         float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
                             float x = __uint_as_float(v[16 * g + i]), y = __uint_as_float(v[16 * g + i + 1]);
-                            if (CAP) {
-                                // (what is hidden stays hidden: its score is minus infinity, not minus the cap)
-                                const float a = capped(x * factor, cap_log2, cap_factor) + from, b = capped(y * factor, cap_log2, cap_factor) + from;
-                                x = x == -INFINITY ? x : a, y = y == -INFINITY ? y : b;
-                            } else {
-                                fma_pair(x, y, factor, from);
-                            }
+                            if (CAP) add_pair(x, y, from, from);
+                            else fma_pair(x, y, factor, from);
                             x = exp2_fast(x), y = exp2_fast(y);
                             add_pair(sum[(i >> 1) & 1][0], sum[(i >> 1) & 1][1], x, y);
                             packed[8 * g + i / 2] = half2_of(x, y);

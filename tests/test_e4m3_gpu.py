@@ -449,11 +449,12 @@ def test_scales_far_apart_and_scores_far_apart():
             check_attention(got, q, pool, table, entries, 3, scale, torch.bfloat16)
 
 
-@pytest.mark.parametrize("cap", [2.0 ** -100, 1e-3, 8192.0])
+@pytest.mark.parametrize("cap", [2.0 ** -100, 1e-3, 2.0, 10.0, 60.0, 8192.0])
 def test_caps_at_their_borders(cap):
     """The least cap leaves all keys alike.  With the largest the hardware's approximations show: in cap * (1 - 2 r), r = 1 / (1 + e), the
     exponential's error of 2^-22 moves 2 r by 2^-23 (r' = -r^2, e = 1), the reciprocal's unit in the last place by 2^-23, the sum's rounding by
-    2^-24: 1.25 * 2^-22 of the cap together."""
+    2^-24: 1.25 * 2^-22 of the cap together.  (Scores up to a quarter of the cap, with a cap of 10 some, of 60 all, have less: the series that
+    portions take for them ends 2^-23.5 of the cap early.)"""
     rng = np.random.default_rng(15)
     shapes = [(140, 60), (1, 150), (1, 0)]
     pool, table = filled_pool(rng, [count + start for count, start in shapes], 2, 32, 64, 48)
