@@ -125,10 +125,17 @@ struct Schedule {
     const E4m3Attention& p;
     long total, stretch, lo, hi;                   // the row's length, a CTA's share, this CTA's
     long begin;                                    // of the unit that is next
-    int entry, tile, head, blocks, length, start, count;
+    int entry, tile, head, blocks, length, start, count, offset;
+    int base, count_of_lane, start_of_lane, offset_of_lane;          // 32 entries, one a lane
     int set_up;                                    // places that a unit's set-up takes
     bool apart;                                    // every unit has CTAs of its own: it begins at a multiple of the stretch
 
+    __device__ void load(int from, int lane) {
+        base = from;
+        const int e = from + lane;
+        const bool there = e < p.n_items;
+        count_of_lane = there ? p.item_count[e] : 0, start_of_lane = there ? p.item_start[e] : 0, offset_of_lane = there ? p.item_offset[e] : 0;
+    }
     __device__ int first_block(int s, int t) const {
         const int first = p.window > 0 ? s + t * UNIT - p.window + 1 : 0;
         return first > 0 ? first / TILE : 0;
@@ -144,11 +151,10 @@ struct Schedule {
 
     __device__ Schedule(const E4m3Attention& params, int lane) : p(params), total(0), entry(-1) {
         int sum = 0, none = 0, most = 0, units = 0;         // blocks of this lane's units, those without any, the longest; all units
-        for (int base = 0; base < p.n_items; base += 32) {
-            const int e = base + lane;
-            const int c_of = e < p.n_items ? p.item_count[e] : 0, s_of = e < p.n_items ? p.item_start[e] : 0;
-            for (uint32_t bits = __ballot_sync(0xffffffffu, c_of > 1); bits != 0; bits &= bits - 1) {
-                const int c = __shfl_sync(0xffffffffu, c_of, __ffs(bits) - 1), s = __shfl_sync(0xffffffffu, s_of, __ffs(bits) - 1);
+        for (int from = 0; from < p.n_items; from += 32) {
+            load(from, lane);
+            for (uint32_t bits = __ballot_sync(0xffffffffu, count_of_lane > 1); bits != 0; bits &= bits - 1) {
+                const int c = __shfl_sync(0xffffffffu, count_of_lane, __ffs(bits) - 1), s = __shfl_sync(0xffffffffu, start_of_lane, __ffs(bits) - 1);
                 for (int t = lane; t < tiles_of(c); t += 32) {
                     const int n = blocks_of(s, c, t);
                     sum += n, none += n == 0 ? 1 : 0, most = max(most, n);
@@ -171,12 +177,11 @@ struct Schedule {
         if (lo >= hi) return;
         // the unit in which the stretch begins
         begin = 0;
-        for (int base = 0; base < p.n_items; base += 32) {
-            const int e = base + lane;
-            const int c_of = e < p.n_items ? p.item_count[e] : 0, s_of = e < p.n_items ? p.item_start[e] : 0;
-            for (uint32_t bits = __ballot_sync(0xffffffffu, c_of > 1); bits != 0; bits &= bits - 1) {
+        for (int from = 0; from < p.n_items; from += 32) {
+            if (base != from) load(from, lane);
+            for (uint32_t bits = __ballot_sync(0xffffffffu, count_of_lane > 1); bits != 0; bits &= bits - 1) {
                 const int src = __ffs(bits) - 1;
-                const int c = __shfl_sync(0xffffffffu, c_of, src), s = __shfl_sync(0xffffffffu, s_of, src), n = tiles_of(c);
+                const int c = __shfl_sync(0xffffffffu, count_of_lane, src), s = __shfl_sync(0xffffffffu, start_of_lane, src), n = tiles_of(c);
                 for (int first = 0; first < n; first += 32) {
                     const int t = n - 1 - first - lane;
                     const int of_lane = t >= 0 ? blocks_of(s, c, t) : 0, mine = t >= 0 ? places(of_lane) : 0;
@@ -194,6 +199,7 @@ struct Schedule {
                         head = (int)divided(lo - begin, length);
                         begin += (long)head * length;
                         entry = base + src, tile = n - 1 - first - at, start = s, count = c;
+                        offset = __shfl_sync(0xffffffffu, offset_of_lane, src);
                         return;
                     }
                     begin += (long)__shfl_sync(0xffffffffu, upto, 31) * p.n_heads;
@@ -207,7 +213,7 @@ struct Schedule {
         const long end = begin + length;
         const int from = (int)(max(lo, begin) - begin), to = (int)(min(hi, end) - begin);      // place 0 is the unit's set-up
         u.entry = entry, u.head = head;
-        u.row0 = p.item_offset[entry] + tile * UNIT, u.rows = min(UNIT, count - tile * UNIT), u.pos0 = start + tile * UNIT;
+        u.row0 = offset + tile * UNIT, u.rows = min(UNIT, count - tile * UNIT), u.pos0 = start + tile * UNIT;
         u.block_lo = first_block(start, tile) + max(0, from - set_up);
         u.blocks = min(blocks, max(0, to - set_up)) - max(0, from - set_up);
         u.first_cta = (int)divided(begin, stretch);
@@ -218,7 +224,7 @@ struct Schedule {
             head = 0;
             if (--tile < 0) {
                 do entry++; while (p.item_count[entry] <= 1);          // (the row goes on, so there is one)
-                start = p.item_start[entry], count = p.item_count[entry];
+                start = p.item_start[entry], count = p.item_count[entry], offset = p.item_offset[entry];
                 tile = tiles_of(count) - 1;
             }
             blocks = blocks_of(start, count, tile), length = places(blocks);
