@@ -117,6 +117,7 @@ STORES = [
     (1, 1, 256, 16, 256, 128, [[300], [21], [1]]),
     (5, 5, 32, 48, 32, 112, [[1] * 20, [1] * 20, [7] * 20]),
     (12, 12, 64, 64, 64, 64, [[700, 1, 350], [300, 60, 1]]),
+    (2, 1, 32, 16, 24, 48, [[70 + i for i in range(50)], [1] * 50]),
 ]
 
 
