@@ -155,8 +155,7 @@ def prepare(case, seed):
     taken = torch.arange(max(blocks), device="cuda")[None, :] < ints(blocks)[:, None]
     table = torch.full((len(entries), max(blocks)), -1, dtype=torch.int32, device="cuda")
     table[taken] = places
-    # (a program that has put a step together knows whether its entries are single tokens)
-    state = {"case": case, "longest": max(counts), "singles": min(counts) == 1, "block_table": table, "item_start": ints(starts), "item_count": ints(counts),
+    state = {"case": case, "block_table": table, "item_start": ints(starts), "item_count": ints(counts),
              "item_offset": ints([sum(counts[:i]) for i in range(len(counts))])}
     state["k_pages"], state["k_scales"] = _filled(generator, pages, kv_heads, page, dim)
     state["v_pages"], state["v_scales"] = _filled(generator, pages, kv_heads, page, vdim)
@@ -212,9 +211,10 @@ def _attention_own(state):
     c = state["case"]
     if c["vdim"] not in _workspaces:
         _workspaces[c["vdim"]] = ops.e4m3_workspace(state["q"].device, c["vdim"])
+    counts = [count for _, count in _entries(c)]
     ops.e4m3_attention(state["out"], state["q"], state["k_pages"], state["v_pages"], state["k_scales"], state["v_scales"],
                        state["block_table"], state["item_offset"], state["item_count"], state["item_start"], c["heads"], c["kv_heads"],
-                       c["dim"] ** -0.5, cap=c["cap"], window=c["window"], longest=state["longest"], singles=state["singles"],
+                       c["dim"] ** -0.5, cap=c["cap"], window=c["window"], longest=max(counts), singles=min(counts) == 1,
                        workspace=_workspaces[c["vdim"]])
 
 
