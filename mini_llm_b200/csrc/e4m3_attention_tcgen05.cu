@@ -270,6 +270,10 @@ __device__ __forceinline__ void give_up(Shared& sh, const E4m3Attention& p, int 
 
 // A place in the ring of stages, and how often the ring has been around (its parity).  Counted, not divided: a division by a number that is not
 // known beforehand costs a lone thread a hundred clocks, and several a block made the products' issue the longest chain of all.
+// A wait by parity is exact only where the phase before the one that is meant is known to be over.  A role that walks every block knows it from its
+// own waits.  A softmax tile passes over the blocks of a unit in which it has no rows (or fewer) without waiting, so that it waits for a ring's
+// barrier only behind s_ready, whose phases it counts itself: S of a block is made when all converter warps have put the block's keys, which
+// each does after the values of the block before, and so after all earlier blocks of the stage.
 struct Ring {
     int stage = 0;
     uint32_t parity = 0;
@@ -504,8 +508,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             bool sees_none = false;
             for (int j = 0; j < n; j++, seen_blocks++) {
                 const int s = ring.stage, key0 = (u.block_lo + j) * TILE + 64 * half;
-                // (the values' barrier too: what stands beside the tiles comes with it)
-                ok = wait_or_fail(sh, &sh.v_full[s], ring.parity) && wait_or_fail(sh, &sh.s_ready[tile], seen_blocks & 1);
+                // The values' barrier too: what stands beside the tiles comes with it.  Behind S, not ahead of it: a tile that has passed over blocks does not
+                // know how far the converters are, and takes a phase two older for the one it means; that S is there shows the older one over.
+                ok = wait_or_fail(sh, &sh.s_ready[tile], seen_blocks & 1) && wait_or_fail(sh, &sh.v_full[s], ring.parity);
                 ring = ring.next(stages);
                 tcgen05_after_sync();
                 if (j == 0) q_factor = sh.q_factor[row];

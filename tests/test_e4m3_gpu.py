@@ -636,3 +636,32 @@ def test_refusals():
     ops.e4m3_store(**{**good, "qkv": qkv[:0], "q_out": out[:0], "positions": ints([]), "token_item": ints([])})
     none = torch.zeros((0, 2), dtype=torch.int32, device="cuda")
     ops.e4m3_attention(out[:0], q[:0], kp, vp, ks, vs, none, ints([]), ints([]), ints([]), 4, 2, 0.1, workspace=workspace)
+
+
+# ---- units that stand behind one another in a CTA --------------------------------------------------
+
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(12, 4, 64, 64), (12, 4, 128, 32)])
+@pytest.mark.parametrize("shapes", [
+    [(100, 90)] + [(700, 0)] * 16,                                        # few blocks of one tile, then units of two
+    [(256 * 5 + 100, 300)] * 6,                                           # the remainder of every portion comes ahead of its full units
+    [(count, 100 * i) for i in range(16) for count in (40, 500)],         # a short portion ahead of every long one
+])
+def test_units_of_one_tile_ahead_of_units_of_two(heads, kv_heads, dim, page, shapes):
+    """The scales differ from block to block, so that a tile that meets another block's would show; against the kernel of every size.  Both results are
+    rounded to bfloat16, 2^-8 each.  Of the sum of the weights times |v|, `top` at most, are off: the weights of 16 bits by 2^-11, sums of N terms
+    in 32 bits by N 2^-24, and by scores as in ``check_attention``, of both kernels."""
+    rng = np.random.default_rng(dim + len(shapes))
+    pool, table = filled_pool(rng, [count + start for count, start in shapes], kv_heads, page, dim, dim)
+    entries, scale, longest = laid_out(shapes), 0.1 * dim ** -0.5, max(count + start for count, start in shapes)
+    q = torch.tensor(rng.normal(0, 1, (entries[-1][0] + entries[-1][1], heads * dim)), dtype=torch.float32, device="cuda").to(torch.bfloat16)
+    k, v = (np.abs(plain.VALUES[pool.codes[name]]) * pool.scales[name].repeat(16, axis=2)[..., None] for name in ("k", "v"))
+    top, edge = np.nanmax(v), longest * 448.0 * np.nanmax(pool.scales["v"])
+    most = scale * np.sqrt(np.nanmax((k * k).sum(axis=3))) * float(q.float().view(-1, dim).norm(dim=1).max())
+    for window in (0, 200):
+        want = attend(pool, table, entries, q, heads, dim, scale, window=window, plain=True).float()
+        first = attend(pool, table, entries, q, heads, dim, scale, window=window)
+        for _ in range(4):
+            assert torch.equal(attend(pool, table, entries, q, heads, dim, scale, window=window), first)
+        got = first.float()
+        bound = 2.0 ** -8 * (want.abs() + got.abs()) + top * (2.0 ** -11 + longest * 2.0 ** -24 + 2 * 2.0 ** -20 * (1 + most)) + edge * 2.0 ** -32
+        assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
