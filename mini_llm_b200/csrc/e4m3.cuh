@@ -52,6 +52,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// Queries as 16-bit floats: the e for which 2^e brings the largest entry of a head to between 2^14 and 2^15.  From -113 on, for entries up to 2^128; not beyond
+// 110, whose inverse and scale still make a number (entries below 2^-96 become smaller ones).  Zeros, and what is not finite, stay as they are.
+__device__ __forceinline__ int query_exponent(float largest) {
+    return largest > 0.0f && largest < INFINITY ? min(110, 14 - exponent_of(largest)) : 0;
+}
+// What brings a head's scores into place as a number: an infinite one would make none of a product of zero.  Where it is cut off, at 2^128, scores differ by
+// 2^30 and more or not at all (a product is a whole number of 2^-33, a key's scale 2^-64 or more), and do so still.  (Cutting it off again where it
+// meets a block's scale, in the loops, cost 3 % of a long prompt and 5 % of 64 single tokens; what the caller keeps to excludes that it passes 2^128 there.)
+__device__ __forceinline__ float finite_factor(float factor) { return fminf(factor, 3.402823466e38f); }
+
 // a / b of numbers that are not negative (the 64-bit division costs some hundred clocks, and a row is hardly ever that long).
 __device__ __forceinline__ long divided(long a, long b) {
     return ((a | b) >> 31) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;

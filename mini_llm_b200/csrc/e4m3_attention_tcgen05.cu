@@ -417,10 +417,9 @@ __device__ __forceinline__ void put_queries(const E4m3Attention& p, const Unit& 
             for (int c = 0; c < 4; c++) top = max_of_three(top, fabsf(__uint_as_float(w[c] << 16)), fabsf(__uint_as_float(w[c] & 0xffff0000u)));
 #pragma unroll
             for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // (zeros, and what is not finite, stay as they are)
-            const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
+            const int e = query_exponent(top);
             const float factor = power_of_two(e);
-            if (chunk == 0) factors[row] = p.scale * power_of_two(-e) * LOG2E;
+            if (chunk == 0) factors[row] = finite_factor(p.scale * power_of_two(-e) * LOG2E);
             uint32_t h[4];
 #pragma unroll
             for (int c = 0; c < 4; c++) h[c] = half2_of(__uint_as_float(w[c] << 16) * factor, __uint_as_float(w[c] & 0xffff0000u) * factor);

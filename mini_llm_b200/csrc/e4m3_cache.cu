@@ -595,10 +595,9 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // (zeros, and what is not finite, stay as they are)
-            const int e = top > 0.0f && top < INFINITY ? max(-110, min(110, 14 - exponent_of(top))) : 0;
+            const int e = query_exponent(top);
             const float factor = power_of_two(e);
-            if (c == 0) q_factors[r] = p.scale * power_of_two(-e) * (has_cap ? 1.0f : LOG2E);
+            if (c == 0) q_factors[r] = finite_factor(p.scale * power_of_two(-e) * (has_cap ? 1.0f : LOG2E));
 #pragma unroll
             for (int d = 0; d < KG; d++)
 #pragma unroll

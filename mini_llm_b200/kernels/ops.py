@@ -2168,6 +2168,7 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
     head is NaN throughout or nowhere and a scale a power of two from 2^-64 on, as ``e4m3_store`` leaves them.  score = q . k * ``scale``, with
     ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if given; softmax and the weighted sum
     in 32 bits; query head h reads key/value head h // (heads / kv_heads).  A row that sees no key (a negative position) is zero; pages that the table does not name are not seen.
+    The largest entry of a query head times ``scale`` times a visible block's scale stays below 2^112: beyond it a result may be NaN where 32-bit scores are not.
 
     ``longest=1``: the caller knows that no entry brings more than one token (one that does is left out: its rows stay as they are);
     ``singles=False``: that none brings just one (likewise).  Other values of ``longest`` change nothing.  ``workspace``

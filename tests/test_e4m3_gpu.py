@@ -665,3 +665,37 @@ def test_units_of_one_tile_ahead_of_units_of_two(heads, kv_heads, dim, page, sha
         got = first.float()
         bound = 2.0 ** -8 * (want.abs() + got.abs()) + top * (2.0 ** -11 + longest * 2.0 ** -24 + 2 * 2.0 ** -20 * (1 + most)) + edge * 2.0 ** -32
         assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+
+
+# ---- the ends of what 32 bits hold -----------------------------------------------------------------
+
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("query, held, scale", [
+    (126, -64, -60), (127, -64, -62), (126, -64, -62), (127, -64, -70), (111, -64, -47),       # the largest queries: scores of 4, 2, 1, 2^-7 and 1
+    (100, -64, 60), (127, -64, 50), (100, 20, -110), (125, 0, -20),                            # products of factors beyond 32 bits
+    (-100, 40, 127), (0, 40, 60), (-126, 55, 126), (-126, 55, 72),                             # the smallest queries, the largest scales
+])
+def test_queries_and_scales_of_all_sizes(query, held, scale, cap):
+    """Queries of one entry, +-2^query, over keys that are zero but for one, 1 at a scale of 2^held: that key's score is +-2^(query + held + scale), all
+    others' zero."""
+    rng = np.random.default_rng(17)
+    shapes = [(150, 70), (1, 99), (3, 60), (1, 40)]
+    pool, table = filled_pool(rng, [count + start for count, start in shapes], 2, 32, 64, 48)
+    stored = ~np.isnan(pool.scales["k"])
+    pool.codes["k"][...] = 0
+    pool.scales["k"][stored] = 2.0 ** held
+    for item in range(len(shapes)):
+        pool.codes["k"][table[item, 1], :, 5, 5] = 0x38                           # position 37
+    pool.up()
+    entries = laid_out(shapes)
+    q = torch.zeros((entries[-1][0] + 1, 4, 64), device="cuda")
+    q[:, 0::2, 5], q[:, 1::2, 5] = 2.0 ** query, -2.0 ** query
+    q = q.flatten(1).to(torch.bfloat16)
+    want, spread, most, edge = plain.attention(q.float().cpu().numpy(), pool.codes["k"], pool.codes["v"], pool.scales["k"], pool.scales["v"], table,
+                                               entries, 4, 2.0 ** scale, cap)
+    # (scores are powers of two or zero, so that but for a cap only the exponential, its argument's rounding and the weights' 16 bits are off)
+    bound = np.abs(want) * 2.0 ** -8 + spread * (2.0 ** -11 + 2.0 ** -20 * (1 + (cap or min(most, 16.0)))) + edge * 2.0 ** -32
+    for plain_kernel in (True, False):
+        got = attend(pool, table, entries, q, 4, 48, 2.0 ** scale, cap=cap, plain=plain_kernel).float().cpu().numpy()
+        assert np.isfinite(got).all()
+        assert (np.abs(got - want) <= bound).all()
