@@ -78,18 +78,20 @@ __device__ __forceinline__ void turn_eight(float (&x)[8], int first, int rot_dim
     }
 }
 
-// The largest squares of eight columns, as bits (what is no number, or no finite one, is the largest of all): of pairs that turn, and of others.
-__device__ __forceinline__ void square_bits(const float (&x)[8], int first, int rot_dims, uint32_t& turned, uint32_t& still) {
+// The larger of `most` and the squares of eight columns, as bits (what is no number, or no finite one, is the largest of all): of the lengths of pairs that
+// turn, their entries times the amplitude (the square of the one or the other alone may lie beyond 32 bits where that of both does not), and of
+// other entries.
+__device__ __forceinline__ uint32_t largest_square(float (&x)[8], int first, int rot_dims, float amplitude, uint32_t most) {
+    if (first < rot_dims && amplitude != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __fmul_rn(x[i], first + i < rot_dims ? amplitude : 1.0f);
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float a = __fmul_rn(x[2 * i], x[2 * i]), b = __fmul_rn(x[2 * i + 1], x[2 * i + 1]);
-        if (first + 2 * i < rot_dims) turned = max(turned, __float_as_uint(__fadd_rn(a, b)));
-        else still = max(still, max(__float_as_uint(a), __float_as_uint(b)));
+        most = max(most, first + 2 * i < rot_dims ? __float_as_uint(__fadd_rn(a, b)) : max(__float_as_uint(a), __float_as_uint(b)));
     }
-}
-// The larger of the two, the amplitude's square on what turns (rounding keeps the order, so that the largest one's is the largest).
-__device__ __forceinline__ uint32_t largest_square(uint32_t turned, uint32_t still, float amplitude_squared) {
-    return max(still, __float_as_uint(__fmul_rn(__uint_as_float(turned), amplitude_squared)));
+    return most;
 }
 
 // A lane's pieces of eight columns of rows side by side, every 32nd, row by row: `act(row, column, numbers)` for each, the next one on its way
@@ -199,7 +201,6 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const E4m3Store p,
             const bool values = slot >= p.kv_heads;
             const int head = slot - (values ? p.kv_heads : 0);
             const int size = values ? p.vdim : p.dim, rot = values ? 0 : p.rot_dims;
-            const float amplitude_squared = p.amplitude * p.amplitude;
             const T* from = qkv + (values ? p.v_off : p.k_off) + (long)head * size + (first + r0) * p.ld;
             uint8_t* pages = values ? p.v_pages : p.k_pages;
             float* scales = values ? p.v_scales : p.k_scales;
@@ -209,22 +210,22 @@ __global__ void __launch_bounds__(STORE_THREADS) store_kernel(const E4m3Store p,
             const long place = (long)page_id * p.kv_heads + head;
             float* scale_at = scales + place * (p.page / E4M3_BLOCK) + slot0 / E4M3_BLOCK;
             const float held = lead > 0 ? *scale_at : 0.0f;
-            uint32_t turned = 0, still = 0;
-            each_piece(from, p.ld, count, size, lane, [&](int, int col, float (&x)[8]) { square_bits(x, col, rot, turned, still); });
-            uint32_t top = __reduce_max_sync(0xffffffffu, largest_square(turned, still, amplitude_squared));
+            uint32_t most_here = 0;
+            each_piece(from, p.ld, count, size, lane, [&](int, int col, float (&x)[8]) { most_here = largest_square(x, col, rot, p.amplitude, most_here); });
+            uint32_t top = __reduce_max_sync(0xffffffffu, most_here);
             uint32_t bad = 0;                                                  // rows that are not finite
             if (top >= 0x7f800000u) {
                 top = 0;
                 for (int r = 0; r < count; r++) {
-                    turned = still = 0;
+                    most_here = 0;
                     for (int col = lane * 8; col < size; col += 256) {
                         EightOf<T> held_here;
                         float x[8];
                         held_here.load(from + r * p.ld + col);
                         held_here.unpack(x);
-                        square_bits(x, col, rot, turned, still);
+                        most_here = largest_square(x, col, rot, p.amplitude, most_here);
                     }
-                    const uint32_t of_row = __reduce_max_sync(0xffffffffu, largest_square(turned, still, amplitude_squared));
+                    const uint32_t of_row = __reduce_max_sync(0xffffffffu, most_here);
                     if (of_row >= 0x7f800000u) bad |= 1u << r;
                     else top = max(top, of_row);
                 }

@@ -1900,6 +1900,7 @@ E4M3_NONE = 0x7f               # the code that is no number
 E4M3_LEAST_CAP = 2.0 ** -100   # (its inverse is a 32-bit number)
 E4M3_MOST_CAP = 8192.0         # (a capped score is off by 2^-22 of the cap: here 2^-9, half of what a bfloat16 result is rounded by)
 E4M3_MOST_SCALE = 2.0 ** 127   # of scores, and the most amplitude: numbers that 32 bits hold
+E4M3_LEAST_AMPLITUDE = 2.0 ** -100  # but for 0: a cosine times it keeps its digits
 E4M3_FAST_SIZES = 128          # entries of a key or value up to which the kernels on tensor cores take them
 
 
@@ -2018,8 +2019,8 @@ def _check_e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_
         raise KernelError(f"{who} does not take heads of {dim} and {vdim} entries (multiples of 16 up to 256)")
     if rot_dims < 0 or rot_dims % 2 or rot_dims > dim:
         raise KernelError(f"{who}: {rot_dims} turned entries do not fit a head of {dim}")
-    if not -E4M3_MOST_SCALE <= amplitude <= E4M3_MOST_SCALE:
-        raise KernelError(f"{who}: an amplitude of {amplitude} is not finite in 32 bits")
+    if not (amplitude == 0 or E4M3_LEAST_AMPLITUDE <= abs(amplitude) <= E4M3_MOST_SCALE):
+        raise KernelError(f"{who}: an amplitude of {amplitude} is not finite in 32 bits, or so small that its products lose digits")
     if min(k_off, v_off) < 0 or max(heads * dim, k_off + kv_heads * dim, v_off + kv_heads * vdim) > columns or k_off % 8 or v_off % 8:
         raise KernelError(f"{who}: the columns do not hold queries, keys and values, or are not multiples of 8")
     for name, t, kind in (("inv_freq", inv_freq, torch.float64), ("positions", positions, torch.int32), ("token_item", token_item, torch.int32)):
@@ -2048,7 +2049,7 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
 
     Rows of ``qkv`` (fp32 or bf16 [T, columns]) hold [q | k | v], k from column ``k_off``, v from ``v_off``.  The first ``rot_dims``
     entries of every query and key head turn in interleaved pairs by position * ``inv_freq`` [rot_dims / 2] (float64; None without
-    turned entries), cosine and sine times ``amplitude``.  The turned queries go to ``q_out`` [T, heads * dim] (None: they are
+    turned entries), cosine and sine times ``amplitude`` (0, or 2^-100 to 2^127 in size).  The turned queries go to ``q_out`` [T, heads * dim] (None: they are
     not wanted), which may be the queries' own columns of ``qkv``, and no other part of it; all else of ``qkv`` stays as it is.
     ``writes=False``: queries only.
 
@@ -2056,8 +2057,8 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
     rows stand side by side at positions that grow by one (rows of one request that repeat a position, as rows that fill a step up do, may
     leave anything in the blocks that they name, and nothing elsewhere); no two requests of a step store into one page; a row at a negative
     position, or whose page the table does not name (an index outside the pages, a column outside the table), is stored nowhere.  The scale of a block of 16
-    positions is the least power of two s >= 2^-64 with n <= (448 s)^2 for all its rows so far, n being x^2 + y^2 of a pair that turns (times ``amplitude``^2; a turn
-    keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
+    positions is the least power of two s >= 2^-64 with n <= (448 s)^2 for all its rows so far, n being x^2 + y^2 of a pair that turns (its entries
+    times ``amplitude``; a turn keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
     row that begins a block begins it anew, whatever was there.  A key or value head with an n that is not finite is stored as
     NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes."""
     n_pages = page = max_blocks = ld_q = 0
@@ -2068,7 +2069,7 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
         (n_positions,), (n_places,), bits = positions.shape, token_item.shape, 2 if dtype is _FP32 else 1
         fits = (index >= 0 and (bits == 2 or dtype is _BF16) and step == 1 and not (at | (ld << bits)) & 15
                 and heads > 0 and kv_heads > 0 and 0 < dim <= 256 and 0 < vdim <= 256 and not (dim | vdim) & 15
-                and 0 <= rot_dims <= dim and not rot_dims & 1 and -E4M3_MOST_SCALE <= amplitude <= E4M3_MOST_SCALE
+                and 0 <= rot_dims <= dim and not rot_dims & 1 and (amplitude == 0 or E4M3_LEAST_AMPLITUDE <= abs(amplitude) <= E4M3_MOST_SCALE)
                 and k_off >= 0 and v_off >= 0 and not (k_off | v_off) & 7
                 and heads * dim <= columns and k_off + kv_heads * dim <= columns and v_off + kv_heads * vdim <= columns
                 and n_positions >= n and n_places >= n and positions.dtype is _INT32 and token_item.dtype is _INT32

@@ -699,3 +699,58 @@ def test_queries_and_scales_of_all_sizes(query, held, scale, cap):
         got = attend(pool, table, entries, q, 4, 48, 2.0 ** scale, cap=cap, plain=plain_kernel).float().cpu().numpy()
         assert np.isfinite(got).all()
         assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rot", [0, 8, 32])
+@pytest.mark.parametrize("power", [-100, -80, -70, 0, 40, 63, 64, 100, 127])
+def test_amplitudes_of_all_sizes(power, rot, dtype):
+    """Keys whose turned entries, times an amplitude of 2^power, are of any size and others of size 1; values, which no amplitude touches, are what
+    they are without one, and so is a key of zeros."""
+    from mini_llm_b200.kernels import ops
+    rng = np.random.default_rng(18)
+    n, dim = 21, 32
+    amplitude = 2.0 ** power
+    rows = rng.normal(0, 1, (n, 3 * dim))
+    # (turned keys of size 2^-20 to 2^20: the largest amplitudes want small entries, the smallest large ones)
+    rows[:, dim:dim + rot] *= 2.0 ** float(np.clip(-power + rng.integers(-20, 20), -120, 110))
+    rows[4, dim:2 * dim] = 0.0
+    qkv = torch.tensor(rows, dtype=torch.float32, device="cuda").to(dtype)
+    inv_freq = 100.0 ** (-np.arange(max(rot // 2, 1)) / 16)
+    pool, before = (Pool(2, 1, 32, dim, dim) for _ in range(2))
+    table, positions, items = [[1]], np.arange(n), [0] * n
+    ops.e4m3_store(None, qkv, dim, 2 * dim, 1, 1, dim, dim, rot, torch.tensor(inv_freq, dtype=torch.float64, device="cuda"), amplitude, ints(positions),
+                   ints(items), ints(table), *pool.operands)
+    pool.down()
+    host = qkv.float().cpu().numpy()
+    compare_append(pool, before, "v", host[:, None, 2 * dim:], 0, positions, items, np.array(table), inv_freq, 1.0)
+    # the same numbers from entries that are multiplied already: a power of two leaves their digits
+    already = host[:, None, dim:2 * dim].astype(np.float64)
+    already[..., :rot] *= amplitude
+    with np.errstate(over="ignore"):
+        squares = already ** 2
+    lengths = np.concatenate((squares[..., 0:rot:2] + squares[..., 1:rot:2], squares[..., rot:]), axis=-1).max(axis=-1)[:, 0]
+    for block in (slice(0, 16), slice(16, n)):
+        scale = float(pool.scales["k"][1, 0, block.start // 16])
+        assert scale == plain.least_scale(float(lengths[block].max()))
+        for t in range(n)[block]:
+            exact = plain.turned(already[t, 0], rot, t, inv_freq) / scale
+            got = plain.VALUES[pool.codes["k"][1, 0, t]]
+            assert (np.abs(got - np.clip(exact, -448.0, 448.0)) <= np.maximum(np.abs(exact) * 2.0 ** -4, 2.0 ** -10) + 448 * 2.0 ** -21).all()
+
+
+def test_amplitudes_that_are_refused():
+    from mini_llm_b200.kernels import ops
+    from mini_llm_b200.kernels.lib import KernelError
+    pool, qkv = Pool(2, 1, 32, 32, 32), torch.ones((3, 96), device="cuda")
+    for amplitude in (2.0 ** -101, -2.0 ** -140, 2.0 ** 127.5, -1e39, float("inf"), float("nan")):
+        with pytest.raises(KernelError, match="amplitude"):
+            ops.e4m3_store(None, qkv, 32, 64, 1, 1, 32, 32, 32, torch.ones(16, dtype=torch.float64, device="cuda"), amplitude, ints([0, 1, 2]),
+                           ints([0] * 3), ints([[0]]), *pool.operands)
+    # none at all leaves zeros, a negative one turns by half a turn more
+    for amplitude in (0.0, -1.0):
+        ops.e4m3_store(None, qkv, 32, 64, 1, 1, 32, 32, 32, torch.zeros(16, dtype=torch.float64, device="cuda"), amplitude, ints([0, 1, 2]),
+                       ints([0] * 3), ints([[0]]), *pool.operands)
+        pool.down()
+        np.testing.assert_array_equal(plain.VALUES[pool.codes["k"][0, 0, :3]] * pool.scales["k"][0, 0, 0], np.full((3, 32), amplitude))
+        np.testing.assert_array_equal(plain.VALUES[pool.codes["v"][0, 0, :3]] * pool.scales["v"][0, 0, 0], np.ones((3, 32)))
