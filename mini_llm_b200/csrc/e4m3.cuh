@@ -123,5 +123,7 @@ struct E4m3Attention {
     float* partial;                // results of parts, and how many of a result's parts have arrived (zero between launches)
     int* counters;
     int* status;                   // where a bounded wait that ran out leaves its code
+    int wait_limit_ns;             // of every wait; 0: as elsewhere
+    int role_away;                 // a test's switch: the role with this give-up code does nothing, and the others' waits run out; 0: none
 };
-static_assert(sizeof(E4m3Attention) == 168, "packed by the caller field by field, with C's alignment");
+static_assert(sizeof(E4m3Attention) == 176, "packed by the caller field by field, with C's alignment");

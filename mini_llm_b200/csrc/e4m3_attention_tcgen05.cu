@@ -244,21 +244,28 @@ struct Shared {
     float of_half[2][2][TILE];                     // what the two threads of a row tell one another
     // of the blocks of 16 keys: the keys' scale, the values' scale's exponent, and one by the values' scale
     float k_scale[MAX_STAGES][TILE / E4M3_BLOCK], v_exponent[MAX_STAGES][TILE / E4M3_BLOCK], v_inverse[MAX_STAGES][TILE / E4M3_BLOCK];
-    uint32_t absent[MAX_STAGES][4], none[MAX_STAGES][4];      // keys that are not there, and whose values are no numbers (a bit a key)
+    alignas(8) uint32_t absent[MAX_STAGES][4];     // keys that are not there, and whose values are no numbers (a bit a key; read two words at a time)
+    alignas(8) uint32_t none[MAX_STAGES][4];
+    // (last: 12 bytes more ahead of the units move what is read in the loops, 616 us for 573 of 2,000 tokens at the end of 16,000)
+    uint32_t wait_limit;                           // of every wait, in ns
+    alignas(8) uint64_t all_done;
 };
 
-// (a role that gave up leaves its barriers as they are, so that the others' waits run out, or find out here)
+// Codes of the roles that give up.
+constexpr int CONVERTERS_GAVE_UP = 31, PRODUCTS_GAVE_UP = 33, SOFTMAX_GAVE_UP = 34, SCHEDULE_GAVE_UP = 35;
+
+// (a role that gave up leaves its barriers as they are; the others find out here)
 // By a whole warp, with one answer for all of its lanes: what follows does not branch apart, and the compiler knows it.  Code that is seldom reached
 // is kept out of the way here and in the softmax: 24 warps in four roles share the instruction caches, and what they fetch past, they wait for
 // (766 us and 612 us for 2,000 tokens at the end of 16,000 of 32 heads of 128 with all of it in line; 704 and 574 this way).
 __device__ __forceinline__ bool wait_or_fail(Shared& sh, uint64_t* bar, uint32_t parity) {
     if (__builtin_expect(__any_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
-    const unsigned long long start = now_ns();
+    const uint32_t start = (uint32_t)now_ns();       // (32 bits of it: looks lie microseconds apart, and the limit is below 2^31)
     do {
 #pragma unroll 1
         for (int i = 0; i < 256; i++)
             if (__any_sync(0xffffffffu, mbar_try_wait(bar, parity))) return !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sh.failed));
-    } while (!__any_sync(0xffffffffu, now_ns() - start > WAIT_LIMIT_NS));
+    } while (!__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sh.failed) || (uint32_t)now_ns() - start > sh.wait_limit));
     return false;
 }
 __device__ __forceinline__ void give_up(Shared& sh, const E4m3Attention& p, int code) {
@@ -463,7 +470,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             mbar_init(&sh.o_added[i], 1);
             mbar_init(&sh.o_free[i], SOFTMAX_WARPS / 2);
         }
+        mbar_init(&sh.all_done, 1);
         sh.failed = 0;
+        sh.wait_limit = p.wait_limit_ns > 0 ? p.wait_limit_ns : (uint32_t)WAIT_LIMIT_NS;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == MMA_WARP) tmem_alloc(&sh.tmem, 512);
@@ -485,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
         const float cap_log2 = p.cap * LOG2E, cap_factor = CAP ? 2.0f / p.cap : 0.0f, by_cap = CAP ? 1.0f / cap_log2 : 0.0f;
         uint32_t seen_blocks = 0;                    // of this tile, over all units
         bool ok = true;
-        for (int k = 0;; k++) {
+        for (int k = 0; p.role_away != SOFTMAX_GAVE_UP; k++) {
             const bool more = next_unit(sh, k, u, ok);
             if (any_of_tile(tile, !ok)) ok = false;
             if (!ok || !more) break;
@@ -690,7 +699,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 }
             }
         }
-        if (!ok && lane == 0) give_up(sh, p, 34);
+        if (!ok && lane == 0) give_up(sh, p, SOFTMAX_GAVE_UP);
+    } else if (warp < MMA_WARP && p.role_away == CONVERTERS_GAVE_UP) {
+        // (a test's switch; within the loop below it makes registers spill)
     } else if (warp < MMA_WARP) {
         // ---- converters: a thread a key ----
         const int t = threadIdx.x - SOFTMAX_WARPS * 32;
@@ -800,7 +811,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             }
             if (!ok) break;
         }
-        if (!ok && lane == 0) give_up(sh, p, 31);
+        if (!ok && lane == 0) give_up(sh, p, CONVERTERS_GAVE_UP);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(IDLE_REGISTERS));
         if (warp == MMA_WARP) {
@@ -830,7 +841,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 umma_commit_by(elected, &sh.o_added[tile]);
             };
             bool ok = true;
-            for (int k = 0; next_unit(sh, k, u, ok); k++) {
+            for (int k = 0; p.role_away != PRODUCTS_GAVE_UP && next_unit(sh, k, u, ok); k++) {
                 const Blocks of_unit(u);
                 // (the same for all lanes, and the compiler knows it)
                 const int n0 = __shfl_sync(0xffffffffu, of_unit.n[0], 0), n1 = __shfl_sync(0xffffffffu, of_unit.n[1], 0), most = max(n0, n1);
@@ -879,13 +890,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
                 seen_blocks[0] += n0, seen_blocks[1] += n1;
                 seen_units[0] += n0 > 0 ? 1 : 0, seen_units[1] += n1 > 0 ? 1 : 0;
             }
-            if (!ok && lane == 0) give_up(sh, p, 33);
+            if (!ok && lane == 0) give_up(sh, p, PRODUCTS_GAVE_UP);
+            // No product is on its way any more, whether all went well or a role gave up, when the memory that they read and write is given back.
+            umma_commit_by(elected, &sh.all_done);
+            mbar_wait(&sh.all_done, 0);
         } else if (warp == MMA_WARP + 1) {
             // ---- the next unit, while the others work on this one ----
             Schedule schedule(p, lane);
-            for (int k = 0;; k++) {
+            for (int k = 0; p.role_away != SCHEDULE_GAVE_UP; k++) {
                 if (!wait_or_fail(sh, &sh.unit_empty[k & 1], ((k >> 1) & 1) ^ 1)) {
-                    if (lane == 0) give_up(sh, p, 35);
+                    if (lane == 0) give_up(sh, p, SCHEDULE_GAVE_UP);
                     break;
                 }
                 u.entry = -1;
@@ -898,7 +912,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             }
         }
     }
+    tcgen05_before_sync();
     __syncthreads();
+    tcgen05_after_sync();
     if (warp == MMA_WARP) tmem_free(tmem, 512);
 }
 

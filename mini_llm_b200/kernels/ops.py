@@ -1905,11 +1905,11 @@ E4M3_FAST_SIZES = 128          # entries of a key or value up to which the kerne
 
 
 # struct E4m3Attention: out, ld_out, q, ld_q, k_pages, v_pages, k_scales, v_scales, block_table; max_blocks, n_pages, page; item_offset, item_count,
-# item_start; n_items, n_heads, n_kv_heads, dim, vdim; scale, cap; window; partial, counters, status
+# item_start; n_items, n_heads, n_kv_heads, dim, vdim; scale, cap; window; partial, counters, status; wait_limit_ns, role_away
 # struct E4m3Store: q_out, ld_q, qkv, ld; k_off, v_off, heads, kv_heads, dim, vdim, rot_dims; inv_freq, amplitude; positions, token_item, block_table;
 # max_blocks, n_pages, page; k_pages, v_pages, k_scales, v_scales; n
 _e4m3_rows = struct.Struct("@PlPl7iPf3P3i4Pi0P").pack
-_e4m3_operands = struct.Struct("@PlPlPPPPP3iPPP5i2fiPPP").pack
+_e4m3_operands = struct.Struct("@PlPlPPPPP3iPPP5i2fiPPP2i").pack
 
 _e4m3_store = Function("e4m3", "mllm_e4m3_store", [ctypes.c_char_p, I, I, P])
 _e4m3_plain = Function("e4m3", "mllm_e4m3_attention_plain", [ctypes.c_char_p, I, I, P])
@@ -2122,6 +2122,7 @@ class E4m3Workspace:
         self.counters = torch.zeros(2 * n_sms, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device) if status is None else status
         self.pointers = (self.partial.data_ptr(), self.counters.data_ptr(), self.status.data_ptr())
+        self.wait_limit_ns, self.role_away = 0, 0       # for tests: a shorter limit, and a role that stays away (its give-up code)
 
     def reset(self) -> None:
         """After a kernel gave up: counters and status start over."""
@@ -2207,7 +2208,7 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
     params = _e4m3_operands(
         out_at, ld_out, q_at, ld_q, k_at, v_at, k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), max_blocks, n_pages, page,
         item_offset.data_ptr(), item_count.data_ptr(), item_start.data_ptr(), n_items, heads, kv_heads, dim, vdim, scale, cap, window,
-        *(workspace.pointers if fast else (0, 0, 0)))
+        *(workspace.pointers if fast else (0, 0, 0)), *((workspace.wait_limit_ns, workspace.role_away) if fast else (0, 0)))
     stream = _on_device(index)
     if not fast:
         _launch_on(index, _e4m3_plain, params, n_rows, dtype_code(dtype), stream)

@@ -202,3 +202,32 @@ def test_what_a_cache_in_8_bits_refuses(folders, tmp_path):
     odd = h.make_model(str(tmp_path / "odd"), h.config([h.parallel(dim=16, vdim=24)]))
     with pytest.raises(ValueError, match="multiples of 16"):
         Engine(odd, page_size=16, cache_tokens=256, cache_dtype="e4m3")
+
+
+def test_a_step_whose_kernel_gave_up_is_reported_and_later_steps_are_right(folders):
+    from mini_llm_b200.engine import Engine, StepEntry
+    from mini_llm_b200.kernels.lib import KernelError
+    raw, page, _ = CONFIGS["D"]
+    tokens = random_tokens(8, 400, raw["vocab_size"])
+    engine = Engine(folders["D"], page_size=page, max_requests=2, cache_dtype="e4m3", cuda_graphs=False)
+
+    def logits(check=True):
+        slot = engine.open_request()
+        try:
+            first = engine.step([StepEntry(slot, tokens[:390], [389])])
+            if check:
+                engine.check_status()
+            return [first.cpu().numpy()] + [engine.step([StepEntry(slot, [t], [0])]).cpu().numpy() for t in tokens[390:]]
+        finally:
+            engine.close_request(slot)
+
+    want = logits()
+    workspace = engine.kernels._e4m3_workspace
+    workspace.wait_limit_ns, workspace.role_away = 2_000_000, 33
+    with pytest.raises(KernelError, match="bounded wait"):
+        logits()
+    workspace.wait_limit_ns = workspace.role_away = 0
+    for _ in range(2):
+        for a, b in zip(logits(), want):
+            np.testing.assert_array_equal(a, b)
+    engine.check_status()

@@ -754,3 +754,30 @@ def test_amplitudes_that_are_refused():
         pool.down()
         np.testing.assert_array_equal(plain.VALUES[pool.codes["k"][0, 0, :3]] * pool.scales["k"][0, 0, 0], np.full((3, 32), amplitude))
         np.testing.assert_array_equal(plain.VALUES[pool.codes["v"][0, 0, :3]] * pool.scales["v"][0, 0, 0], np.ones((3, 32)))
+
+
+# ---- waits that run out ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("away", [31, 33, 34, 35])                            # converters, products, softmax, schedule
+def test_a_role_that_stays_away_is_reported_and_the_next_call_is_right(away, dim, cap):
+    """Every wait of the portions' kernel is bounded.  Here one of its roles does nothing (a test's switch) and the limit is 2 ms: the others give up and
+    the kernel returns with a code of one of them; after ``reset`` the workspace serves as a new one does."""
+    from mini_llm_b200.kernels import ops
+    rng = np.random.default_rng(19)
+    shapes = [(100, 30), (700, 200), (1, 90), (300, 3000)]
+    pool, table = filled_pool(rng, [count + start for count, start in shapes], 2, 32, dim, dim)
+    entries = laid_out(shapes)
+    q = rows_of(rng, entries[-1][0] + entries[-1][1], 4 * dim, torch.bfloat16)
+    want = attend(pool, table, entries, q, 4, dim, 0.05, cap=cap)
+    workspace = ops.e4m3_workspace("cuda", dim)
+    for _ in range(2):
+        workspace.wait_limit_ns, workspace.role_away = 2_000_000, away
+        attend(pool, table, entries, q, 4, dim, 0.05, cap=cap, workspace=workspace)
+        assert int(workspace.status) in {31, 33, 34, 35} - {away}
+        workspace.wait_limit_ns = workspace.role_away = 0
+        workspace.reset()
+        assert int(workspace.status) == 0 and int(workspace.counters.abs().sum()) == 0
+        assert torch.equal(attend(pool, table, entries, q, 4, dim, 0.05, cap=cap, workspace=workspace), want)
+        assert int(workspace.status) == 0 and int(workspace.counters.abs().sum()) == 0
