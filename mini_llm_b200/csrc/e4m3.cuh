@@ -5,6 +5,8 @@
 // A head's positions of a page lie side by side, so that a block is one contiguous piece of 16 * size bytes.
 #pragma once
 
+#include <limits.h>
+
 #include "common.cuh"
 
 constexpr int E4M3_BLOCK = 16;                 // positions that share a scale
@@ -127,3 +129,11 @@ struct E4m3Attention {
     int role_away;                 // a test's switch: the role with this give-up code does nothing, and the others' waits run out; 0: none
 };
 static_assert(sizeof(E4m3Attention) == 176, "packed by the caller field by field, with C's alignment");
+
+// The keys that a query at a position sees: from here on (within a window, which may be as long as an int; positions may lie before the first) ...
+__device__ __forceinline__ int first_seen(int position, int window) { return window > 0 && position >= window ? position - window + 1 : 0; }
+// ... up to its own, but for those behind the last that a request's row of the block table names, where every walk ends (a row of blocks of 128 from there
+// on is counted in an int).
+__device__ __forceinline__ int last_seen(int position, const E4m3Attention& p) {
+    return (int)min((long)position, min((long)p.max_blocks * p.page, (long)INT_MAX - 255) - 1);
+}

@@ -137,12 +137,11 @@ struct Schedule {
         count_of_lane = there ? p.item_count[e] : 0, start_of_lane = there ? p.item_start[e] : 0, offset_of_lane = there ? p.item_offset[e] : 0;
     }
     __device__ int first_block(int s, int t) const {
-        const int first = p.window > 0 ? s + t * UNIT - p.window + 1 : 0;
-        return first > 0 ? first / TILE : 0;
+        return first_seen(s + t * UNIT, p.window) / TILE;
     }
     __device__ int blocks_of(int s, int c, int t) const {
-        const int last = s + min(c, (t + 1) * UNIT) - 1;
-        return last < 0 ? 0 : last / TILE - first_block(s, t) + 1;
+        const int last = last_seen(s - 1 + min(c, (t + 1) * UNIT), p);
+        return last < 0 ? 0 : max(0, last / TILE - first_block(s, t) + 1);
     }
     __device__ int places(int of_blocks) const {
         return apart ? (max(of_blocks, 1) + (int)stretch - 1) / (int)stretch * (int)stretch : of_blocks + set_up;
@@ -295,7 +294,7 @@ struct Ring {
 struct Blocks {
     int n[2], most;
     __device__ explicit Blocks(const Unit& u) {
-        const int last0 = u.pos0 + min(u.rows, TILE) - 1, last1 = u.pos0 + u.rows - 1;
+        const int last0 = u.pos0 - 1 + min(u.rows, TILE), last1 = u.pos0 - 1 + u.rows;
         n[0] = last0 < 0 ? 0 : max(0, min(u.blocks, last0 / TILE - u.block_lo + 1));
         n[1] = u.rows > TILE && last1 >= 0 ? u.blocks : 0;
         most = max(n[0], n[1]);
@@ -510,8 +509,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             }
             const bool has_row = row < u.rows;
             const int pos = u.pos0 + (has_row ? row : u.rows - 1);
-            const int first = p.window > 0 ? pos - p.window + 1 : 0;
-            const int unseen = p.window > 0 ? u.pos0 + (tile + 1) * TILE - 1 - p.window : -1;      // keys up to here some row of the tile does not see
+            const int first = first_seen(pos, p.window);
+            const int unseen = first_seen(u.pos0 - 1 + min(u.rows, (tile + 1) * TILE), p.window) - 1;      // keys up to here some row of the tile does not see
             float m = -INFINITY, l = 0.0f, q_factor = 0.0f;
             bool sees_none = false;
             for (int j = 0; j < n; j++, seen_blocks++) {
@@ -712,9 +711,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             const int* table = p.block_table + (long)u.entry * p.max_blocks;
             // This thread's key, block after block: its position, its page's place in the table and its own in the page.
             int key = u.block_lo * TILE + t, page_index = key / p.page, slot = key - page_index * p.page;
-            const int key_end = min(u.pos0 + u.rows, (u.block_lo + n_blocks) * TILE);
+            const int key_last = min(u.pos0 - 1 + u.rows, (u.block_lo + n_blocks) * TILE - 1);
             auto look_up = [&]() -> int {                    // the key's page, or -1 where it is not there
-                const int id = key < key_end && page_index < p.max_blocks ? table[page_index] : -1;
+                const int id = key <= key_last && page_index < p.max_blocks ? table[page_index] : -1;
                 return id < p.n_pages ? id : -1;
             };
             auto row_of = [&](int id) -> long { return id >= 0 ? ((long)id * p.n_kv_heads + kv_head) * p.page + slot : -1; };

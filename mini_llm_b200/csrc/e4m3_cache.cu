@@ -282,16 +282,16 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attention_plain_kernel(const E4
     __syncthreads();
     if (entry < 0) return;                               // rows behind the last entry stay as they are
     const int pos = p.item_start[entry] + row - p.item_offset[entry];
-    const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    const int first = first_seen(pos, p.window), last = last_seen(pos, p);
     for (int d = threadIdx.x; d < p.dim; d += PLAIN_THREADS)
         q[d] = to_f32(static_cast<const T*>(p.q)[row * p.ld_q + (long)head * p.dim + d]);
     float o[2] = {0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-    for (int base = first; base <= pos; base += PLAIN_THREADS) {
+    for (int base = first; base <= last; base += PLAIN_THREADS) {
         const int key = base + threadIdx.x, index = key / p.page;
         float s = -INFINITY;
         long at = -1;
         __syncthreads();
-        if (key <= pos && index < p.max_blocks) {
+        if (key <= last) {
             const int id = p.block_table[(long)entry * p.max_blocks + index];
             if (id >= 0 && id < p.n_pages) at = ((long)id * p.n_kv_heads + kv_head) * p.page + key % p.page;
         }
@@ -403,9 +403,8 @@ struct StepSchedule {
         count_of_lane = there ? p.item_count[e] : 0, start_of_lane = there ? p.item_start[e] : 0, row_of_lane = there ? p.item_offset[e] : 0;
     }
     __device__ void of_position(int position, int& lowest, int& count) const {
-        const int first = p.window > 0 ? max(0, position - p.window + 1) : 0;
-        lowest = first / E4M3_BLOCK;
-        count = position >= 0 ? max(0, min(position / E4M3_BLOCK + 1, p.max_blocks * (p.page / E4M3_BLOCK)) - lowest) : 0;
+        lowest = first_seen(position, p.window) / E4M3_BLOCK;
+        count = position >= 0 ? max(0, (last_seen(position, p) + E4M3_BLOCK) / E4M3_BLOCK - lowest) : 0;
     }
     __device__ int places(int of_blocks) const {
         if (!apart) return of_blocks + set_up;
@@ -520,7 +519,7 @@ __global__ void __launch_bounds__(STEP_THREADS, STEP_CTAS) attention_step_kernel
         u.kv_head = at.unit / head_tiles;
         const int head_tile = at.unit - u.kv_head * head_tiles;
         u.n_rows = min(ROWS, group - head_tile * ROWS), u.head0 = u.kv_head * group + head_tile * ROWS;
-        u.row = at.row, u.pos = at.pos, u.first = p.window > 0 ? max(0, at.pos - p.window + 1) : 0;
+        u.row = at.row, u.pos = at.pos, u.first = first_seen(at.pos, p.window);
         // places of the unit in this stretch: the set-up's, then a block each
         const int from = (int)(max(at.lo, at.begin) - at.begin), to = (int)(min(at.hi, at.begin + at.length) - at.begin);
         u.lo = at.first_block + max(0, from - at.set_up), u.hi = at.first_block + min(at.blocks, max(0, to - at.set_up));

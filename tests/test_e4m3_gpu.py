@@ -781,3 +781,37 @@ def test_a_role_that_stays_away_is_reported_and_the_next_call_is_right(away, dim
         assert int(workspace.status) == 0 and int(workspace.counters.abs().sum()) == 0
         assert torch.equal(attend(pool, table, entries, q, 4, dim, 0.05, cap=cap, workspace=workspace), want)
         assert int(workspace.status) == 0 and int(workspace.counters.abs().sum()) == 0
+
+
+# ---- positions of all sizes ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(4, 2, 64, 16), (3, 1, 128, 48)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40, 1000])
+def test_windows_longer_than_any_context(window, heads, kv_heads, dim, page):
+    """Also with positions before the first: rows there are zero, the others see what they see without a window."""
+    rng = np.random.default_rng(20)
+    shapes = [(40, -5), (300, -200), (1, -3), (130, 20), (1, 77), (2, -1), (600, -300)]
+    pool, table = filled_pool(rng, [max(1, count + start) for count, start in shapes], kv_heads, page, dim, dim)
+    entries = laid_out(shapes)
+    q = rows_of(rng, entries[-1][0] + entries[-1][1], heads * dim, torch.bfloat16)
+    for plain_kernel in (False, True):
+        got = attend(pool, table, entries, q, heads, dim, 0.05, window=window, plain=plain_kernel)
+        check_attention(got, q, pool, table, entries, heads, 0.05, torch.bfloat16, 0.0, window)
+        assert torch.equal(got, attend(pool, table, entries, q, heads, dim, 0.05, plain=plain_kernel))
+
+
+@pytest.mark.parametrize("start", [129, 10 ** 6, 2 ** 31 - 40])
+def test_walks_end_where_the_block_table_does(start):
+    """Queries at positions behind the last that the table has a page for see all that it has, whatever their position, or, within a window that ends
+    behind it, nothing."""
+    rng = np.random.default_rng(21)
+    heads, dim, page, reach = 4, 64, 16, 128
+    pool, table = filled_pool(rng, [reach] * 3, 2, page, dim, dim)
+    entries = [(0, 40, start), (40, 1, start + 39), (41, 2, start + 5)]
+    q = rows_of(rng, 43, heads * dim, torch.bfloat16)
+    at_its_end = [(row, 1, reach - 1) for row in range(43)]
+    rows = np.array([0] * 40 + [1] + [2] * 2)
+    for plain_kernel in (False, True):
+        got = attend(pool, table, entries, q, heads, dim, 0.05, plain=plain_kernel)
+        check_attention(got, q, pool, table[rows], at_its_end, heads, 0.05, torch.bfloat16)
+        assert (attend(pool, table, entries, q, heads, dim, 0.05, window=1, plain=plain_kernel) == 0).all()
