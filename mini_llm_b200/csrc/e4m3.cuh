@@ -7,6 +7,8 @@
 
 #include <limits.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 constexpr int E4M3_BLOCK = 16;                 // positions that share a scale
@@ -78,14 +80,15 @@ __device__ __forceinline__ float capped(float x, float cap, float two_log2e_over
     return cap - 2.0f * cap * r;
 }
 
-// Raises a kernel's limit of dynamic shared memory to `bytes`, once on each device (`raised`: of this kernel, what each device's limit is).
+// Raises a kernel's limit of dynamic shared memory, once on each device (`raised`), to the `most` that any launch of it takes: threads that come here at the
+// same time set the same limit, whatever the sizes of their calls.
 template <typename Kernel>
-static cudaError_t raise_shared_limit(Kernel kernel, size_t bytes, size_t (&raised)[64]) {
+static cudaError_t raise_shared_limit(Kernel kernel, size_t most, std::atomic<bool> (&raised)[64]) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess || (device < 64 && raised[device] >= bytes)) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess && device < 64) raised[device] = bytes;
+    if (e != cudaSuccess || (device < 64 && raised[device])) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e == cudaSuccess && device < 64) raised[device] = true;
     return e;
 }
 

@@ -925,10 +925,10 @@ extern "C" int mllm_e4m3_tiles_attention(const E4m3Attention* p, int n_rows, int
     const int groups = p->dim <= 64 && p->vdim <= 64 ? 1 : 2, stages = groups == 1 ? 4 : 2;
     const size_t bytes = 1024 + (size_t)(2 + 2 * stages) * groups * GROUP_BYTES;
     const int which = (p->cap > 0.0f ? 2 : 0) + groups - 1;
-    static size_t raised[4][64];
+    static std::atomic<bool> raised[4][64];
     auto kernel = which == 0 ? attention_tiles_kernel<false, 1> : which == 1 ? attention_tiles_kernel<false, 2>
                 : which == 2 ? attention_tiles_kernel<true, 1> : attention_tiles_kernel<true, 2>;
-    static bool suffices[4];
+    static std::atomic<bool> suffices[4];
     if (!suffices[which]) {
         cudaFuncAttributes attributes;
         const cudaError_t e = cudaFuncGetAttributes(&attributes, kernel);

@@ -853,10 +853,11 @@ int launch_step(const E4m3Attention& p, int n_sms, cudaStream_t stream) {
     const int stage_bytes = 128 + E4M3_BLOCK * (p.dim + p.vdim), of_all = STEP_WARPS * stage_bytes;
     const int stages = of_all * 6 <= STEP_RING_BYTES ? 6 : of_all * 4 <= STEP_RING_BYTES ? 4 : 3;
     const size_t bytes = max((size_t)stages * of_all, STEP_WARPS * rows * (64 * VG + 2) * sizeof(float));
-    static_assert(STEP_WARPS * 16 * (128 + 2) * 4 <= 100 * 1024 && 3 * STEP_WARPS * (128 + 16 * 256) <= 104 * 1024, "two CTAs of the largest size share an SM");
+    constexpr size_t MOST = 3 * STEP_WARPS * (128 + E4M3_BLOCK * 256);
+    static_assert(MOST <= 104 * 1024 && STEP_RING_BYTES <= MOST && STEP_WARPS * 16 * (128 + 2) * 4 <= MOST, "two CTAs of the largest size share an SM");
     auto kernel = attention_step_kernel<KG, VG, TILES, EXACT>;
-    static size_t raised[64];
-    const cudaError_t e = raise_shared_limit(kernel, bytes, raised);
+    static std::atomic<bool> raised[64];
+    const cudaError_t e = raise_shared_limit(kernel, MOST, raised);
     if (e != cudaSuccess) return launched(e, "e4m3_attention_step");
     // as many CTAs as the SMs hold, or as the longest row that the tables allow is cut into
     const long units = (long)p.n_items * p.n_kv_heads * head_tiles, most = (long)p.max_blocks * (p.page / E4M3_BLOCK);

@@ -815,3 +815,50 @@ def test_walks_end_where_the_block_table_does(start):
         got = attend(pool, table, entries, q, heads, dim, 0.05, plain=plain_kernel)
         check_attention(got, q, pool, table[rows], at_its_end, heads, 0.05, torch.bfloat16)
         assert (attend(pool, table, entries, q, heads, dim, 0.05, window=1, plain=plain_kernel) == 0).all()
+
+
+def test_first_calls_of_several_threads_at_once():
+    """Heads of several sizes that share kernels, each thread on a stream and with a workspace of its own, in a process that has made no such call: what the
+    calls set once must suffice for all of them."""
+    code = '''
+import threading
+import torch
+from mini_llm_b200.kernels import ops
+SIZES = [(16, 16), (80, 16), (128, 112), (96, 96), (16, 64), (64, 64), (128, 128), (48, 48)]
+work = []
+for i, (dim, vdim) in enumerate(SIZES * 3):
+    heads = (1, 12, 16)[i % 3]
+    generator = torch.Generator(device="cuda").manual_seed(i)
+    k, v = (torch.randint(0, 120, (60, 1, 32, size), generator=generator, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for size in (dim, vdim))
+    scales = torch.full((60, 1, 2), 2.0 ** -7, device="cuda")
+    q = torch.randn((201, heads * dim), generator=generator, device="cuda").bfloat16()
+    ints = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 1], [1, 200], [900, 700])]
+    table = torch.randperm(60, generator=generator, device="cuda").to(torch.int32).view(2, 30)
+    out = torch.zeros((201, heads * vdim), dtype=torch.bfloat16, device="cuda")
+    work.append((out, q, k, v, scales, scales, table, *ints, heads, 1, 0.01))
+spaces = [ops.e4m3_workspace("cuda", vdim) for _, vdim in SIZES * 3]
+torch.cuda.synchronize()
+start, errors = threading.Barrier(len(work)), []
+def call(args, space):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            ops.e4m3_attention(*args, workspace=space)
+            torch.cuda.current_stream().synchronize()
+    except Exception as error:
+        errors.append(error)
+threads = [threading.Thread(target=call, args=pair) for pair in zip(work, spaces)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not errors, errors
+for args, space in zip(work, spaces):
+    got = args[0].clone()
+    ops.e4m3_attention(*args, workspace=space)
+    assert torch.equal(args[0], got) and int(space.status) == 0 and bool(got.abs().sum() > 0)
+'''
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert done.returncode == 0, done.stderr[-2000:]
