@@ -12,7 +12,6 @@
 #include "common.cuh"
 
 constexpr int E4M3_BLOCK = 16;                 // positions that share a scale
-constexpr float E4M3_TOP = 448.0f;             // the largest code
 constexpr int E4M3_LEAST_EXPONENT = -64;       // of a scale
 
 // Two numbers to two codes, nearest, ties to even; beyond 448 to 448, what is no number to the code that is none.
