@@ -2096,7 +2096,7 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
     if not fits:
         _check_e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, inv_freq, amplitude, positions, token_item, block_table,
                           k_pages, v_pages, k_scales, v_scales, writes)
-        if not known:
+        if not known or n > 1:                     # (the two differ in the strides of a lone row, which do not matter)
             raise KernelError("e4m3_store: operands of other kinds than it takes")
     params = _e4m3_rows(q_at, ld_q, at, ld, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, freq_at, amplitude, positions.data_ptr(),
                         token_item.data_ptr(), table_at, max_blocks, n_pages, page, *pages, n)
@@ -2197,7 +2197,7 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
     if not fits:
         _check_e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, item_offset, item_count, item_start, heads, kv_heads, scale,
                               cap, window)
-        if not known:
+        if not known or n_rows > 1:                # (as in e4m3_store)
             raise KernelError("e4m3_attention: operands of other kinds than it takes")
     fast = not plain and dtype is _BF16 and dim <= E4M3_FAST_SIZES and vdim <= E4M3_FAST_SIZES
     if fast:

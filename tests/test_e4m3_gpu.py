@@ -862,3 +862,76 @@ for args, space in zip(work, spaces):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ---- what the calls ask of their operands ----------------------------------------------------------
+
+def _changes(value):
+    """Other operands in the place of one: other types, shapes, strides, devices, alignments and numbers."""
+    if isinstance(value, torch.Tensor):
+        yield from (value.cpu(), value[:-1], value[:0], value[None], value.reshape(-1), list(value.shape), None)
+        for dtype in (torch.int32, torch.int64, torch.float32, torch.float64, torch.bfloat16, torch.float16, torch.uint8, torch.float8_e4m3fn):
+            if dtype != value.dtype:
+                yield torch.zeros(value.shape, dtype=torch.float32, device="cuda").to(dtype)
+        for d in range(value.dim()):
+            shape = list(value.shape)
+            shape[d] *= 2
+            longer = torch.zeros(shape, dtype=torch.float32, device="cuda").to(value.dtype)
+            yield longer
+            yield longer[tuple(slice(None, None, 2) if i == d else slice(None) for i in range(value.dim()))]           # every second
+            shape[d] = value.shape[d] + 1
+            yield torch.zeros(shape, dtype=torch.float32, device="cuda").to(value.dtype)[
+                tuple(slice(1, None) if i == d else slice(None) for i in range(value.dim()))]                           # from the second on
+    elif isinstance(value, int):
+        yield from (0, 1, -1, 2, 3, 16, 17, 48, 256, 272, 10 ** 6, 2 ** 31)
+    else:
+        yield from (0, 1, -1, 0.5, -0.5, 2.0 ** 127, 2.0 ** -140, 1e39, float("inf"), -float("inf"), float("nan"))
+
+
+@pytest.mark.parametrize("rows", [0, 1, 4])
+def test_what_is_refused_is_refused_by_both_checks(rows, monkeypatch):
+    """The calls ask everything in one expression, and again one by one for the error's text.  With one operand changed, a ``KernelError`` is raised, and
+    nothing launched, where the second finds fault, and only there; but for a lone row's strides, which do not matter, the first finds it in the same cases."""
+    from mini_llm_b200.kernels import ops
+    from mini_llm_b200.kernels.lib import KernelError
+    pool = Pool(3, 2, 32, 64, 48)
+    kp, vp, ks, vs = pool.operands
+    table, workspace = ints([[0, 1]]), ops.e4m3_workspace("cuda", 64)
+    q, out = torch.zeros((rows, 4 * 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((rows, 4 * 48), dtype=torch.bfloat16, device="cuda")
+    attention = dict(out=out, q=q, k_pages=kp, v_pages=vp, k_scales=ks, v_scales=vs, block_table=table, item_offset=ints([0]), item_count=ints([rows]),
+                     item_start=ints([0]), heads=4, kv_heads=2, scale=0.1, cap=0.0, window=0)
+    qkv = torch.zeros((rows, 4 * 64 + 2 * (64 + 48)), dtype=torch.bfloat16, device="cuda")
+    store = dict(q_out=q, qkv=qkv, k_off=256, v_off=384, heads=4, kv_heads=2, dim=64, vdim=48, rot_dims=32,
+                 inv_freq=torch.ones(16, dtype=torch.float64, device="cuda"), amplitude=1.0, positions=ints(range(rows)), token_item=ints([0] * rows),
+                 block_table=table, k_pages=kp, v_pages=vp, k_scales=ks, v_scales=vs)
+    launched, asked, cases = [], [], 0
+    monkeypatch.setattr(ops, "_launch_on", lambda *args: launched.append(args))
+    for call, check, good, more in ((ops.e4m3_attention, ops._check_e4m3_attention, attention, dict(workspace=workspace)),
+                                    (ops.e4m3_store, lambda **o: check_store(**o, writes=True), store, {})):
+        check_store = ops._check_e4m3_store
+        of_call = getattr(ops, f"_check_{call.__name__}")
+        monkeypatch.setattr(ops, f"_check_{call.__name__}", lambda *args, of_call=of_call: (asked.append(args), of_call(*args)))
+        launched.clear(), asked.clear()
+        call(**good, **more)
+        assert launched and not asked
+        for name, value in good.items():
+            for other in _changes(value):
+                if name == "q_out" and other is None:
+                    continue                                    # (no queries wanted)
+                operands, what = {**good, name: other}, (name, getattr(other, "shape", other), getattr(other, "dtype", None))
+                launched.clear()
+                try:
+                    check(**operands)
+                    fault = False
+                except KernelError:
+                    fault = True
+                asked.clear()
+                try:
+                    call(**operands, **more)
+                    refused = False
+                except KernelError:
+                    refused = True
+                assert refused == fault and bool(launched) != refused, what
+                assert bool(asked) == fault or (rows <= 1 and asked), what
+                cases += 1
+    assert cases > 300
