@@ -71,6 +71,14 @@ class CompositeLayerCache(LayerCache):
         return CompositeLayerCache({role[len(head):]: view for role, view in self.by_role.items() if role.startswith(head)})
 
 
+def check_e4m3_sizes(need: PagedKV, page_size: int) -> None:
+    """Raises if pages in 8 bits do not take a part's keys and values."""
+    value_size = need.value_size or need.head_size
+    if not need.has_values or not ops.e4m3_sizes_take(need.head_size, value_size, page_size):
+        raise ValueError(f"a cache in 8 bits takes keys and values of 16 to 256 entries and pages, all multiples of 16, not heads of "
+                         f"{need.head_size} and {value_size if need.has_values else 'no'} entries in pages of {page_size}")
+
+
 class CacheStorage:
     def __init__(self, manager, order, dtype: torch.dtype, device, max_items: int, poison: float | None = None, e4m3: bool = False):
         """``poison``: a debugging value.  Every page slot holds it until a token is stored
@@ -151,10 +159,8 @@ class CacheStorage:
 
     def _make_e4m3(self, group, n_entries: int, device) -> None:
         need, page = group.need, self.manager.page_size
+        check_e4m3_sizes(need, page)
         value_size = need.value_size or need.head_size
-        if not need.has_values or not ops.e4m3_sizes_take(need.head_size, value_size, page):
-            raise ValueError(f"a cache in 8 bits takes keys and values of 16 to 256 entries and pages, all multiples of 16, not heads of "
-                             f"{need.head_size} and {value_size if need.has_values else 'no'} entries in pages of {page}")
         shape = (n_entries, group.pool.n_pages + 1, need.n_kv_heads, page)
         code = 0 if self.poison is None else ops.E4M3_NONE
         for pages, scales, size in ((self.keys, self.key_scales, need.head_size), (self.values, self.value_scales, value_size)):

@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from ..cache.manager import CacheManager
-from ..cache.storage import CacheStorage
+from ..cache.storage import CacheStorage, check_e4m3_sizes
 from ..config.registry import config_from_folder, describe_model
 from ..kernels import ops
 from ..kernels.lib import KernelError
@@ -85,7 +85,7 @@ class Engine:
         self.spec = describe_model(self.config)
         self.model = Model(self.spec)
         if cache_dtype is not None:
-            self._check_e4m3()
+            self._check_e4m3(int(page_size))
         self.kernels = Kernels(self.dtype, plain_only=plain_kernels)
         self.model.load(model_dir, self.dtype, self.device, runtime=self)
         self.page_size = int(page_size)
@@ -142,11 +142,15 @@ class Engine:
         self._status_host = self._status_pinned.numpy()
         self.hidden_dump = None               # set by step(dump_hidden=True): the residual stream after every run entry
 
-    def _check_e4m3(self) -> None:
-        """Raises if some part of the model keeps pages that it cannot store and read in 8 bits, before anything is loaded."""
+    def _check_e4m3(self, page_size: int) -> None:
+        """Raises if some part of the model keeps pages that it cannot store and read in 8 bits, or of sizes that they do not come in,
+        before anything is loaded."""
         for part in self.model.parts():
-            if isinstance(part, Mixer) and not part.takes_e4m3_cache():
-                raise ValueError(f"{part.prefix}: {type(part).__name__} does not store and read a cache in 8 bits (cache_dtype='e4m3')")
+            if isinstance(part, Mixer):
+                if not part.takes_e4m3_cache():
+                    raise ValueError(f"{part.prefix}: {type(part).__name__} does not store and read a cache in 8 bits (cache_dtype='e4m3')")
+                for need in part.paged_needs():
+                    check_e4m3_sizes(need, page_size)
         # its attention makes out the prompt portions on the device: no work list is made for it
         self.model.wants_attention_tiles = False
 

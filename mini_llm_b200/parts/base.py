@@ -80,8 +80,12 @@ class Mixer(Part):
 
     def takes_e4m3_cache(self) -> bool:
         """Whether the part stores and reads pages in 8 bits, should the engine hold them so; one that keeps no pages does not mind."""
+        return not self.paged_needs()
+
+    def paged_needs(self) -> list:
+        """Of what the part keeps, that which lies in pages."""
         need = self.cache_need()
-        return not any(isinstance(one, PagedKV) for one in (need.values() if isinstance(need, dict) else (need,)))
+        return [one for one in (need.values() if isinstance(need, dict) else (need,)) if isinstance(one, PagedKV)]
 
     def forward(self, ctx, x, hidden, cache):
         raise NotImplementedError

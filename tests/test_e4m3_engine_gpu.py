@@ -231,3 +231,24 @@ def test_a_step_whose_kernel_gave_up_is_reported_and_later_steps_are_right(folde
         for a, b in zip(logits(), want):
             np.testing.assert_array_equal(a, b)
     engine.check_status()
+
+
+def test_sizes_are_refused_before_weights_are_looked_for(folders, tmp_path):
+    import json
+    import os
+    import shutil
+    from mini_llm_b200.engine import Engine
+    bare = str(tmp_path / "gpt2")
+    os.makedirs(bare)
+    shutil.copy(os.path.join(folders["A"], "config.json"), bare)                                       # (no weights)
+    for page in (8, 24, 40):
+        with pytest.raises(ValueError, match="multiples of 16"):
+            Engine(bare, page_size=page, cache_dtype="e4m3")
+    h = sumozen_helpers
+    for i, mixer in enumerate((h.parallel(dim=16, vdim=24), h.parallel(dim=8, vdim=16, rot_dims=8))):
+        folder = str(tmp_path / f"sumozen{i}")
+        os.makedirs(folder)
+        with open(os.path.join(folder, "config.json"), "w") as handle:
+            json.dump(h.config([h.mamba(), mixer]), handle)
+        with pytest.raises(ValueError, match="multiples of 16"):
+            Engine(folder, page_size=16, cache_tokens=256, cache_dtype="e4m3")
