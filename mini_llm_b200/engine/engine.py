@@ -291,6 +291,7 @@ class Engine:
         ctx = self.ctx
         cache_length = self.cache.length
         decode_only = n_tokens == n_items
+        # (of requests: a filler of one token, below, need not be read for: its row keeps finite numbers of an earlier step and is nobody's)
         ctx.lone_tokens = not decode_only and any(len(e.tokens) == 1 for e in entries)
         slots = ctx.item_slots = [e.slot for e in entries]
         starts = ctx.item_starts = [cache_length(slot) for slot in slots]

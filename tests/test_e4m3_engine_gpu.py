@@ -233,6 +233,30 @@ def test_a_step_whose_kernel_gave_up_is_reported_and_later_steps_are_right(folde
     engine.check_status()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_sumozen_with_experts_over_a_cache_in_8_bits(tmp_path, dtype, monkeypatch):
+    """Every token takes all experts, so that no token lies between two of them; steps are filled up to round shapes with tokens of no request, which
+    read pages of the poison and go through the router and the experts with what that makes of them."""
+    from mini_llm_b200.engine import Engine
+    h = sumozen_helpers
+    raw = h.config([h.parallel(dim=16, vdim=32, scale=0.2, mlp=h.moe(experts=4, top=4)), h.mamba(mlp=None),
+                    h.parallel(heads=6, kv_heads=2, dim=64, vdim=64, rot_dims=64, scale=0.1, softcap=None, mlp=h.moe(experts=3, top=3, shared=None))])
+    folder = h.make_model(str(tmp_path / "model"), raw, seed=9, bfloat16_values=True)
+    requests = {"a": random_tokens(1, 150, raw["vocab"]), "b": random_tokens(2, 40, raw["vocab"]), "c": random_tokens(3, 17, raw["vocab"])}
+    engine = Engine(folder, dtype=dtype, page_size=32, cache_tokens=1024, max_requests=4, cache_dtype="e4m3", debug_poison=True)
+    assert engine._can_pad
+    for kind, steps in schedules(requests).items():
+        for again in range(2):                                # (the second time captured steps are replayed)
+            got, held = drive(engine, requests, steps, [0, 2])
+            for name, tokens in requests.items():
+                want, _ = sumozen_over(folder, tokens, held[name], monkeypatch)
+                if dtype == "bfloat16":
+                    # (the bound of these stacks in bfloat16, as above)
+                    assert np.sqrt(((got[name] - want) ** 2).mean()) <= 0.04 * want.std(), (kind, name)
+                else:
+                    assert np.abs(got[name] - want).max() <= F32_BOUND, (kind, name)
+
+
 def test_sizes_are_refused_before_weights_are_looked_for(folders, tmp_path):
     import json
     import os
