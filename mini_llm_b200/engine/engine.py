@@ -70,7 +70,7 @@ class Engine:
         ``cache_dtype``: how the paged keys and values are held: None as ``dtype`` says, "e4m3" in 8
         bits with a scale for each block of 16 tokens and head (a page is then half as many bytes as in
         bfloat16; the model's attention must be of a kind that reads such pages, and ``page_size`` a
-        multiple of 16)."""
+        multiple of 16).  How a request is cut into steps then shows in the rounding of its smallest entries."""
         if not torch.cuda.is_available():
             raise RuntimeError("mini_llm_b200 runs on a CUDA device (sm_100a) only; none is available "
                                "and there is no CPU path")
@@ -269,7 +269,9 @@ class Engine:
         embedding and after every run entry (a test hook, as the reference's per-layer
         outputs of ``gpt2_gpu_forward_last``, engine/src/gpt2_gpu.cu:224-250).  A step
         that fails after its check (out of pages, a kernel that reports an error) leaves
-        every request as it was."""
+        every request as it was; over a cache in 8 bits, where its kernels ran, but for the scale
+        of a request's last block, which its tokens may have raised (the smallest of the
+        block's codes are then rounded again; the same step again gives what it would have given)."""
         ids = self._validate(entries)
         n_want = sum(len(e.want) for e in entries)
         if sampling is not None and len(sampling) != n_want:

@@ -21,7 +21,9 @@ pages and mixed batches:
 * a request that cannot fit even alone fails with "out of pages".
 
 Sampling uses (seed, number of tokens generated so far) per request, so a
-request's tokens depend neither on its batch nor on preemption.
+request's tokens depend neither on its batch nor on preemption, but for rounding:
+a request that is run again, or cut into other portions, meets other kernels, and
+over a cache in 8 bits codes that were rounded at other scales on their way.
 
 With ``run_ahead`` the scheduler launches a step before it has read the tokens
 of the step before: a decoding request's entry names its token as ``PREVIOUS``

@@ -276,3 +276,52 @@ def test_sizes_are_refused_before_weights_are_looked_for(folders, tmp_path):
             json.dump(h.config([h.mamba(), mixer]), handle)
         with pytest.raises(ValueError, match="multiples of 16"):
             Engine(folder, page_size=16, cache_tokens=256, cache_dtype="e4m3")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_preempted_requests_are_right_over_what_the_cache_holds_each_time(folders, dtype):
+    """So few pages that decoding requests are preempted and their tokens run again as a prompt, which stores them in other steps than before.  Whenever a
+    request is closed, preempted or at its end, what the cache held of it is that of its tokens, and its logits are the plain ones over that;
+    every token is the largest of its logits."""
+    from mini_llm_b200.generate import LLM
+    raw = CONFIGS["D"][0]
+    prompts = [random_tokens(30 + i, n, raw["vocab_size"]) for i, n in enumerate((90, 60, 75))]
+    llm = LLM(folders["D"], dtype=dtype, cache_dtype="e4m3", page_size=16, cache_tokens=272, max_sessions=3, run_ahead=False)
+    engine, of_slot, closed = llm.engine, {}, []
+    step, close = engine.step, engine.close_request
+
+    def recorded_step(entries, *args, **how):
+        logits = step(entries, *args, **how)
+        rows = iter(logits.cpu().numpy() if logits is not None else ())
+        for entry in entries:
+            tokens, seen = of_slot.setdefault(entry.slot, ([], {}))
+            for place in entry.want:
+                seen[len(tokens) + place] = next(rows)
+            tokens.extend(int(t) for t in entry.tokens)
+        return logits
+
+    def recorded_close(slot):
+        if slot in of_slot:
+            closed.append((*of_slot.pop(slot), [tuple(x.double().cpu().numpy() for x in engine.read_kv(slot, layer)) for layer in range(raw["n_layer"])]))
+        close(slot)
+
+    engine.step, engine.close_request = recorded_step, recorded_close
+    got = llm.generate(prompts, max_new_tokens=40)
+    preemptions = llm.scheduler.stats()["preemptions"]
+    assert preemptions >= 1 and len(closed) == 3 + preemptions
+    chosen = [{} for _ in prompts]
+    for tokens, seen, held in closed:
+        which = [i for i, prompt in enumerate(prompts) if tokens[:len(prompt)] == list(prompt)]
+        assert len(which) == 1 and tokens == (list(prompts[which[0]]) + got[which[0]])[:len(tokens)]
+        want, layers = gpt2_over(folders["D"], tokens, held, dtype == "bfloat16")
+        atol = F32_BOUND if dtype == "float32" else bf16_atol(want)
+        for position, logits in seen.items():
+            assert np.abs(logits - want[position]).max() <= atol, position
+            chosen[which[0]][position + 1 - len(prompts[which[0]])] = int(logits.argmax())
+        for (k8, v8), (k, v) in zip(held, layers):
+            for codes, rows in ((k8, k), (v8, v)):
+                check_held([codes.reshape(len(rows), -1)], [rows], 1e-4 if dtype == "float32" else 0.04 * np.abs(rows).max())
+    for tokens, of_request in zip(got, chosen):
+        assert tokens == [of_request[i] for i in range(40)]
+    assert engine.cache.pages_in_use() == [0]
+    engine.cache.check()
