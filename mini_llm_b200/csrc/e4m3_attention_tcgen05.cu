@@ -43,8 +43,10 @@ constexpr bool registers_suffice(int at_launch) {
 }
 constexpr int MAX_STAGES = 4;
 constexpr int MIN_STRETCH = 5;                     // of a CTA, where no unit is longer: its blocks and one more
-constexpr int MIN_STRETCH_APART = 3;               // the same where every unit is cut by itself, in blocks (prompts of 300 and 700 tokens, 12 heads of
-                                                   // 64: 2 15.8 and 19.7 us, 3 13.8 and 22.2; one row for all units 22.6 and 26.3)
+constexpr int MIN_STRETCH_APART = 4;               // the same where every unit is cut by itself, in blocks (prompts of 300, 400, 500, 700 and 1,000 tokens, 12 heads
+                                                   // of 64: 2 14.5, 16.5, 17.4, 18.5, 21.3 us; 3 12.2, 19.6, 20.3, 20.5, 21.3; 4 12.2, 16.0, 16.6, 21.6,
+                                                   // 22.0; 5 12.2, 16.0, 16.6, 24.4, 24.8; of 300, 400 and 500, 32 heads of 128: 2 20.3, 26.7, 28.4; 3 15.6,
+                                                   // 26.7, 28.5; 4 15.6, 20.6, 21.3)
 constexpr float LOG2E = 1.4426950408889634f;
 
 // What one thread of the MMA warp does while all of its lanes run: a warp that does not branch apart keeps descriptors where the
