@@ -8,12 +8,12 @@
 //   softmax warps    two threads a row, each with 64 of a block's columns: read S, apply scale, cap and mask, write P as 16-bit floats; and, since they have
 //                    nothing else to do at a unit's start, its queries.
 // While one tile's softmax runs the other's products do.  Scales cost nothing an entry: a block of 16 keys has one factor for its scores, and
-// its values' scale 2^t goes into the exponent, p = 2^(s + t - m + 7), with the sum of the weights getting p / 2^t; p keeps the 11 bits of a
-// 16-bit float however far apart the scales lie.  Queries are scaled by a power of two to lie below 2^15.  O stays in tensor
+// its values' scale 2^t goes into the exponent, p = 2^(s + t - m + 7), with the sum of the weights getting p / 2^t in 32 bits; p, a weight times its value's
+// scale, is a 16-bit float: 11 bits down to 2^-21 of the row's largest, below an error of 2^-32 of the largest, times a code of 448 at most.  Queries are scaled by a power of two to lie below 2^15.  O stays in tensor
 // memory; m moves, and O is scaled down, only where a score passes m by 8 (p stays below 2^15).
 //
 // A unit and block takes the exponential's unit 2,048 clocks (16 a clock and SM), the tensor cores 1,024 with heads of 64 and 2,048 with 128, and reads
-// next to nothing from memory.  It takes 4,250 clocks with heads of 64 (a prompt of 16,000 tokens, 12 heads: 732 us, half of the exponential's rate) and
+// next to nothing from memory.  It takes 4,250 clocks with heads of 64 (a prompt of 16,000 tokens, 12 heads: 738 us, half of the exponential's rate) and
 // 5,250 with 128 (2,000 tokens behind 14,000, 32 heads: 577 us, 0.87 PFLOP/s): what lies between is the chain of a tile's turn, S, its largest, the
 // tile's meeting, the weights, P, which the other tile's turn fills in part, and the instruction fetch of four roles at once.  Without exponentials,
 // largest and conversion the chain alone still took 667 us of 766 in an earlier state.
@@ -35,7 +35,7 @@ constexpr int GROUP_BYTES = TILE * 128;            // 128 rows of 64 16-bit floa
 constexpr int SOFTMAX_WARPS = 16, CONVERTER_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + CONVERTER_WARPS;
 constexpr int THREADS = (MMA_WARP + 4) * 32;       // (the last two warps only make the fourth warp of their group up)
 // Registers a thread: all start with the same, and the last four warps, which need few, give up what the softmax warps take.  The shares never add up
-// to more than the block was launched with (`registers_suffice`).  790 us for 16,000 tokens of 12 heads of 64 without, 766 with it.
+// to more than the block was launched with (`registers_suffice`).  When it was brought in: 790 us for 16,000 tokens of 12 heads of 64 without, 766 with it.
 constexpr int SOFTMAX_REGISTERS = 88, IDLE_REGISTERS = 48;
 constexpr bool registers_suffice(int at_launch) {
     return THREADS / 32 * at_launch >= SOFTMAX_WARPS * SOFTMAX_REGISTERS + CONVERTER_WARPS * at_launch + 4 * IDLE_REGISTERS && at_launch >= IDLE_REGISTERS &&
@@ -258,7 +258,7 @@ constexpr int CONVERTERS_GAVE_UP = 31, PRODUCTS_GAVE_UP = 33, SOFTMAX_GAVE_UP = 
 // (a role that gave up leaves its barriers as they are; the others find out here)
 // By a whole warp, with one answer for all of its lanes: what follows does not branch apart, and the compiler knows it.  Code that is seldom reached
 // is kept out of the way here and in the softmax: 24 warps in four roles share the instruction caches, and what they fetch past, they wait for
-// (766 us and 612 us for 2,000 tokens at the end of 16,000 of 32 heads of 128 with all of it in line; 704 and 574 this way).
+// (when it was brought in: a prompt of 16,000 766 us and 2,000 tokens at its end of 32 heads of 128 612 us with all of it in line, 704 and 574 this way).
 __device__ __forceinline__ bool wait_or_fail(Shared& sh, uint64_t* bar, uint32_t parity) {
     if (__builtin_expect(__any_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
     const uint32_t start = (uint32_t)now_ns();       // (32 bits of it: looks lie microseconds apart, and the limit is below 2^31)
@@ -343,7 +343,8 @@ __device__ __forceinline__ float never_zero(float factor) { return fmaxf(factor,
 
 // 32 products (two blocks of 16 keys) to capped scores.  Up to a quarter of the cap, where scores mostly lie, by the series of tanh u / u in u^2 to its
 // third power (the next term is 2^-23.5 of the cap there): otherwise the exponential's unit, which the weights need, has two more operations a score (a
-// portion of 1,024 behind 1,345 and two short prompts, 12 heads of 64: 48.0 us, and 41.3).
+// portion of 1,024 behind 1,345 and two short prompts, 12 heads of 64: 48.0 us, and 41.3).  One score beyond sends a warp's 32 rows the other way: a prompt of
+// 8,000 takes 208 us without a cap, 311 with scores below a quarter of it and 390 with scores far beyond.
 __device__ __forceinline__ void cap_scores(uint32_t (&v)[32], float q_factor, const float* k_scale, float cap_log2, float cap_factor, float by_cap) {
     float far = 0.0f;
 #pragma unroll

@@ -21,7 +21,8 @@ namespace {
 // maximum, raises the codes that are there already where it must, and writes the new ones: no two warps touch a block, and
 // a step that is run again leaves the same bytes.  A CTA takes G rows and the blocks that begin in them, and a share of the heads; its
 // table of cosines and sines serves all of them.  What bounds it is bytes, rows once in, codes and queries once out, for long
-// portions (8,192 rows of 6,144 columns: 54 us, 3.4 TB/s), and the chain of positions, page and rows for single tokens (2.9 us).
+// portions (8,192 rows of 6,144 columns: 53 us, 3.5 TB/s: a lane has two pieces of 16 bytes on their way, and keys and values are walked twice), and the chain
+// of positions, page and rows for single tokens (2.9 us).
 constexpr int STORE_THREADS = 256, STORE_ROWS = 16;
 
 // Eight numbers of a row, as they lie in memory.
@@ -96,7 +97,7 @@ __device__ __forceinline__ uint32_t largest_square(float (&x)[8], int first, int
 
 // A lane's pieces of eight columns of rows side by side, every 32nd, row by row: `act(row, column, numbers)` for each, the next one on its way
 // (the compiler cannot know that what is stored is none of what is loaded).  One body, not unrolled: a kernel this short waits for its own
-// instructions, and four pieces at a time were slower (64 rows 4.5 and 6.1 us, 8,192 rows 50 and 58).
+// instructions, and four pieces at a time were slower (when it was brought in: 64 rows 4.5 and 6.1 us, 8,192 rows 50 and 58).
 template <typename T, typename Act>
 __device__ __forceinline__ void each_piece(const T* from, long pitch, int rows, int columns, int lane, Act act) {
     const int chunks = columns / 8, step_rows = 32 / chunks, step_cols = 32 % chunks * 8;
@@ -362,8 +363,10 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attention_plain_kernel(const E4
 // ring is divided for.  Half of the issue slots and of the integer unit's, which converts codes, are taken then, with 16 warps an SM.)
 // Q is scaled by a power of two to lie below 2^15 in 16-bit floats (11 bits: bfloat16's 8 fit; an entry 2^29 below the largest of its head
 // begins to lose some, where the 32-bit sum has lost it already).  The weights: a block's value scale 2^t joins the score as t in
-// the exponent, p = 2^(s + t - m + 7), and the sum of the weights gets p / 2^t: no multiplication more, and p keeps the 11 bits of a 16-bit
-// float however far apart the scales lie.  m moves only where a score passes it by 8, so that p stays below 2^15.
+// the exponent, p = 2^(s + t - m + 7), and the sum of the weights gets p / 2^t, in 32 bits: no multiplication more.  m is the largest s + t (and moves
+// only where a score passes it by 8, so that p stays below 2^15): a weight times its value's scale has 11 bits down to 2^-21 of the row's largest, and
+// below that an error of 2^-32 of the largest, times a code of 448 at most.  (Weights as three terms of 8 bits, as for 16-bit pages, would be three
+// products; a code has 4 bits.)
 constexpr int STEP_WARPS = 8, STEP_THREADS = STEP_WARPS * 32, STEP_CTAS = 2;
 constexpr int STEP_SET_UP = 28;                // blocks that a unit's set-up counts as (64 requests of 100 to 4,000 tokens, 8 heads of 128: 16 as many
                                                // 42.1 us, 20 39.2, 24 38.7, 28 38.3, 34 38.8)

@@ -2060,7 +2060,9 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
     positions is the least power of two s >= 2^-64 with n <= (448 s)^2 for all its rows so far, n being x^2 + y^2 of a pair that turns (its entries
     times ``amplitude``; a turn keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
     row that begins a block begins it anew, whatever was there.  A key or value head with an n that is not finite is stored as
-    NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes."""
+    NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes; the same rows in other steps may leave
+    other smallest codes, since raised ones are rounded twice.  An angle is taken as a 64-bit fraction of a turn and given to cosine and sine to
+    2^-28 of a turn, which are 32-bit numbers to a unit or two of their last place."""
     n_pages = page = max_blocks = ld_q = 0
     q_at = freq_at = table_at = 0
     pages = _NO_PAGES
@@ -2168,14 +2170,19 @@ def e4m3_attention(out, q, k_pages, v_pages, k_scales, v_scales, block_table, it
     [T, heads * dim]) and ``out`` [T, heads * vdim], at positions ``item_start[i]``, ... of the request in row i of the block table, whose
     keys and values are stored up to there; entries have rows of their own within ``q``, and rows of no entry stay as they are.  A stored
     head is NaN throughout or nowhere and a scale a power of two from 2^-64 on, as ``e4m3_store`` leaves them.  score = q . k * ``scale``, with
-    ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if given; softmax and the weighted sum
-    in 32 bits; query head h reads key/value head h // (heads / kv_heads).  A row that sees no key (a negative position) is zero; pages that the table does not name are not seen.
+    ``cap`` cap * tanh(score / cap), over the keys at positions <= the query's, of those the last ``window`` if given; softmax, and the sum of the values by
+    its weights; query head h reads key/value head h // (heads / kv_heads).  A row that sees no key (a negative position) is zero; pages that the table does not name are not seen.
     The largest entry of a query head times ``scale`` times a visible block's scale stays below 2^112: beyond it a result may be NaN where 32-bit scores are not.
 
     ``longest=1``: the caller knows that no entry brings more than one token (one that does is left out: its rows stay as they are);
     ``singles=False``: that none brings just one (likewise).  Other values of ``longest`` change nothing.  ``workspace``
     (``e4m3_workspace``) is needed but with ``plain``: the kernel of every size and type, which 32-bit queries, and heads of more than 128
-    entries, take anyway."""
+    entries, take anyway.
+
+    Precision: the kernel of ``plain`` computes in 32 bits throughout.  The others, for bfloat16 heads of up to 128, sum in 32 bits, and give to their products
+    queries as 16-bit floats of a power of two's size (bfloat16's 8 bits, but for entries below 2^-29 of their head's largest) and weights times their
+    values' scale as 16-bit floats (11 bits down to 2^-21 of the row's largest, below that off by 2^-32 of it); 2^x is the hardware's, to 2^-22, and a capped
+    score is off by some 2^-22 of the cap: 2^-11 of the sum of the weighted |v| in all, and as much more as 2^-20 of the scores' sizes is of it."""
     try:
         index, dtype, (n_rows, columns), (ld_q, q_step), q_at = q.get_device(), q.dtype, q.shape, q.stride(), q.data_ptr()
         n_pages, held_heads, page, dim = k_pages.shape
