@@ -2061,8 +2061,8 @@ def e4m3_store(q_out, qkv, k_off, v_off, heads, kv_heads, dim, vdim, rot_dims, i
     times ``amplitude``; a turn keeps it) and x^2 of any other entry, in 32 bits; where new rows raise it, the codes that are there are rounded again.  A
     row that begins a block begins it anew, whatever was there.  A key or value head with an n that is not finite is stored as
     NaN throughout (e4m3 has no infinity) and does not count.  The same step again leaves the same bytes; the same rows in other steps may leave
-    other smallest codes, since raised ones are rounded twice.  An angle is taken as a 64-bit fraction of a turn and given to cosine and sine to
-    2^-28 of a turn, which are 32-bit numbers to a unit or two of their last place."""
+    other smallest codes, since raised ones are rounded twice.  An angle is a 64-bit fraction of a turn, its cosine and sine are
+    rounded to 32 bits as from 64."""
     n_pages = page = max_blocks = ld_q = 0
     q_at = freq_at = table_at = 0
     pages = _NO_PAGES

@@ -935,3 +935,24 @@ def test_what_is_refused_is_refused_by_both_checks(rows, monkeypatch):
                 assert bool(asked) == fault or (rows <= 1 and asked), what
                 cases += 1
     assert cases > 300
+
+
+def test_angles_are_those_of_64_bits():
+    """Queries (1, 0) turn into the cosine and sine themselves.  Their final rounding is half a unit, 2^-25; of a sine's series 0.081 r-cubed terms are off by four
+    roundings, 2^-25.6, and the angle by 2^-32 turns, 2^-29.3.  Nine in ten are the nearest 32-bit number (in a model of the series' arithmetic 96 of 100 are;
+    a 32-bit angle would leave 84 of 100 whatever the functions' own rounding)."""
+    from mini_llm_b200.kernels import ops
+    rng = np.random.default_rng(22)
+    n, half = 4000, 64
+    positions = rng.integers(0, 2 ** 20, n).astype(np.int32)
+    inv_freq = rng.uniform(0.1, 3.0, half)
+    qkv = torch.zeros((n, 2 * half + 2 * 16), device="cuda")
+    qkv[:, 0:2 * half:2] = 1.0
+    q = torch.empty((n, 2 * half), device="cuda")
+    ops.e4m3_store(q, qkv, 0, 2 * half, 1, 1, 2 * half, 16, 2 * half, torch.tensor(inv_freq, dtype=torch.float64, device="cuda"), 1.0, ints(positions),
+                   ints([0] * n), None, None, None, None, None, writes=False)
+    got = q.cpu().numpy().reshape(n, half, 2).astype(np.float64)
+    angle = positions.astype(np.longdouble)[:, None] * inv_freq.astype(np.longdouble)[None, :]
+    want = np.stack((np.cos(angle), np.sin(angle)), axis=-1)
+    assert float(np.abs(got - want).max()) <= 2.0 ** -25 + 2.0 ** -25.6 + 2.0 ** -29
+    assert (got.astype(np.float32) != want.astype(np.float32)).mean() <= 0.1
