@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tiles_kernel(const E4m3A
             const Blocks blocks(u);
             const int n = tile == 0 ? blocks.n[0] : blocks.n[1];
             // The tile's queries: the last unit's have been read for the last time (its last S was there), and there is nothing else to do before there are
-            // some.  (The converter warps took 11,000 clocks for them with heads of 128, ahead of a unit's first keys: a prompt of 100 tokens 9.8 us
+            // some.  (When it was brought in: the converter warps took 11,000 clocks for them with heads of 128, ahead of a unit's first keys: a prompt of 100 tokens 9.8 us
             // for 8.1, 500 behind 3,000 67 for 61.  Where units are many and long they had them ready ahead: 16,000 tokens 707 us for 732.)
             if (n > 0) {
                 put_queries<GROUPS>(p, u, q_tile, sh.q_factor, warp * (UNIT / SOFTMAX_WARPS), lane);

@@ -904,7 +904,7 @@ extern "C" int mllm_e4m3_store(const E4m3Store* operands, int dtype, int n_sms, 
     const int slots = (p.q_out != nullptr ? p.heads : 0) + (p.k_pages != nullptr ? 2 * p.kv_heads : 0);
     if (slots == 0) return 0;
     // Rows a CTA, and the heads shared among as many CTAs as fill the SMs.  Single tokens, of which each begins a block, want few rows a CTA,
-    // long portions many, whose angles are then made once (rows a CTA 4, 8, 16: a portion of 1,500 with shorter ones and 40 single tokens
+    // long portions many, whose angles are then made once (when it was brought in, rows a CTA 4, 8, 16: a portion of 1,500 with shorter ones and 40 single tokens
     // 10.5, 11.3, 15.9 us; 8,192 rows of 40 turned heads of 128 64.9, 55.8, 53.8).
     const int G = n <= 256 ? 1 : (n <= 4096 ? 4 : 16);
     const int groups = (n + G - 1) / G, warps = STORE_THREADS / 32;
